@@ -28,7 +28,10 @@ FUZZ_DIR = os.path.join(HERE, "_fuzz")
 SOURCES = ["capi.hip", "render.hip", "wgrad.hip", "adam.hip", "sampler.hip", "tile_adam.hip", "gridenc.hip", "pose.hip", "encodings.hip"]
 HEADERS = ["mne_device.h", "mne_launch.h", "mne_platform.h", "mlp_mfma.h"]
 
-HIPCC_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-munsafe-fp-atomics"]
+# -packed-fp32-ops: no v_pk_{add,mul,fma}_f32 in the device code (some of their forms have given wrong results now and then); the
+# host pass of hipcc does not know the feature and says so, which is harmless
+HIPCC_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-munsafe-fp-atomics",
+               "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 # name -> extra defines.  Only translation units that see RenderArgs change with MNE_ARGS_PAD; everything is rebuilt
 # anyway so that a variant is one self-contained library.
