@@ -28,7 +28,7 @@
 extern "C" {
 #endif
 
-#define MNE_ABI_VERSION 8
+#define MNE_ABI_VERSION 9
 
 /* orientation index of a plane triple, as in JointEncoding.all_planes (scene_rep.py:117) */
 enum { MNE_XY = 0, MNE_XZ = 1, MNE_YZ = 2 };
@@ -183,6 +183,19 @@ typedef struct mne_clock {
     uint64_t z_offset_stride;      /* mne_sample_z: counter offset used = offset + iteration used * z_offset_stride */
 } mne_clock_t;
 
+/* How an element is held in memory. */
+enum { MNE_T_F32 = 0, MNE_T_BF16 = 1, MNE_T_F16 = 2 };
+
+/* What the tensors of one mne_adamw_step call share. */
+typedef struct mne_adamw_cfg {
+    double lr, beta1, beta2, eps, weight_decay;
+    int32_t step;          /* 1-based */
+    int32_t state_bits;    /* 32: fp32 moments;  8: codes with two scales for each block of 256 elements */
+    int32_t p_type, g_type;/* MNE_T_*; a gradient has its parameter's type or fp32, and any type beside an fp32 parameter */
+    int32_t zero_grad;     /* != 0: the gradients are zero behind the call */
+    uint32_t seed;         /* 8-bit moments: of the dither that their codes are rounded with */
+} mne_adamw_cfg_t;
+
 /* ---- library ------------------------------------------------------------------------- */
 int mne_abi_version(void);
 const char* mne_last_error(void);
@@ -193,6 +206,9 @@ size_t mne_sizeof_tile_bins(void);
 size_t mne_sizeof_plane_opt(void);
 size_t mne_sizeof_clock(void);
 size_t mne_sizeof_fused_opts(void);
+size_t mne_sizeof_adamw_cfg(void);
+/* 1: this library runs its kernels on host memory (the test-only emulation), 0: on device memory. */
+int mne_runs_on_host(void);
 int mne_clock_advance(uint64_t* iteration, int32_t* step_offset, void* stream);
 
 /* Number of samples per ray: n_range_d + n_samples_d with depth guidance, n_samples without
@@ -494,6 +510,24 @@ int mne_decoder_update(const mne_scene_t* scene, const float* partials, int n_ra
  * p -= lr/(1-b1^t) * m / (sqrt(v)/sqrt(1-b2^t) + eps); weight_decay is L2 into g; g is zeroed
  * when zero_grad != 0.  segs is a HOST array of n_seg (<= 32) entries. */
 int mne_adam_step(const mne_adam_seg_t* segs, int n_seg, int zero_grad, const mne_clock_t* clock, void* stream);
+
+/* ---- AdamW over many tensors, moments in 32 bits or in 8 ---------------------------------- */
+/* p = p (1 - lr weight_decay);  m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;
+ * p -= lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)      -- torch.optim.AdamW (amsgrad = False, maximize = False),
+ * in fp32 whatever p and g are held in; a 16-bit parameter is rounded to nearest even.
+ * `table` is a HOST array of n_tensors rows of 7: address of p, of g, of m, of v, of the scales, number of elements, ordinal.
+ * Every tensor is one run of n elements in memory; addresses are multiples of the element's size (of 16 bytes: faster), and no
+ * two tensors overlap.
+ * state_bits 32: m, v fp32 [n] (scales and ordinal unused).
+ * state_bits 8:  m int8 [n], v uint8 [n], scales fp32 [ceil(n / 256)][2].  Block b = elements 256 b .. 256 b + 255:
+ *   m = sign(c) c^2 scales[b][0],  sqrt(v) = c^2 scales[b][1]   (mne_adamw_moments gives both as numbers).
+ *   A code is rounded up or down with a dither of 16 bits, a function of (cfg->seed, ordinal, step, element) alone: the same
+ *   call gives the same codes.  `ordinal` is the caller's number for the tensor (0 .. 2^32 - 1), the same at every step.
+ *   A block that meets a gradient that is not finite holds NaN from then on.
+ * clock: as in mne_adam_step (the step, and with it the dither, comes from device memory). */
+int mne_adamw_step(const int64_t* table, int64_t n_tensors, const mne_adamw_cfg_t* cfg, const mne_clock_t* clock, void* stream);
+/* exp_avg [n] and exp_avg_sq [n] in fp32 of n elements' codes and scales (as above; one run that starts with a block). */
+int mne_adamw_moments(const int8_t* m, const uint8_t* v, const float* scales, int64_t n, float* exp_avg, float* exp_avg_sq, void* stream);
 
 /* ---- point queries (forward only) -------------------------------------------------------- */
 /* Replaces JointEncoding.query_color_sdf / query_sdf / run_network_flat (scene_rep.py:232-331):

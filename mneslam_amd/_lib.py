@@ -3,6 +3,7 @@
 The library is the only compute backend of this package.  If it is missing the import of any hot
 path raises -- there is deliberately no CPU/PyTorch fallback.
 """
+import contextlib
 import ctypes as C
 import os
 import threading
@@ -12,7 +13,7 @@ import torch
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libmneslam_hip.so")
 
-ABI_VERSION = 8
+ABI_VERSION = 9
 N_LOSS = 8
 N_COUNT = 8
 C_NEED = 6
@@ -44,6 +45,12 @@ class AdamSeg(C.Structure):
     _fields_ = [("p", C.c_void_p), ("g", C.c_void_p), ("m", C.c_void_p), ("v", C.c_void_p), ("n", C.c_int64),
                 ("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double),
                 ("weight_decay", C.c_double), ("step", C.c_int32), ("p_f16", C.c_int32)]
+
+
+class AdamwCfg(C.Structure):
+    _fields_ = [("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double), ("weight_decay", C.c_double),
+                ("step", C.c_int32), ("state_bits", C.c_int32), ("p_type", C.c_int32), ("g_type", C.c_int32),
+                ("zero_grad", C.c_int32), ("seed", C.c_uint32)]
 
 
 class TileBins(C.Structure):
@@ -116,6 +123,10 @@ _PROTOS = {
     "mne_sizeof_clock": (C.c_size_t, []),
     "mne_sizeof_fused_opts": (C.c_size_t, []),
     "mne_sizeof_decoder_opt": (C.c_size_t, []),
+    "mne_sizeof_adamw_cfg": (C.c_size_t, []),
+    "mne_runs_on_host": (C.c_int, []),
+    "mne_adamw_step": (C.c_int, [C.c_void_p, C.c_int64, C.POINTER(AdamwCfg), C.POINTER(Clock), C.c_void_p]),
+    "mne_adamw_moments": (C.c_int, [C.c_void_p] * 3 + [C.c_int64] + [C.c_void_p] * 3),
     "mne_sample_batch": (C.c_int, [C.c_void_p, C.c_int64, C.c_int, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_int,
                                    C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_uint64, C.c_uint64] + [C.c_void_p] * 5
                          + [C.POINTER(RenderCfg), C.c_void_p, C.c_void_p, C.c_uint64] + [C.c_void_p] * 5 + [C.POINTER(Clock), C.c_void_p]),
@@ -224,7 +235,7 @@ def load(path=None):
         for fn, st in ((lib.mne_sizeof_scene, Scene), (lib.mne_sizeof_render_cfg, RenderCfg),
                        (lib.mne_sizeof_adam_seg, AdamSeg), (lib.mne_sizeof_tile_bins, TileBins),
                        (lib.mne_sizeof_plane_opt, PlaneOpt), (lib.mne_sizeof_clock, Clock),
-                       (lib.mne_sizeof_fused_opts, FusedOpts), (lib.mne_sizeof_decoder_opt, DecoderOpt),
+                       (lib.mne_sizeof_fused_opts, FusedOpts), (lib.mne_sizeof_adamw_cfg, AdamwCfg), (lib.mne_sizeof_decoder_opt, DecoderOpt),
                        (lib.mne_sizeof_tile_overlap, TileOverlap), (lib.mne_sizeof_pose_state, PoseState)):
             if fn() != C.sizeof(st):
                 raise RuntimeError(f"struct layout mismatch for {st.__name__}: C {fn()} vs ctypes {C.sizeof(st)}")
@@ -257,3 +268,23 @@ def stream_for(t):
     if t.is_cuda:
         return C.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
     return None
+
+
+T_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}       # MNE_T_*
+
+
+def one_device(tensors, what):
+    """The device that all of ``tensors`` are on; raises if there are several, or if the library cannot reach it (a kernel that
+    is given an address of host memory would fault)."""
+    dev = tensors[0].device
+    for t in tensors:
+        if t.device != dev:
+            raise ValueError(f"{what}: tensors on {dev} and on {t.device}")
+    if dev.type != ("cpu" if load().mne_runs_on_host() else "cuda"):
+        raise ValueError(f"{what}: tensors on {dev}: the HIP kernels need them on the GPU")
+    return dev
+
+
+def device_guard(dev):
+    """Makes ``dev`` the current device for a launch (the streams of another device are not the current one's)."""
+    return torch.cuda.device(dev) if dev.type == "cuda" and dev.index != torch.cuda.current_device() else contextlib.nullcontext()

@@ -78,6 +78,14 @@ size_t mne_sizeof_adam_seg(void) { return sizeof(mne_adam_seg_t); }
 size_t mne_sizeof_tile_bins(void) { return sizeof(mne_tile_bins_t); }
 size_t mne_sizeof_plane_opt(void) { return sizeof(mne_plane_opt_t); }
 size_t mne_sizeof_clock(void) { return sizeof(mne_clock_t); }
+size_t mne_sizeof_adamw_cfg(void) { return sizeof(mne_adamw_cfg_t); }
+int mne_runs_on_host(void) {
+#ifdef MNE_HOST_EMU
+    return 1;
+#else
+    return 0;
+#endif
+}
 size_t mne_sizeof_fused_opts(void) { return sizeof(mne_fused_opts_t); }
 size_t mne_sizeof_decoder_opt(void) { return sizeof(mne_decoder_opt_t); }
 
@@ -699,6 +707,71 @@ int mne_adam_step(const mne_adam_seg_t* segs, int n_seg, int zero_grad, const mn
     }
     mne_launch_adam(a, (hipStream_t)stream);
     return check_launch("adam_step");
+}
+
+static bool adamw_types(int p, int g) {
+    return p == MNE_T_F32 ? g >= MNE_T_F32 && g <= MNE_T_F16 : (p == MNE_T_BF16 || p == MNE_T_F16) && (g == p || g == MNE_T_F32);
+}
+
+int mne_adamw_step(const int64_t* table, int64_t n_tensors, const mne_adamw_cfg_t* cfg, const mne_clock_t* clock, void* stream) {
+    if (!cfg || n_tensors < 0 || (n_tensors && !table)) return fail(-1, "mne_adamw_step: NULL argument");
+    if (cfg->state_bits != 32 && cfg->state_bits != 8) return fail(-1, "mne_adamw_step: state_bits must be 32 or 8");
+    if (!adamw_types(cfg->p_type, cfg->g_type)) return fail(-1, "mne_adamw_step: unsupported types of parameter and gradient");
+    if (cfg->step < 1) return fail(-1, "mne_adamw_step: step counts from 1");
+    const bool small = cfg->state_bits == 8;
+    const int64_t psize = cfg->p_type == MNE_T_F32 ? 4 : 2, gsize = cfg->g_type == MNE_T_F32 ? 4 : 2;
+    for (int64_t i = 0; i < n_tensors; ++i) {               // nothing is launched unless every row is sound
+        const int64_t* t = table + 7 * i;
+        if (t[5] < 0 || t[5] > (1ll << 42)) return fail(-1, "mne_adamw_step: bad number of elements");
+        if (t[5] && (!t[0] || !t[1] || !t[2] || !t[3] || (small && !t[4]))) return fail(-1, "mne_adamw_step: NULL address");
+        if (t[0] % psize || t[1] % gsize || (small ? t[4] % 8 : t[2] % 4 || t[3] % 4)) return fail(-1, "mne_adamw_step: misaligned address");
+    }
+    AdamwHyper h = {};
+    const double bc1 = 1.0 - std::pow(cfg->beta1, (double)cfg->step), bc2 = 1.0 - std::pow(cfg->beta2, (double)cfg->step);
+    h.lr = cfg->lr; h.step = cfg->step;
+    h.decay = (float)(1.0 - cfg->lr * cfg->weight_decay);
+    h.b1 = (float)cfg->beta1; h.omb1 = (float)(1.0 - cfg->beta1);
+    h.b2 = (float)cfg->beta2; h.omb2 = (float)(1.0 - cfg->beta2);
+    h.eps = (float)cfg->eps;
+    h.step_size = (float)(cfg->lr / bc1); h.root_bc2 = (float)std::sqrt(bc2);
+    Clock clk = {};
+    if (clock && fill_clock(clock, clk, cfg->beta1, cfg->beta2, true))
+        return fail(-1, "mne_adamw_step: clock incomplete or made for other betas");
+    Adamw32Args a32;
+    Adamw8Args a8;
+    a32.h = a8.h = h; a32.clk = a8.clk = clk; a32.zero_grad = a8.zero_grad = cfg->zero_grad;
+    int n_seg = 0;
+    long long blocks = 0;
+    for (int64_t i = 0; i <= n_tensors; ++i) {
+        const int64_t* t = table + 7 * i;
+        const long long more = i < n_tensors ? mne_adamw_blocks_for(t[5]) : 0;
+        if (n_seg && (i == n_tensors || n_seg == (small ? MNE_ADAMW8_SEGS : MNE_ADAMW32_SEGS) || blocks + more > 0x7FFFFFFFll)) {
+            a32.n_seg = a8.n_seg = n_seg;
+            if (small) mne_launch_adamw8(a8, cfg->p_type, cfg->g_type, (unsigned)blocks, (hipStream_t)stream);
+            else mne_launch_adamw32(a32, cfg->p_type, cfg->g_type, (unsigned)blocks, (hipStream_t)stream);
+            if (check_launch("adamw_step")) return -10;
+            n_seg = 0; blocks = 0;
+        }
+        if (!more) continue;
+        if (small) {
+            a8.p[n_seg] = (void*)t[0]; a8.g[n_seg] = (void*)t[1]; a8.m[n_seg] = (void*)t[2]; a8.v[n_seg] = (void*)t[3];
+            a8.scales[n_seg] = (float*)t[4]; a8.n[n_seg] = t[5]; a8.key[n_seg] = mne_adamw_key(cfg->seed, (unsigned)t[6]);
+            a8.first[n_seg] = (int)blocks;
+        } else {
+            a32.p[n_seg] = (void*)t[0]; a32.g[n_seg] = (void*)t[1]; a32.m[n_seg] = (void*)t[2]; a32.v[n_seg] = (void*)t[3];
+            a32.n[n_seg] = t[5]; a32.first[n_seg] = (int)blocks;
+        }
+        ++n_seg; blocks += more;
+    }
+    return 0;
+}
+
+int mne_adamw_moments(const int8_t* m, const uint8_t* v, const float* scales, int64_t n, float* exp_avg, float* exp_avg_sq, void* stream) {
+    if (n < 0 || n > (1ll << 38)) return fail(-1, "mne_adamw_moments: bad number of elements");
+    if (n == 0) return 0;
+    if (!m || !v || !scales || !exp_avg || !exp_avg_sq) return fail(-1, "mne_adamw_moments: NULL argument");
+    mne_launch_adamw_moments(m, v, scales, n, exp_avg, exp_avg_sq, (hipStream_t)stream);
+    return check_launch("adamw_moments");
 }
 
 int mne_encode_oneblob(int64_t n_pts, int dims, const float* x, float* out, void* stream) {

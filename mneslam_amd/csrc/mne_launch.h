@@ -307,6 +307,41 @@ struct AdamArgs {
     Clock clk;
 };
 
+// One launch of mne_adamw_step: what its tensors share, and per tensor the addresses, the size and the first workgroup.  Kernel
+// arguments end at 4 KB, which is what sets the number of tensors of a launch.
+struct AdamwHyper {
+    double lr;
+    float decay, b1, omb1, b2, omb2, eps, step_size, root_bc2;
+    int step;
+};
+#define MNE_ADAMW32_SEGS 80
+#define MNE_ADAMW8_SEGS 64
+struct Adamw32Args {
+    AdamwHyper h;
+    Clock clk;
+    int n_seg, zero_grad;
+    void *p[MNE_ADAMW32_SEGS], *g[MNE_ADAMW32_SEGS], *m[MNE_ADAMW32_SEGS], *v[MNE_ADAMW32_SEGS];
+    long long n[MNE_ADAMW32_SEGS];
+    int first[MNE_ADAMW32_SEGS];
+};
+struct Adamw8Args {
+    AdamwHyper h;
+    Clock clk;
+    int n_seg, zero_grad;
+    void *p[MNE_ADAMW8_SEGS], *g[MNE_ADAMW8_SEGS], *m[MNE_ADAMW8_SEGS], *v[MNE_ADAMW8_SEGS];
+    float* scales[MNE_ADAMW8_SEGS];
+    long long n[MNE_ADAMW8_SEGS];
+    unsigned key[MNE_ADAMW8_SEGS];
+    int first[MNE_ADAMW8_SEGS];
+};
+static_assert(sizeof(Adamw32Args) <= 4096 && sizeof(Adamw8Args) <= 4096, "kernel arguments are limited to 4 KB");
+
+int mne_launch_adamw32(const Adamw32Args& a, int p_type, int g_type, unsigned blocks, hipStream_t st);
+int mne_launch_adamw8(const Adamw8Args& a, int p_type, int g_type, unsigned blocks, hipStream_t st);
+int mne_launch_adamw_moments(const signed char* mc, const unsigned char* rc, const float* scales, long long n, float* m, float* v, hipStream_t st);
+long long mne_adamw_blocks_for(long long n);
+unsigned mne_adamw_key(unsigned seed, unsigned ordinal);
+
 int mne_launch_sample_z(const ZArgs& a, hipStream_t st);
 int mne_launch_pack(const mne_scene_t& sc, float* pk, hipStream_t st);
 // mode: 0 = forward, every sample decoded (raw complete);  1 = forward with early ray termination (maps only);

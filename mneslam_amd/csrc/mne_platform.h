@@ -4,6 +4,13 @@
 #pragma once
 #ifdef MNE_HOST_EMU
 #include "hip_emu.h"
+// bf16 <-> fp32, rounded to nearest even
+static inline float mne_bf16_to_float(unsigned short x) { return __uint_as_float((unsigned)x << 16); }
+static inline unsigned short mne_float_to_bf16(float x) {
+    const unsigned u = __float_as_uint(x);
+    if ((u & 0x7FFFFFFFu) > 0x7F800000u) return (unsigned short)((u >> 16) | 0x40u);
+    return (unsigned short)((u + 0x7FFFu + ((u >> 16) & 1u)) >> 16);
+}
 #else
 #include <hip/hip_runtime.h>
 #define MNE_LAUNCH(kern, grid, block, lds, stream, ...) \
@@ -37,6 +44,10 @@ static __device__ __forceinline__ int mne_bcast8(int v, int k) {
     }
 }
 static __device__ __forceinline__ float mne_bcast8(float v, int k) { return __int_as_float(mne_bcast8(__float_as_int(v), k)); }
+static __device__ __forceinline__ float mne_bf16_to_float(unsigned short x) { return __uint_as_float((unsigned)x << 16); }
+static __device__ __forceinline__ unsigned short mne_float_to_bf16(float x) {         // one v_cvt_pk_bf16_f32: to nearest even
+    return __builtin_bit_cast(unsigned short, (__bf16)x);
+}
 // The XCD (accelerator complex die, 0..7 on MI355X) this wave runs on: hardware register XCC_ID.
 static __device__ __forceinline__ int mne_xcc_id() {
     int v;

@@ -111,3 +111,213 @@ class FusedAdam(torch.optim.Optimizer):
                 if getattr(p, "grad32", None) is not None:
                     p.grad32 = None                      # the fp32 gradient sum of a half-precision plane (see ``segments``)
         return super().zero_grad(set_to_none=set_to_none)
+
+
+# ---- AdamW -------------------------------------------------------------------------------------------------------------
+MOMENT_BLOCK = 256             # consecutive elements of an 8-bit moment that share a scale
+
+
+def _is_dense(t):
+    return t.is_contiguous() or (t.dim() == 4 and t.is_contiguous(memory_format=torch.channels_last)) \
+        or (t.dim() == 5 and t.is_contiguous(memory_format=torch.channels_last_3d))
+
+
+def _laid_out_alike(a, b):
+    """Equal strides in every dimension that has more than one entry (the shapes are equal)."""
+    return a.stride() == b.stride() or all(x == y for n, x, y in zip(a.shape, a.stride(), b.stride()) if n > 1)
+
+
+def _check_hyper(lr, betas, eps, weight_decay):
+    if not 0.0 <= lr < float("inf"):
+        raise ValueError(f"Invalid learning rate: {lr}")
+    if not (len(betas) == 2 and all(0.0 <= b < 1.0 for b in betas)):
+        raise ValueError(f"Invalid betas: {betas}")
+    if not 0.0 <= eps < float("inf"):
+        raise ValueError(f"Invalid epsilon value: {eps}")
+    if not 0.0 <= weight_decay < float("inf"):
+        raise ValueError(f"Invalid weight_decay value: {weight_decay}")
+
+
+@torch.no_grad()
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, scales=None, *, step, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
+               seed=0, ordinals=None, zero_grad=False, clock=None):
+    """One AdamW step (decoupled decay, torch.optim.AdamW with amsgrad=False, maximize=False) over a list of tensors, in place and
+    in as few launches as the list allows (80 tensors each, 64 with 8-bit moments): ``params``, ``grads``, ``exp_avgs`` and
+    ``exp_avg_sqs`` are lists of one length.
+
+    Parameters are float32, bfloat16 or float16; a gradient has its parameter's type or float32 (any of the three beside a float32
+    parameter).  The arithmetic is fp32; a 16-bit parameter is rounded to nearest even.  Every tensor is dense (contiguous or
+    channels_last); moments are laid out like their parameter, a gradient laid out otherwise is copied.  Parameters do not overlap.
+
+    ``scales`` None: moments are float32.  Otherwise they are held in 8 bits: ``exp_avgs`` int8, ``exp_avg_sqs`` uint8, and
+    ``scales`` the list of their float32 [ceil(n / 256), 2] scales, two for each 256 consecutive elements of the tensor's memory
+    (all zero: all moments zero; ``adamw_moments`` gives the moments in fp32).  Their codes are rounded up or down with a dither that
+    depends on ``seed``, the tensor's entry of ``ordinals`` (its place in the list by default; keep it the same at every step),
+    ``step`` and the element alone.  A block that meets a gradient that is not finite holds NaN from then on.
+
+    ``step`` counts from 1 and is the list's; ``clock`` (mneslam_amd._lib.Clock, graph recording) adds the device's step offset.
+    Without one a step is not recorded into a graph: every replay would be the same step."""
+    params, grads, exp_avgs, exp_avg_sqs = list(params), list(grads), list(exp_avgs), list(exp_avg_sqs)
+    small = scales is not None
+    scales = list(scales) if small else [None] * len(params)
+    ordinals = list(range(len(params))) if ordinals is None else [int(o) for o in ordinals]
+    if not len(params) == len(grads) == len(exp_avgs) == len(exp_avg_sqs) == len(scales) == len(ordinals):
+        raise ValueError("adamw_step: lists of different lengths")
+    lr, eps, weight_decay, step = float(lr), float(eps), float(weight_decay), int(step)
+    _check_hyper(lr, betas, eps, weight_decay)
+    if not 1 <= step < 1 << 31:
+        raise ValueError(f"adamw_step: step counts from 1, got {step}")
+    if not 0 <= int(seed) < 1 << 32 or not all(0 <= o < 1 << 32 for o in ordinals):
+        raise ValueError("adamw_step: seed and ordinals are numbers of 32 bits")
+    if not params:
+        return
+    dev = _lib.one_device(params + grads + exp_avgs + exp_avg_sqs + (scales if small else []), "adamw_step")
+    if clock is None and dev.type == "cuda" and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("adamw_step: recording a step needs a clock (the step count would be the same at every replay)")
+    m_type, v_type = (torch.int8, torch.uint8) if small else (torch.float32, torch.float32)
+    tables, keep, seen = {}, [], set()
+    for p, g, m, v, s, o in zip(params, grads, exp_avgs, exp_avg_sqs, scales, ordinals):
+        pt, gt, n = p.dtype, g.dtype, p.numel()
+        if pt not in _lib.T_CODES or not (gt == pt or gt == torch.float32 or (pt == torch.float32 and gt in _lib.T_CODES)):
+            raise TypeError(f"adamw_step: parameter {pt} with gradient {gt} is not supported")
+        if g.layout != torch.strided or g.shape != p.shape or m.shape != p.shape or v.shape != p.shape:
+            raise ValueError("adamw_step: gradient and moments need their parameter's shape")
+        if m.dtype != m_type or v.dtype != v_type:
+            raise TypeError(f"adamw_step: moments must be {m_type} and {v_type}")
+        if n == 0:
+            continue
+        if not _is_dense(p):
+            raise ValueError("adamw_step: parameters must be dense (contiguous or channels_last)")
+        if not (_laid_out_alike(m, p) and _laid_out_alike(v, p)):
+            raise ValueError("adamw_step: moments must be laid out like their parameter")
+        if not _laid_out_alike(g, p):
+            if zero_grad:
+                raise ValueError("adamw_step: zero_grad needs gradients laid out like their parameters")
+            g = torch.empty_like(p, dtype=gt).copy_(g)
+            keep.append(g)
+        if small and (s.dtype != torch.float32 or s.shape != (-(-n // MOMENT_BLOCK), 2) or not s.is_contiguous()):
+            raise ValueError("adamw_step: scales must be contiguous float32 [ceil(n / 256), 2]")
+        at = p.data_ptr()
+        if at in seen:
+            raise ValueError("adamw_step: the same parameter twice")
+        seen.add(at)
+        tables.setdefault((pt, gt), []).extend((at, g.data_ptr(), m.data_ptr(), v.data_ptr(), s.data_ptr() if small else 0, n, o))
+    lib = _lib.load()
+    with _lib.device_guard(dev):
+        stream = _lib.stream_for(params[0])
+        for (pt, gt), table in tables.items():
+            cfg = _lib.AdamwCfg(lr, betas[0], betas[1], eps, weight_decay, step, 8 if small else 32, _lib.T_CODES[pt],
+                                _lib.T_CODES[gt], 1 if zero_grad else 0, int(seed))
+            _lib.check(lib.mne_adamw_step((C.c_int64 * len(table))(*table), len(table) // 7, C.byref(cfg),
+                                          C.byref(clock) if clock is not None else None, stream), "mne_adamw_step")
+    torch.autograd.graph.increment_version([p for p in params if not p.is_inference()])
+
+
+@torch.no_grad()
+def adamw_moments(exp_avg, exp_avg_sq, scales):
+    """The fp32 moments (exp_avg, exp_avg_sq) that 8-bit codes and their ``scales`` stand for (see ``adamw_step``), in the codes'
+    shape and layout."""
+    n = exp_avg.numel()
+    if exp_avg.dtype != torch.int8 or exp_avg_sq.dtype != torch.uint8:
+        raise TypeError("adamw_moments: the codes are int8 and uint8")
+    if exp_avg_sq.shape != exp_avg.shape or not _laid_out_alike(exp_avg_sq, exp_avg) or not _is_dense(exp_avg):
+        raise ValueError("adamw_moments: the codes must be dense and laid out alike")
+    if scales.dtype != torch.float32 or scales.shape != (-(-n // MOMENT_BLOCK), 2) or not scales.is_contiguous():
+        raise ValueError("adamw_moments: scales must be contiguous float32 [ceil(n / 256), 2]")
+    dev = _lib.one_device([exp_avg, exp_avg_sq, scales], "adamw_moments")
+    m, v = torch.empty_like(exp_avg, dtype=torch.float32), torch.empty_like(exp_avg, dtype=torch.float32)
+    with _lib.device_guard(dev):
+        _lib.check(_lib.load().mne_adamw_moments(_lib.ptr(exp_avg), _lib.ptr(exp_avg_sq), _lib.ptr(scales), n, _lib.ptr(m), _lib.ptr(v),
+                                                 _lib.stream_for(exp_avg)), "mne_adamw_moments")
+    return m, v
+
+
+class FusedAdamW(torch.optim.Optimizer):
+    """torch.optim.AdamW (amsgrad=False, maximize=False) whose ``step()`` is ``adamw_step``: one launch for up to 80 tensors of a
+    group that are at the same step count.  ``state_bits`` 8 (also per group) holds the moments in 8 bits with two scales for each 256
+    elements -- 2.06 bytes an element instead of 8; ``moments(p)`` gives them in fp32.  ``seed`` is that of the codes' dither."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, seed=0):
+        if not 0 <= int(seed) < 1 << 32:
+            raise ValueError(f"Invalid seed: {seed}")
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits, seed=int(seed)))
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        group = self.param_groups[-1]
+        _check_hyper(group["lr"], group["betas"], group["eps"], group["weight_decay"])
+        if group["state_bits"] not in (8, 32):
+            raise ValueError(f"Invalid state_bits: {group['state_bits']} (8 or 32)")
+
+    def _state(self, p, bits):
+        st = self.state[p]
+        if len(st) == 0:
+            if p.is_cuda and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("FusedAdamW: take a step before recording one (the moments would be cleared at every replay)")
+            st["step"] = 0
+            # preserve_format: the same physical layout as p
+            st["exp_avg"] = torch.zeros_like(p, dtype=torch.int8 if bits == 8 else torch.float32)
+            st["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.uint8 if bits == 8 else torch.float32)
+            if bits == 8:
+                st["scales"] = torch.zeros(-(-p.numel() // MOMENT_BLOCK), 2, device=p.device)
+        return st
+
+    @torch.no_grad()
+    def step(self, closure=None, zero_grad=False, clock=None):
+        """``zero_grad``: the gradients are zero behind the step (one pass less over them).  ``clock`` (graph recording): the kernels
+        add the device step offset to the parameters' CURRENT step + 1, and the step counts here are left alone."""
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        ordinal = 0
+        for group in self.param_groups:
+            batches = {}                                # tensors of one device at one step count
+            for p in group["params"]:
+                ordinal += 1
+                if p.grad is None:
+                    if getattr(p, "grad32", None) is not None:
+                        p.grad32 = None                 # .grad was dropped by someone else: the fp32 sum beside it is stale
+                    continue
+                if p.grad.is_sparse:
+                    raise RuntimeError("FusedAdamW does not support sparse gradients")
+                # a half-precision plane: the render node leaves the fp32 sum beside the rounded gradient
+                g = p.grad32 if getattr(p, "grad32", None) is not None else p.grad
+                st = self._state(p, group["state_bits"])
+                batches.setdefault((p.device, st["step"] + 1), []).append((p, g, st, ordinal - 1))
+            for (_, step), batch in batches.items():
+                ps, gs, sts, ords = zip(*batch)
+                adamw_step(ps, gs, [s["exp_avg"] for s in sts], [s["exp_avg_sq"] for s in sts],
+                           [s["scales"] for s in sts] if group["state_bits"] == 8 else None, step=step, lr=group["lr"],
+                           betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"], seed=group["seed"],
+                           ordinals=ords, zero_grad=zero_grad, clock=clock)
+                if clock is None:
+                    for s in sts:
+                        s["step"] = step
+                if zero_grad:
+                    for p, g in zip(ps, gs):
+                        if g is not p.grad:
+                            p.grad.zero_()
+        return loss
+
+    def moments(self, p):
+        """(exp_avg, exp_avg_sq) of ``p`` in fp32."""
+        st = self.state[p]
+        return adamw_moments(st["exp_avg"], st["exp_avg_sq"], st["scales"]) if "scales" in st else (st["exp_avg"], st["exp_avg_sq"])
+
+    def load_state_dict(self, state_dict):
+        """The base class casts floating-point state to its parameter's type: moments and scales are put back as they were saved."""
+        super().load_state_dict(state_dict)
+        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
+        for i, p in zip(saved, (p for g in self.param_groups for p in g["params"])):
+            for key, value in state_dict["state"].get(i, {}).items():
+                if torch.is_tensor(value):
+                    like = p if value.shape == p.shape else value
+                    self.state[p][key] = torch.empty_like(like, dtype=value.dtype, device=p.device).copy_(value)
+
+    def zero_grad(self, set_to_none=True):
+        for group in self.param_groups:
+            for p in group["params"]:
+                if getattr(p, "grad32", None) is not None:
+                    p.grad32 = None                      # the fp32 gradient sum of a half-precision plane
+        return super().zero_grad(set_to_none=set_to_none)
