@@ -5,6 +5,7 @@ path raises -- there is deliberately no CPU/PyTorch fallback.
 """
 import contextlib
 import ctypes as C
+import importlib.util
 import os
 import threading
 
@@ -239,6 +240,7 @@ def load(path=None):
                        (lib.mne_sizeof_tile_overlap, TileOverlap), (lib.mne_sizeof_pose_state, PoseState)):
             if fn() != C.sizeof(st):
                 raise RuntimeError(f"struct layout mismatch for {st.__name__}: C {fn()} vs ctypes {C.sizeof(st)}")
+        lib.on_host = bool(lib.mne_runs_on_host())
         _lib = lib
         return lib
 
@@ -280,7 +282,7 @@ def one_device(tensors, what):
     for t in tensors:
         if t.device != dev:
             raise ValueError(f"{what}: tensors on {dev} and on {t.device}")
-    if dev.type != ("cpu" if load().mne_runs_on_host() else "cuda"):
+    if dev.type != ("cpu" if load().on_host else "cuda"):
         raise ValueError(f"{what}: tensors on {dev}: the HIP kernels need them on the GPU")
     return dev
 
@@ -288,3 +290,32 @@ def one_device(tensors, what):
 def device_guard(dev):
     """Makes ``dev`` the current device for a launch (the streams of another device are not the current one's)."""
     return torch.cuda.device(dev) if dev.type == "cuda" and dev.index != torch.cuda.current_device() else contextlib.nullcontext()
+
+
+def address(lib, name):
+    """Address of an entry point (for callers in C++)."""
+    return C.cast(getattr(lib, name), C.c_void_p).value
+
+
+def raw_stream(dev):
+    """Handle of the current stream of ``dev`` as a number."""
+    return torch.cuda.current_stream(dev).cuda_stream if dev.type == "cuda" else 0
+
+
+_host = None
+
+
+def host_tensors():
+    """The in-tree extension module of csrc/host_tensors.cpp."""
+    global _host
+    if _host is None:
+        path = os.path.join(_HERE, "_host_tensors.so")
+        if not os.path.exists(path):
+            raise RuntimeError(f"{path} not found. Build it with `python -m mneslam_amd.build`.")
+        spec = importlib.util.spec_from_file_location("mneslam_amd._host_tensors", path)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        if mod.ABI_VERSION != ABI_VERSION:
+            raise RuntimeError("_host_tensors ABI version mismatch")
+        _host = mod
+    return _host

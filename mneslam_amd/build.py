@@ -16,6 +16,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 from . import isa_check
@@ -24,6 +25,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 LIB = os.path.join(HERE, "libmneslam_hip.so")
+HOST_LIB = os.path.join(HERE, "_host_tensors.so")
 FUZZ_DIR = os.path.join(HERE, "_fuzz")
 SOURCES = ["capi.hip", "render.hip", "wgrad.hip", "adam.hip", "adamw.hip", "sampler.hip", "tile_adam.hip", "gridenc.hip", "pose.hip", "encodings.hip"]
 HEADERS = ["mne_device.h", "mne_launch.h", "mne_platform.h", "mlp_mfma.h"]
@@ -126,7 +128,26 @@ def _compile_all(obj_dir, lib, extra, force, verbose, jobs):
     return lib
 
 
+def build_host(force=False, verbose=False):
+    """The extension module that reads lists of torch tensors (csrc/host_tensors.cpp): host code only."""
+    src = os.path.join(CSRC, "host_tensors.cpp")
+    if not force and not _stale(HOST_LIB, [src, os.path.join(INCLUDE, "mneslam_hip.h")]):
+        return HOST_LIB
+    import torch
+    from torch.utils import cpp_extension
+    lib_dir = os.path.join(os.path.dirname(torch.__file__), "lib")
+    inc = [INCLUDE, *cpp_extension.include_paths(), sysconfig.get_paths()["include"]]
+    cmd = [shutil.which("g++") or "c++", "-std=c++17", "-O2", "-shared", "-fPIC", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[f"-I{i}" for i in inc], src, "-o", HOST_LIB,
+           f"-L{lib_dir}", "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.check_call(cmd)
+    return HOST_LIB
+
+
 def build(force=False, verbose=False, jobs=None):
+    build_host(force, verbose)
     return _compile_all(CSRC, LIB, [], force, verbose, jobs or (os.cpu_count() or 4))
 
 

@@ -22,7 +22,15 @@
 
 #define AW_THREADS 256
 #define AW_BLOCK 256                                 // elements that share two scales
-#define AW_PER_WG 4096                               // elements of a workgroup: 16 of each thread
+// Elements of a workgroup.
+#ifndef AW32_WG
+#define AW32_WG 2048
+#endif
+#define AW8_WG 4096
+#define AW_SMALL_WG 1024
+#ifndef AW_SMALL
+#define AW_SMALL (1 << 20)
+#endif
 
 __device__ __forceinline__ unsigned aw_mix(unsigned h) {      // a multiply-xorshift mix of 32 bits
     h = (h ^ (h >> 16)) * 0x7FEB352Du;
@@ -58,141 +66,325 @@ __device__ __forceinline__ int aw_segment(const int* first, int n, int blk) {
     return lo;
 }
 
-template <int PT, int GT>
+// N consecutive elements of memory from (to) element i, as fp32: vectors of up to 16 bytes, or, with FULL false, element by element
+// and only those below n (zeros stand for the others).
+template <int T, int N, bool FULL>
+__device__ __forceinline__ void aw_load(float* out, const void* base, long long i, long long n) {
+    typedef typename AwType<T>::mem mem;
+    const mem* q = (const mem*)base + i;
+    if (FULL) {
+        constexpr int B = N * (int)sizeof(mem) < 16 ? N * (int)sizeof(mem) : 16;
+        union { MneBytes<B> v[N * sizeof(mem) / B]; mem e[N]; } r;
+#pragma unroll
+        for (int k = 0; k < N * (int)sizeof(mem) / B; ++k) r.v[k] = ((const MneBytes<B>*)q)[k];
+#pragma unroll
+        for (int k = 0; k < N; ++k) out[k] = AwType<T>::get(r.e[k]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k) out[k] = i + k < n ? AwType<T>::get(q[k]) : 0.0f;
+    }
+}
+template <int T, int N, bool FULL>
+__device__ __forceinline__ void aw_store(const float* x, void* base, long long i, long long n) {
+    typedef typename AwType<T>::mem mem;
+    mem* q = (mem*)base + i;
+    if (FULL) {
+        constexpr int B = N * (int)sizeof(mem) < 16 ? N * (int)sizeof(mem) : 16;
+        union { MneBytes<B> v[N * sizeof(mem) / B]; mem e[N]; } r;
+#pragma unroll
+        for (int k = 0; k < N; ++k) r.e[k] = AwType<T>::put(x[k]);
+#pragma unroll
+        for (int k = 0; k < N * (int)sizeof(mem) / B; ++k) ((MneBytes<B>*)q)[k] = r.v[k];
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k) if (i + k < n) q[k] = AwType<T>::put(x[k]);
+    }
+}
+
+// Consecutive elements of a thread's pieces: 16 bytes of the parameter, as far as the thread has that many.
+template <int PT, int EACH> struct AwPiece { static constexpr int N = PT == MNE_T_F32 || EACH < 8 ? 4 : 8; };
+
+template <int PT, int GT, int EACH, bool FULL>
+__device__ __forceinline__ void adamw32_body(const Adamw32Args& a, const AdamwHyper& h, int s, long long base) {
+    constexpr int N = AwPiece<PT, EACH>::N, K = EACH / N;
+    const long long n = a.n[s], i0 = base + threadIdx.x * N;
+    float p[K][N], g[K][N], m[K][N], v[K][N];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const long long i = i0 + k * (AW_THREADS * N);
+        aw_load<PT, N, FULL>(p[k], a.p[s], i, n);
+        aw_load<GT, N, FULL>(g[k], a.g[s], i, n);
+        aw_load<MNE_T_F32, N, FULL>(m[k], a.m[s], i, n);
+        aw_load<MNE_T_F32, N, FULL>(v[k], a.v[s], i, n);
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const long long i = i0 + k * (AW_THREADS * N);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            m[k][j] = m[k][j] * h.b1 + g[k][j] * h.omb1;
+            v[k][j] = v[k][j] * h.b2 + (g[k][j] * g[k][j]) * h.omb2;
+            p[k][j] = p[k][j] * h.decay - h.step_size * (m[k][j] / (sqrtf(v[k][j]) / h.root_bc2 + h.eps));
+            g[k][j] = 0.0f;
+        }
+        aw_store<PT, N, FULL>(p[k], a.p[s], i, n);
+        aw_store<MNE_T_F32, N, FULL>(m[k], a.m[s], i, n);
+        aw_store<MNE_T_F32, N, FULL>(v[k], a.v[s], i, n);
+        if (a.zero_grad) aw_store<GT, N, FULL>(g[k], a.g[s], i, n);
+    }
+}
+
+template <int PT, int GT, int EACH>
 __global__ __launch_bounds__(AW_THREADS) void adamw32_kernel(Adamw32Args a) {
     const int s = aw_segment(a.first, a.n_seg, (int)blockIdx.x);
     AdamwHyper h = a.h;
     if (a.clk.bias_table) clock_bias(a.clk, h.lr, h.step, h.step_size, h.root_bc2);
-    typename AwType<PT>::mem* p = (typename AwType<PT>::mem*)a.p[s];
-    typename AwType<GT>::mem* g = (typename AwType<GT>::mem*)a.g[s];
-    float *m = (float*)a.m[s], *v = (float*)a.v[s];
-    const long long n = a.n[s], base = (long long)((int)blockIdx.x - a.first[s]) * AW_PER_WG;
-    for (int k = 0; k < AW_PER_WG / AW_THREADS; ++k) {
-        const long long i = base + k * AW_THREADS + threadIdx.x;
-        if (i >= n) return;
-        const float gg = AwType<GT>::get(g[i]);
-        const float mm = m[i] * h.b1 + gg * h.omb1;
-        const float vv = v[i] * h.b2 + (gg * gg) * h.omb2;
-        p[i] = AwType<PT>::put(AwType<PT>::get(p[i]) * h.decay - h.step_size * (mm / (sqrtf(vv) / h.root_bc2 + h.eps)));
-        m[i] = mm; v[i] = vv;
-        if (a.zero_grad) g[i] = AwType<GT>::put(0.0f);
+    const long long base = (long long)((int)blockIdx.x - a.first[s]) * (AW_THREADS * EACH);
+    if (a.aligned[s] && base + AW_THREADS * EACH <= a.n[s]) adamw32_body<PT, GT, EACH, true>(a, h, s, base);
+    else adamw32_body<PT, GT, EACH, false>(a, h, s, base);
+}
+
+// Code of x in 0..most^2 with the dither k / 65536: floor of the root, or one more if k / 65536 (2 c + 1) < x - c^2.  The floor is exact
+// with a root that is 1 ulp off: it is the floor of the root of floor(x) + 1/2, which is no nearer than 1 / (4 most) to a whole number.
+// The difference is exact too (a multiple of x's last place, no larger than x).
+__device__ __forceinline__ int aw_code(float x, unsigned k) {
+    const int c = (int)mne_sqrt_fast(floorf(x) + 0.5f);
+    const float f = (float)c;
+    return (float)k * fmaf(f, 2.0f / 65536.0f, 1.0f / 65536.0f) < x - f * f ? c + 1 : c;
+}
+
+template <int LANES> __device__ __forceinline__ unsigned aw_max(unsigned x) {
+    x = mne_max16(x);
+#pragma unroll
+    for (int d = 16; d < LANES; d <<= 1) {
+        const unsigned o = __shfl_xor(x, d);
+        x = o > x ? o : x;
+    }
+    return x;
+}
+
+// LANES lanes have a block of 256, EACH = 256 / LANES elements each.
+template <int PT, int GT, int LANES, bool FULL>
+__device__ __forceinline__ void adamw8_body(const Adamw8Args& a, const AdamwHyper& h, int step, int s, long long b) {
+    constexpr int EACH = AW_BLOCK / LANES, N = AwPiece<PT, EACH>::N, K = EACH / N;
+    const int l = threadIdx.x % LANES;
+    const long long n = a.n[s], i0 = b * AW_BLOCK + l * N;
+    const bool there = FULL || b * AW_BLOCK < n;
+    const float2 scale = there ? ((const float2*)a.scales[s])[b] : make_float2(0.0f, 0.0f);
+    float m[K][N], r[K][N];
+    {
+        float p[K][N], g[K][N];
+        union { MneBytes<N> v; signed char c[N]; } mc[K];
+        union { MneBytes<N> v; unsigned char c[N]; } rc[K];
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const long long i = i0 + k * (LANES * N);
+            aw_load<PT, N, FULL>(p[k], a.p[s], i, n);
+            aw_load<GT, N, FULL>(g[k], a.g[s], i, n);
+            if (FULL) {
+                mc[k].v = *(const MneBytes<N>*)((const signed char*)a.m[s] + i);
+                rc[k].v = *(const MneBytes<N>*)((const unsigned char*)a.v[s] + i);
+            } else {
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    mc[k].c[j] = i + j < n ? ((const signed char*)a.m[s])[i + j] : (signed char)0;
+                    rc[k].c[j] = i + j < n ? ((const unsigned char*)a.v[s])[i + j] : (unsigned char)0;
+                }
+            }
+        }
+        unsigned least = 0xFFFFFFFFu;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const float c = (float)mc[k].c[j], d = (float)rc[k].c[j], gg = g[k][j], r0 = d * d * scale.y;
+                m[k][j] = (c * fabsf(c) * scale.x) * h.b1 + gg * h.omb1;
+                r[k][j] = (r0 * r0) * h.b2 + (gg * gg) * h.omb2;
+                const unsigned below = __float_as_uint(r[k][j]) - 1u;            // zero is out of the way, at the top
+                least = below < least ? below : least;
+            }
+        if (least < 0x0F800000u - 1u) {               // a square below 2^-96: the root with scaling
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int j = 0; j < N; ++j) r[k][j] = sqrtf(r[k][j]);
+        } else {
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int j = 0; j < N; ++j) r[k][j] = mne_sqrt_rn(r[k][j]);
+        }
+        const float inv = 1.0f / h.root_bc2;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const long long i = i0 + k * (LANES * N);
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                // (a reciprocal is enough here: nothing of the parameter enters the codes)
+                p[k][j] = p[k][j] * h.decay - h.step_size * (m[k][j] * mne_rcp_fast(fmaf(r[k][j], inv, h.eps)));
+                g[k][j] = 0.0f;
+            }
+            aw_store<PT, N, FULL>(p[k], a.p[s], i, n);
+            if (a.zero_grad) aw_store<GT, N, FULL>(g[k], a.g[s], i, n);
+        }
+    }
+    // Largest magnitudes of the block.  Of sqrt(v) by the bits, where NaN is above infinity; where all of it is finite, all of m is.
+    float most = 0.0f;
+    unsigned br = 0;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const unsigned ur = __float_as_uint(r[k][j]);
+            most = fmaxf(most, fabsf(m[k][j]));
+            br = ur > br ? ur : br;
+        }
+    unsigned bm = __float_as_uint(most);
+    br = aw_max<LANES>(br);
+    if (__ballot(br >= 0x7F800000u)) {                // (the whole wave goes this way)
+        bm = 0;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const unsigned um = __float_as_uint(m[k][j]) & 0x7FFFFFFFu;
+                bm = um > bm ? um : bm;
+            }
+    }
+    bm = aw_max<LANES>(bm);
+    const bool fine_m = bm < 0x7F800000u, fine_r = br < 0x7F800000u;
+    const float fm = __uint_as_float(bm), fr = __uint_as_float(br);
+    const bool some_m = fine_m && fm > 7.8886090522101181e-31f, some_r = fine_r && fr > 0.0f;      // 2^-100: 127^2 / max stays finite
+    const float im = some_m ? 16129.0f / fm : 0.0f, ir = some_r ? 65025.0f / fr : 0.0f;
+    if (!(fine_m && fine_r)) {                        // codes 0 in what is not finite
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                if (!fine_m) m[k][j] = 0.0f;
+                if (!fine_r) r[k][j] = 0.0f;
+            }
+    }
+    const unsigned kb = aw_mix((a.key[s] + (unsigned)step * AW_GOLD) ^ aw_mix((unsigned)b)) + (unsigned)(l * N) * AW_GOLD;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const long long i = i0 + k * (LANES * N);
+        union { MneBytes<N> v; unsigned char c[N]; } mc, rc;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            unsigned u = kb + (unsigned)(k * LANES * N + j) * AW_GOLD;
+            u = (u ^ (u >> 16)) * 0x7FEB352Du;
+            u ^= u >> 15;
+            int cm = aw_code(fabsf(m[k][j]) * im, u & 0xFFFFu), cr = aw_code(r[k][j] * ir, u >> 16);
+            cm = cm < 127 ? cm : 127;
+            const int least = r[k][j] > 0.0f ? 1 : 0;
+            cr = cr < least ? least : cr < 255 ? cr : 255;
+            mc.c[j] = (unsigned char)(m[k][j] < 0.0f ? -cm : cm);
+            rc.c[j] = (unsigned char)cr;
+        }
+        if (FULL) {
+            *(MneBytes<N>*)((signed char*)a.m[s] + i) = mc.v;
+            *(MneBytes<N>*)((unsigned char*)a.v[s] + i) = rc.v;
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                if (i + j < n) { ((unsigned char*)a.m[s])[i + j] = mc.c[j]; ((unsigned char*)a.v[s])[i + j] = rc.c[j]; }
+        }
+    }
+    if (l == 0 && there) {
+        const float nan = __uint_as_float(0x7FC00000u);
+        ((float2*)a.scales[s])[b] = make_float2(fine_m ? (some_m ? fm / 16129.0f : 0.0f) : nan, fine_r ? (some_r ? fr / 65025.0f : 0.0f) : nan);
     }
 }
 
-// code of x in 0..top (top = most^2): floor of the root, or one more where the dither says so
-__device__ __forceinline__ float aw_code(float x, float u) {
-    float c = floorf(sqrtf(x));
-    if (c * c > x) c -= 1.0f;                         // the root was rounded up to the next whole number
-    return u * (2.0f * c + 1.0f) < x - c * c ? c + 1.0f : c;
-}
-
-template <int PT, int GT>
+template <int PT, int GT, int LANES>
 __global__ __launch_bounds__(AW_THREADS) void adamw8_kernel(Adamw8Args a) {
-    const int s = aw_segment(a.first, a.n_seg, (int)blockIdx.x), lane = threadIdx.x & 63;
+    const int s = aw_segment(a.first, a.n_seg, (int)blockIdx.x);
     AdamwHyper h = a.h;
     int step = h.step;
     if (a.clk.bias_table) {
         clock_bias(a.clk, h.lr, h.step, h.step_size, h.root_bc2);
         step += *a.clk.step_offset;
     }
-    typename AwType<PT>::mem* p = (typename AwType<PT>::mem*)a.p[s];
-    typename AwType<GT>::mem* g = (typename AwType<GT>::mem*)a.g[s];
-    signed char* mc = (signed char*)a.m[s];
-    unsigned char* rc = (unsigned char*)a.v[s];
-    const long long n = a.n[s];
-    for (int k = 0; k < 4; ++k) {                     // one wave a block of 256, four blocks a wave
-        const long long b = (long long)((int)blockIdx.x - a.first[s]) * (AW_PER_WG / AW_BLOCK) + (threadIdx.x >> 6) * 4 + k;
-        if (b * AW_BLOCK >= n) return;
-        const float sm = a.scales[s][2 * b], sr = a.scales[s][2 * b + 1];
-        float mm[4], rr[4];
-        unsigned bm = 0, br = 0;
+    constexpr int BLOCKS = AW_THREADS / LANES;
+    const long long wg = (int)blockIdx.x - a.first[s], b = wg * BLOCKS + threadIdx.x / LANES;
+    if (a.aligned[s] && (wg + 1) * (BLOCKS * AW_BLOCK) <= a.n[s]) adamw8_body<PT, GT, LANES, true>(a, h, step, s, b);
+    else adamw8_body<PT, GT, LANES, false>(a, h, step, s, b);
+}
+
+// what 8-bit moments stand for, in 32 bits: exp_avg and exp_avg_sq, four elements a thread
+__global__ __launch_bounds__(AW_THREADS) void adamw_moments_kernel(const signed char* mc, const unsigned char* rc, const float* scales,
+                                                                   long long n, float* m, float* v, int aligned) {
+    const long long i = 4 * ((long long)blockIdx.x * AW_THREADS + threadIdx.x);
+    if (i >= n) return;
+    const float2 scale = ((const float2*)scales)[i / AW_BLOCK];
+    union { MneBytes<4> v; signed char c[4]; } a;
+    union { MneBytes<4> v; unsigned char c[4]; } b;
+    const bool full = aligned && i + 4 <= n;
+    if (full) {
+        a.v = *(const MneBytes<4>*)(mc + i);
+        b.v = *(const MneBytes<4>*)(rc + i);
+    } else {
         for (int j = 0; j < 4; ++j) {
-            const long long i = b * AW_BLOCK + j * 64 + lane;
-            mm[j] = rr[j] = 0.0f;
-            if (i < n) {
-                const float gg = AwType<GT>::get(g[i]), c = (float)mc[i], d = (float)rc[i], r0 = d * d * sr;
-                mm[j] = (c * fabsf(c) * sm) * h.b1 + gg * h.omb1;
-                rr[j] = sqrtf((r0 * r0) * h.b2 + (gg * gg) * h.omb2);
-                p[i] = AwType<PT>::put(AwType<PT>::get(p[i]) * h.decay - h.step_size * (mm[j] / (rr[j] / h.root_bc2 + h.eps)));
-                if (a.zero_grad) g[i] = AwType<GT>::put(0.0f);
-            }
-            const unsigned um = __float_as_uint(mm[j]) & 0x7FFFFFFFu, ur = __float_as_uint(rr[j]) & 0x7FFFFFFFu;
-            bm = um > bm ? um : bm;                   // order of the bits = order of the magnitudes, NaN above infinity
-            br = ur > br ? ur : br;
+            a.c[j] = i + j < n ? mc[i + j] : (signed char)0;
+            b.c[j] = i + j < n ? rc[i + j] : (unsigned char)0;
         }
-        for (int d = 32; d; d >>= 1) {
-            const unsigned om = __shfl_xor(bm, d), orr = __shfl_xor(br, d);
-            bm = om > bm ? om : bm;
-            br = orr > br ? orr : br;
-        }
-        const float fm = __uint_as_float(bm), fr = __uint_as_float(br);
-        const bool fine_m = bm < 0x7F800000u, fine_r = br < 0x7F800000u;
-        const bool some_m = fine_m && fm > 7.8886090522101181e-31f, some_r = fine_r && fr > 0.0f;      // 2^-100: 127^2 / max stays finite
-        const float im = some_m ? 16129.0f / fm : 0.0f, ir = some_r ? 65025.0f / fr : 0.0f;
-        const unsigned kb = aw_mix((a.key[s] + (unsigned)step * AW_GOLD) ^ aw_mix((unsigned)b));
-        for (int j = 0; j < 4; ++j) {
-            const int e = j * 64 + lane;
-            const long long i = b * AW_BLOCK + e;
-            if (i >= n) continue;
-            unsigned u = kb + (unsigned)e * AW_GOLD;
-            u = (u ^ (u >> 16)) * 0x7FEB352Du;
-            u ^= u >> 15;
-            float cm = 0.0f, cr = 0.0f;
-            if (some_m) cm = fminf(aw_code(fabsf(mm[j]) * im, (float)(u & 0xFFFFu) * (1.0f / 65536.0f)), 127.0f);
-            if (some_r) cr = fminf(aw_code(rr[j] * ir, (float)(u >> 16) * (1.0f / 65536.0f)), 255.0f);
-            if (some_r && cr == 0.0f && rr[j] > 0.0f) cr = 1.0f;
-            mc[i] = (signed char)(mm[j] < 0.0f ? -(int)cm : (int)cm);
-            rc[i] = (unsigned char)(int)cr;
-        }
-        if (lane == 0) {
-            const float nan = __uint_as_float(0x7FC00000u);
-            a.scales[s][2 * b] = fine_m ? (some_m ? fm / 16129.0f : 0.0f) : nan;
-            a.scales[s][2 * b + 1] = fine_r ? (some_r ? fr / 65025.0f : 0.0f) : nan;
-        }
+    }
+    float x[4], y[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float c = (float)a.c[j], d = (float)b.c[j], r = d * d * scale.y;
+        x[j] = c * fabsf(c) * scale.x;
+        y[j] = r * r;
+    }
+    if (full) {
+        aw_store<MNE_T_F32, 4, true>(x, m, i, n);
+        aw_store<MNE_T_F32, 4, true>(y, v, i, n);
+    } else {
+        aw_store<MNE_T_F32, 4, false>(x, m, i, n);
+        aw_store<MNE_T_F32, 4, false>(y, v, i, n);
     }
 }
 
-// what 8-bit moments stand for, in 32 bits: exp_avg and exp_avg_sq
-__global__ __launch_bounds__(AW_THREADS) void adamw_moments_kernel(const signed char* mc, const unsigned char* rc, const float* scales,
-                                                                   long long n, float* m, float* v) {
-    const long long i = (long long)blockIdx.x * AW_THREADS + threadIdx.x;
-    if (i >= n) return;
-    const float sm = scales[2 * (i / AW_BLOCK)], sr = scales[2 * (i / AW_BLOCK) + 1];
-    const float c = (float)mc[i], d = (float)rc[i], r = d * d * sr;
-    m[i] = c * fabsf(c) * sm;
-    v[i] = r * r;
-}
-
 template <class Args, template <int, int> class Launch>
-static int aw_by_type(const Args& a, int pt, int gt, unsigned blocks, hipStream_t st) {
-    if (pt == MNE_T_F32 && gt == MNE_T_F32) Launch<MNE_T_F32, MNE_T_F32>::go(a, blocks, st);
-    else if (pt == MNE_T_F32 && gt == MNE_T_BF16) Launch<MNE_T_F32, MNE_T_BF16>::go(a, blocks, st);
-    else if (pt == MNE_T_F32 && gt == MNE_T_F16) Launch<MNE_T_F32, MNE_T_F16>::go(a, blocks, st);
-    else if (pt == MNE_T_BF16 && gt == MNE_T_F32) Launch<MNE_T_BF16, MNE_T_F32>::go(a, blocks, st);
-    else if (pt == MNE_T_BF16 && gt == MNE_T_BF16) Launch<MNE_T_BF16, MNE_T_BF16>::go(a, blocks, st);
-    else if (pt == MNE_T_F16 && gt == MNE_T_F32) Launch<MNE_T_F16, MNE_T_F32>::go(a, blocks, st);
-    else if (pt == MNE_T_F16 && gt == MNE_T_F16) Launch<MNE_T_F16, MNE_T_F16>::go(a, blocks, st);
+static int aw_by_type(const Args& a, int pt, int gt, int per_wg, unsigned blocks, hipStream_t st) {
+    if (pt == MNE_T_F32 && gt == MNE_T_F32) Launch<MNE_T_F32, MNE_T_F32>::go(a, per_wg, blocks, st);
+    else if (pt == MNE_T_F32 && gt == MNE_T_BF16) Launch<MNE_T_F32, MNE_T_BF16>::go(a, per_wg, blocks, st);
+    else if (pt == MNE_T_F32 && gt == MNE_T_F16) Launch<MNE_T_F32, MNE_T_F16>::go(a, per_wg, blocks, st);
+    else if (pt == MNE_T_BF16 && gt == MNE_T_F32) Launch<MNE_T_BF16, MNE_T_F32>::go(a, per_wg, blocks, st);
+    else if (pt == MNE_T_BF16 && gt == MNE_T_BF16) Launch<MNE_T_BF16, MNE_T_BF16>::go(a, per_wg, blocks, st);
+    else if (pt == MNE_T_F16 && gt == MNE_T_F32) Launch<MNE_T_F16, MNE_T_F32>::go(a, per_wg, blocks, st);
+    else if (pt == MNE_T_F16 && gt == MNE_T_F16) Launch<MNE_T_F16, MNE_T_F16>::go(a, per_wg, blocks, st);
     else return -1;
     return 0;
 }
 template <int PT, int GT> struct Launch32 {
-    static void go(const Adamw32Args& a, unsigned blocks, hipStream_t st) { MNE_LAUNCH((adamw32_kernel<PT, GT>), blocks, AW_THREADS, 0, st, a); }
+    static void go(const Adamw32Args& a, int per_wg, unsigned blocks, hipStream_t st) {
+        if (per_wg == AW_SMALL_WG) MNE_LAUNCH((adamw32_kernel<PT, GT, AW_SMALL_WG / AW_THREADS>), blocks, AW_THREADS, 0, st, a);
+        else MNE_LAUNCH((adamw32_kernel<PT, GT, AW32_WG / AW_THREADS>), blocks, AW_THREADS, 0, st, a);
+    }
 };
 template <int PT, int GT> struct Launch8 {
-    static void go(const Adamw8Args& a, unsigned blocks, hipStream_t st) { MNE_LAUNCH((adamw8_kernel<PT, GT>), blocks, AW_THREADS, 0, st, a); }
+    static void go(const Adamw8Args& a, int per_wg, unsigned blocks, hipStream_t st) {
+        if (per_wg == AW_SMALL_WG) MNE_LAUNCH((adamw8_kernel<PT, GT, AW_THREADS * AW_BLOCK / AW_SMALL_WG>), blocks, AW_THREADS, 0, st, a);
+        else MNE_LAUNCH((adamw8_kernel<PT, GT, AW_THREADS * AW_BLOCK / AW8_WG>), blocks, AW_THREADS, 0, st, a);
+    }
 };
 
-int mne_launch_adamw32(const Adamw32Args& a, int p_type, int g_type, unsigned blocks, hipStream_t st) {
-    return aw_by_type<Adamw32Args, Launch32>(a, p_type, g_type, blocks, st);
+int mne_launch_adamw32(const Adamw32Args& a, int p_type, int g_type, int per_wg, unsigned blocks, hipStream_t st) {
+    return aw_by_type<Adamw32Args, Launch32>(a, p_type, g_type, per_wg, blocks, st);
 }
-int mne_launch_adamw8(const Adamw8Args& a, int p_type, int g_type, unsigned blocks, hipStream_t st) {
-    return aw_by_type<Adamw8Args, Launch8>(a, p_type, g_type, blocks, st);
+int mne_launch_adamw8(const Adamw8Args& a, int p_type, int g_type, int per_wg, unsigned blocks, hipStream_t st) {
+    return aw_by_type<Adamw8Args, Launch8>(a, p_type, g_type, per_wg, blocks, st);
 }
 int mne_launch_adamw_moments(const signed char* mc, const unsigned char* rc, const float* scales, long long n, float* m, float* v, hipStream_t st) {
-    MNE_LAUNCH(adamw_moments_kernel, (unsigned)((n + AW_THREADS - 1) / AW_THREADS), AW_THREADS, 0, st, mc, rc, scales, n, m, v);
+    const int aligned = ((uintptr_t)mc % 4 | (uintptr_t)rc % 4 | (uintptr_t)m % 16 | (uintptr_t)v % 16) == 0;
+    MNE_LAUNCH(adamw_moments_kernel, (unsigned)((n + 4 * AW_THREADS - 1) / (4 * AW_THREADS)), AW_THREADS, 0, st, mc, rc, scales, n, m, v, aligned);
     return 0;
 }
-long long mne_adamw_blocks_for(long long n) { return (n + AW_PER_WG - 1) / AW_PER_WG; }
+int mne_adamw_per_wg(long long elements, int state_bits) {
+    return elements <= AW_SMALL ? AW_SMALL_WG : state_bits == 8 ? AW8_WG : AW32_WG;
+}
 unsigned mne_adamw_key(unsigned seed, unsigned ordinal) {
     unsigned h = seed + ordinal * AW_GOLD;
     h = (h ^ (h >> 16)) * 0x7FEB352Du;

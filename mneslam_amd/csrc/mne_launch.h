@@ -323,6 +323,7 @@ struct Adamw32Args {
     void *p[MNE_ADAMW32_SEGS], *g[MNE_ADAMW32_SEGS], *m[MNE_ADAMW32_SEGS], *v[MNE_ADAMW32_SEGS];
     long long n[MNE_ADAMW32_SEGS];
     int first[MNE_ADAMW32_SEGS];
+    unsigned char aligned[MNE_ADAMW32_SEGS];      // every address a multiple of 16 bytes
 };
 struct Adamw8Args {
     AdamwHyper h;
@@ -333,13 +334,14 @@ struct Adamw8Args {
     long long n[MNE_ADAMW8_SEGS];
     unsigned key[MNE_ADAMW8_SEGS];
     int first[MNE_ADAMW8_SEGS];
+    unsigned char aligned[MNE_ADAMW8_SEGS];       // parameter and gradient at multiples of 16 bytes, codes of 8
 };
 static_assert(sizeof(Adamw32Args) <= 4096 && sizeof(Adamw8Args) <= 4096, "kernel arguments are limited to 4 KB");
 
-int mne_launch_adamw32(const Adamw32Args& a, int p_type, int g_type, unsigned blocks, hipStream_t st);
-int mne_launch_adamw8(const Adamw8Args& a, int p_type, int g_type, unsigned blocks, hipStream_t st);
+int mne_launch_adamw32(const Adamw32Args& a, int p_type, int g_type, int per_wg, unsigned blocks, hipStream_t st);
+int mne_launch_adamw8(const Adamw8Args& a, int p_type, int g_type, int per_wg, unsigned blocks, hipStream_t st);
 int mne_launch_adamw_moments(const signed char* mc, const unsigned char* rc, const float* scales, long long n, float* m, float* v, hipStream_t st);
-long long mne_adamw_blocks_for(long long n);
+int mne_adamw_per_wg(long long elements, int state_bits);       // elements of a workgroup, by those of the whole call
 unsigned mne_adamw_key(unsigned seed, unsigned ordinal);
 
 int mne_launch_sample_z(const ZArgs& a, hipStream_t st);

@@ -4,6 +4,13 @@
 #pragma once
 #ifdef MNE_HOST_EMU
 #include "hip_emu.h"
+static inline float mne_sqrt_fast(float x) { return std::sqrt(x); }
+static inline float mne_sqrt_rn(float x) { return std::sqrt(x); }
+static inline float mne_rcp_fast(float x) { return 1.0f / x; }
+static inline unsigned mne_max16(unsigned v) {                    // largest value of the 16 lanes of a row
+    for (int d = 1; d < 16; d <<= 1) { const unsigned o = __shfl_xor(v, d); v = o > v ? o : v; }
+    return v;
+}
 // bf16 <-> fp32, rounded to nearest even
 static inline float mne_bf16_to_float(unsigned short x) { return __uint_as_float((unsigned)x << 16); }
 static inline unsigned short mne_float_to_bf16(float x) {
@@ -44,6 +51,24 @@ static __device__ __forceinline__ int mne_bcast8(int v, int k) {
     }
 }
 static __device__ __forceinline__ float mne_bcast8(float v, int k) { return __int_as_float(mne_bcast8(__float_as_int(v), k)); }
+static __device__ __forceinline__ float mne_sqrt_fast(float x) { return __builtin_amdgcn_sqrtf(x); }      // v_sqrt_f32: 1 ulp
+// The root rounded to nearest, for 0, 2^-96 and above, infinity and NaN: of s (1 ulp off) and its neighbours the one whose product with
+// the next lower one is below x and with the next higher one is not (between neighbours s < t: x > s t puts the root above their middle).
+static __device__ __forceinline__ float mne_sqrt_rn(float x) {
+    const float s = __builtin_amdgcn_sqrtf(x);
+    const float lo = __int_as_float(__float_as_int(s) - 1), hi = __int_as_float(__float_as_int(s) + 1);
+    float r = fmaf(-lo, s, x) <= 0.0f ? lo : s;
+    return fmaf(-hi, s, x) > 0.0f ? hi : r;
+}
+static __device__ __forceinline__ float mne_rcp_fast(float x) { return __builtin_amdgcn_rcpf(x); }        // v_rcp_f32: 1 ulp
+// largest value of the 16 lanes of a row: four rotations within the row, no LDS
+template <int CTRL> static __device__ __forceinline__ unsigned mne_max_ror(unsigned v) {
+    const unsigned o = (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true);
+    return o > v ? o : v;
+}
+static __device__ __forceinline__ unsigned mne_max16(unsigned v) {
+    return mne_max_ror<0x121>(mne_max_ror<0x122>(mne_max_ror<0x124>(mne_max_ror<0x128>(v))));
+}
 static __device__ __forceinline__ float mne_bf16_to_float(unsigned short x) { return __uint_as_float((unsigned)x << 16); }
 static __device__ __forceinline__ unsigned short mne_float_to_bf16(float x) {         // one v_cvt_pk_bf16_f32: to nearest even
     return __builtin_bit_cast(unsigned short, (__bf16)x);
@@ -65,3 +90,11 @@ static __device__ __forceinline__ int mne_xcc_id() {
         __builtin_amdgcn_wave_barrier();                        \
     } while (0)
 #endif
+
+// B bytes of memory that are loaded and stored as one
+template <int B> struct MneBytes;
+template <> struct MneBytes<16> { uint4 v; };
+template <> struct MneBytes<8> { uint2 v; };
+template <> struct MneBytes<4> { unsigned v; };
+template <> struct MneBytes<2> { unsigned short v; };
+template <> struct MneBytes<1> { unsigned char v; };

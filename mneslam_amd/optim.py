@@ -117,16 +117,6 @@ class FusedAdam(torch.optim.Optimizer):
 MOMENT_BLOCK = 256             # consecutive elements of an 8-bit moment that share a scale
 
 
-def _is_dense(t):
-    return t.is_contiguous() or (t.dim() == 4 and t.is_contiguous(memory_format=torch.channels_last)) \
-        or (t.dim() == 5 and t.is_contiguous(memory_format=torch.channels_last_3d))
-
-
-def _laid_out_alike(a, b):
-    """Equal strides in every dimension that has more than one entry (the shapes are equal)."""
-    return a.stride() == b.stride() or all(x == y for n, x, y in zip(a.shape, a.stride(), b.stride()) if n > 1)
-
-
 def _check_hyper(lr, betas, eps, weight_decay):
     if not 0.0 <= lr < float("inf"):
         raise ValueError(f"Invalid learning rate: {lr}")
@@ -138,7 +128,6 @@ def _check_hyper(lr, betas, eps, weight_decay):
         raise ValueError(f"Invalid weight_decay value: {weight_decay}")
 
 
-@torch.no_grad()
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, scales=None, *, step, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
                seed=0, ordinals=None, zero_grad=False, clock=None):
     """One AdamW step (decoupled decay, torch.optim.AdamW with amsgrad=False, maximize=False) over a list of tensors, in place and
@@ -157,60 +146,22 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, scales=None, *, step, lr, b
 
     ``step`` counts from 1 and is the list's; ``clock`` (mneslam_amd._lib.Clock, graph recording) adds the device's step offset.
     Without one a step is not recorded into a graph: every replay would be the same step."""
-    params, grads, exp_avgs, exp_avg_sqs = list(params), list(grads), list(exp_avgs), list(exp_avg_sqs)
-    small = scales is not None
-    scales = list(scales) if small else [None] * len(params)
-    ordinals = list(range(len(params))) if ordinals is None else [int(o) for o in ordinals]
-    if not len(params) == len(grads) == len(exp_avgs) == len(exp_avg_sqs) == len(scales) == len(ordinals):
-        raise ValueError("adamw_step: lists of different lengths")
-    lr, eps, weight_decay, step = float(lr), float(eps), float(weight_decay), int(step)
+    lr, eps, weight_decay = float(lr), float(eps), float(weight_decay)
     _check_hyper(lr, betas, eps, weight_decay)
-    if not 1 <= step < 1 << 31:
-        raise ValueError(f"adamw_step: step counts from 1, got {step}")
-    if not 0 <= int(seed) < 1 << 32 or not all(0 <= o < 1 << 32 for o in ordinals):
-        raise ValueError("adamw_step: seed and ordinals are numbers of 32 bits")
+    if not 1 <= step < 1 << 31 or not 0 <= seed < 1 << 32:
+        raise ValueError(f"adamw_step: step counts from 1 and seed is a number of 32 bits, got {step} and {seed}")
+    params = list(params)
     if not params:
         return
-    dev = _lib.one_device(params + grads + exp_avgs + exp_avg_sqs + (scales if small else []), "adamw_step")
+    lib, dev = _lib.load(), params[0].device
     if clock is None and dev.type == "cuda" and torch.cuda.is_current_stream_capturing():
         raise RuntimeError("adamw_step: recording a step needs a clock (the step count would be the same at every replay)")
-    m_type, v_type = (torch.int8, torch.uint8) if small else (torch.float32, torch.float32)
-    tables, keep, seen = {}, [], set()
-    for p, g, m, v, s, o in zip(params, grads, exp_avgs, exp_avg_sqs, scales, ordinals):
-        pt, gt, n = p.dtype, g.dtype, p.numel()
-        if pt not in _lib.T_CODES or not (gt == pt or gt == torch.float32 or (pt == torch.float32 and gt in _lib.T_CODES)):
-            raise TypeError(f"adamw_step: parameter {pt} with gradient {gt} is not supported")
-        if g.layout != torch.strided or g.shape != p.shape or m.shape != p.shape or v.shape != p.shape:
-            raise ValueError("adamw_step: gradient and moments need their parameter's shape")
-        if m.dtype != m_type or v.dtype != v_type:
-            raise TypeError(f"adamw_step: moments must be {m_type} and {v_type}")
-        if n == 0:
-            continue
-        if not _is_dense(p):
-            raise ValueError("adamw_step: parameters must be dense (contiguous or channels_last)")
-        if not (_laid_out_alike(m, p) and _laid_out_alike(v, p)):
-            raise ValueError("adamw_step: moments must be laid out like their parameter")
-        if not _laid_out_alike(g, p):
-            if zero_grad:
-                raise ValueError("adamw_step: zero_grad needs gradients laid out like their parameters")
-            g = torch.empty_like(p, dtype=gt).copy_(g)
-            keep.append(g)
-        if small and (s.dtype != torch.float32 or s.shape != (-(-n // MOMENT_BLOCK), 2) or not s.is_contiguous()):
-            raise ValueError("adamw_step: scales must be contiguous float32 [ceil(n / 256), 2]")
-        at = p.data_ptr()
-        if at in seen:
-            raise ValueError("adamw_step: the same parameter twice")
-        seen.add(at)
-        tables.setdefault((pt, gt), []).extend((at, g.data_ptr(), m.data_ptr(), v.data_ptr(), s.data_ptr() if small else 0, n, o))
-    lib = _lib.load()
     with _lib.device_guard(dev):
-        stream = _lib.stream_for(params[0])
-        for (pt, gt), table in tables.items():
-            cfg = _lib.AdamwCfg(lr, betas[0], betas[1], eps, weight_decay, step, 8 if small else 32, _lib.T_CODES[pt],
-                                _lib.T_CODES[gt], 1 if zero_grad else 0, int(seed))
-            _lib.check(lib.mne_adamw_step((C.c_int64 * len(table))(*table), len(table) // 7, C.byref(cfg),
-                                          C.byref(clock) if clock is not None else None, stream), "mne_adamw_step")
-    torch.autograd.graph.increment_version([p for p in params if not p.is_inference()])
+        rc = _lib.host_tensors().adamw_step(
+            _lib.address(lib, "mne_adamw_step"), params, list(grads), list(exp_avgs), list(exp_avg_sqs),
+            None if scales is None else list(scales), None if ordinals is None else list(ordinals), lr, betas[0], betas[1], eps,
+            weight_decay, step, seed, zero_grad, 0 if clock is None else C.addressof(clock), _lib.raw_stream(dev), lib.on_host)
+    _lib.check(rc, "mne_adamw_step")
 
 
 @torch.no_grad()
@@ -220,12 +171,12 @@ def adamw_moments(exp_avg, exp_avg_sq, scales):
     n = exp_avg.numel()
     if exp_avg.dtype != torch.int8 or exp_avg_sq.dtype != torch.uint8:
         raise TypeError("adamw_moments: the codes are int8 and uint8")
-    if exp_avg_sq.shape != exp_avg.shape or not _laid_out_alike(exp_avg_sq, exp_avg) or not _is_dense(exp_avg):
-        raise ValueError("adamw_moments: the codes must be dense and laid out alike")
+    m, v = torch.empty_like(exp_avg, dtype=torch.float32), torch.empty_like(exp_avg_sq, dtype=torch.float32)
+    if exp_avg_sq.shape != exp_avg.shape or not m.stride() == v.stride() == exp_avg.stride() == exp_avg_sq.stride():
+        raise ValueError("adamw_moments: the codes must be dense and laid out alike")       # (what is not dense is laid out anew)
     if scales.dtype != torch.float32 or scales.shape != (-(-n // MOMENT_BLOCK), 2) or not scales.is_contiguous():
         raise ValueError("adamw_moments: scales must be contiguous float32 [ceil(n / 256), 2]")
     dev = _lib.one_device([exp_avg, exp_avg_sq, scales], "adamw_moments")
-    m, v = torch.empty_like(exp_avg, dtype=torch.float32), torch.empty_like(exp_avg, dtype=torch.float32)
     with _lib.device_guard(dev):
         _lib.check(_lib.load().mne_adamw_moments(_lib.ptr(exp_avg), _lib.ptr(exp_avg_sq), _lib.ptr(scales), n, _lib.ptr(m), _lib.ptr(v),
                                                  _lib.stream_for(exp_avg)), "mne_adamw_moments")

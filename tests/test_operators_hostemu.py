@@ -17,6 +17,8 @@ DEV = "cpu"
 @pytest.fixture(scope="module", autouse=True)
 def emulator_library():
     import build_emu
+    from mneslam_amd import build
+    build.build_host()
     path = build_emu.build()
     _lib.unload()
     _lib.load(path)
