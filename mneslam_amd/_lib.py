@@ -241,6 +241,7 @@ def load(path=None):
             if fn() != C.sizeof(st):
                 raise RuntimeError(f"struct layout mismatch for {st.__name__}: C {fn()} vs ctypes {C.sizeof(st)}")
         lib.on_host = bool(lib.mne_runs_on_host())
+        lib.adamw_step_address = C.cast(lib.mne_adamw_step, C.c_void_p).value      # (called from host_tensors.cpp)
         _lib = lib
         return lib
 
@@ -290,11 +291,6 @@ def one_device(tensors, what):
 def device_guard(dev):
     """Makes ``dev`` the current device for a launch (the streams of another device are not the current one's)."""
     return torch.cuda.device(dev) if dev.type == "cuda" and dev.index != torch.cuda.current_device() else contextlib.nullcontext()
-
-
-def address(lib, name):
-    """Address of an entry point (for callers in C++)."""
-    return C.cast(getattr(lib, name), C.c_void_p).value
 
 
 def raw_stream(dev):

@@ -22,15 +22,14 @@
 
 #define AW_THREADS 256
 #define AW_BLOCK 256                                 // elements that share two scales
-// Elements of a workgroup.
-#ifndef AW32_WG
-#define AW32_WG 2048
-#endif
-#define AW8_WG 4096
-#define AW_SMALL_WG 1024
-#ifndef AW_SMALL
-#define AW_SMALL (1 << 20)
-#endif
+// Elements a workgroup takes: 4 a thread with 32-bit moments, and 8 a thread (32 lanes a block) with 8-bit ones.  Measured: 32-bit
+// moments, 67 M bf16 values in 256 tensors: 283 us with 4 a thread, 308 with 8, 335 with 16 (fp32 parameters: no difference); 8-bit
+// moments: 214 us with 32 lanes a block, 239 with 16, 222 with 64 in the largest launches (2^23 values: 25.3 / 25.1 / 27.8 us) and 0.5 us
+// less than 32 in the smallest (5.8 us), which the host call hides.
+#define AW_EACH32 4
+#define AW_LANES8 32
+#define AW_WG32 (AW_THREADS * AW_EACH32)
+#define AW_WG8 (AW_THREADS / AW_LANES8 * AW_BLOCK)
 
 __device__ __forceinline__ unsigned aw_mix(unsigned h) {      // a multiply-xorshift mix of 32 bits
     h = (h ^ (h >> 16)) * 0x7FEB352Du;
@@ -104,9 +103,9 @@ __device__ __forceinline__ void aw_store(const float* x, void* base, long long i
 // Consecutive elements of a thread's pieces: 16 bytes of the parameter, as far as the thread has that many.
 template <int PT, int EACH> struct AwPiece { static constexpr int N = PT == MNE_T_F32 || EACH < 8 ? 4 : 8; };
 
-template <int PT, int GT, int EACH, bool FULL>
+template <int PT, int GT, bool FULL>
 __device__ __forceinline__ void adamw32_body(const Adamw32Args& a, const AdamwHyper& h, int s, long long base) {
-    constexpr int N = AwPiece<PT, EACH>::N, K = EACH / N;
+    constexpr int N = AwPiece<PT, AW_EACH32>::N, K = AW_EACH32 / N;
     const long long n = a.n[s], i0 = base + threadIdx.x * N;
     float p[K][N], g[K][N], m[K][N], v[K][N];
 #pragma unroll
@@ -134,14 +133,14 @@ __device__ __forceinline__ void adamw32_body(const Adamw32Args& a, const AdamwHy
     }
 }
 
-template <int PT, int GT, int EACH>
+template <int PT, int GT>
 __global__ __launch_bounds__(AW_THREADS) void adamw32_kernel(Adamw32Args a) {
     const int s = aw_segment(a.first, a.n_seg, (int)blockIdx.x);
     AdamwHyper h = a.h;
     if (a.clk.bias_table) clock_bias(a.clk, h.lr, h.step, h.step_size, h.root_bc2);
-    const long long base = (long long)((int)blockIdx.x - a.first[s]) * (AW_THREADS * EACH);
-    if (a.aligned[s] && base + AW_THREADS * EACH <= a.n[s]) adamw32_body<PT, GT, EACH, true>(a, h, s, base);
-    else adamw32_body<PT, GT, EACH, false>(a, h, s, base);
+    const long long base = (long long)((int)blockIdx.x - a.first[s]) * AW_WG32;
+    if (a.aligned[s] && base + AW_WG32 <= a.n[s]) adamw32_body<PT, GT, true>(a, h, s, base);
+    else adamw32_body<PT, GT, false>(a, h, s, base);
 }
 
 // Code of x in 0..most^2 with the dither k / 65536: floor of the root, or one more if k / 65536 (2 c + 1) < x - c^2.  The floor is exact
@@ -153,20 +152,20 @@ __device__ __forceinline__ int aw_code(float x, unsigned k) {
     return (float)k * fmaf(f, 2.0f / 65536.0f, 1.0f / 65536.0f) < x - f * f ? c + 1 : c;
 }
 
-template <int LANES> __device__ __forceinline__ unsigned aw_max(unsigned x) {
+__device__ __forceinline__ unsigned aw_max(unsigned x) {        // over the lanes of a block
     x = mne_max16(x);
 #pragma unroll
-    for (int d = 16; d < LANES; d <<= 1) {
+    for (int d = 16; d < AW_LANES8; d <<= 1) {
         const unsigned o = __shfl_xor(x, d);
         x = o > x ? o : x;
     }
     return x;
 }
 
-// LANES lanes have a block of 256, EACH = 256 / LANES elements each.
-template <int PT, int GT, int LANES, bool FULL>
+// LANES lanes have a block of 256 elements, EACH of them each.
+template <int PT, int GT, bool FULL>
 __device__ __forceinline__ void adamw8_body(const Adamw8Args& a, const AdamwHyper& h, int step, int s, long long b) {
-    constexpr int EACH = AW_BLOCK / LANES, N = AwPiece<PT, EACH>::N, K = EACH / N;
+    constexpr int LANES = AW_LANES8, EACH = AW_BLOCK / LANES, N = AwPiece<PT, EACH>::N, K = EACH / N;
     const int l = threadIdx.x % LANES;
     const long long n = a.n[s], i0 = b * AW_BLOCK + l * N;
     const bool there = FULL || b * AW_BLOCK < n;
@@ -240,7 +239,7 @@ __device__ __forceinline__ void adamw8_body(const Adamw8Args& a, const AdamwHype
             br = ur > br ? ur : br;
         }
     unsigned bm = __float_as_uint(most);
-    br = aw_max<LANES>(br);
+    br = aw_max(br);
     if (__ballot(br >= 0x7F800000u)) {                // (the whole wave goes this way)
         bm = 0;
 #pragma unroll
@@ -251,11 +250,15 @@ __device__ __forceinline__ void adamw8_body(const Adamw8Args& a, const AdamwHype
                 bm = um > bm ? um : bm;
             }
     }
-    bm = aw_max<LANES>(bm);
+    bm = aw_max(bm);
     const bool fine_m = bm < 0x7F800000u, fine_r = br < 0x7F800000u;
     const float fm = __uint_as_float(bm), fr = __uint_as_float(br);
     const bool some_m = fine_m && fm > 7.8886090522101181e-31f, some_r = fine_r && fr > 0.0f;      // 2^-100: 127^2 / max stays finite
-    const float im = some_m ? 16129.0f / fm : 0.0f, ir = some_r ? 65025.0f / fr : 0.0f;
+    // Four quotients a block, one for each lane of four: 127^2 / max |m|, 255^2 / max sqrt(v), and the scales the other way round.
+    const int q = l & 3;
+    const float top = q & 1 ? 65025.0f : 16129.0f, big = q & 1 ? fr : fm, quotient = q & 2 ? big / top : top / big;
+    const float up_m = mne_quad(quotient, 0), up_r = mne_quad(quotient, 1), scale_m = mne_quad(quotient, 2), scale_r = mne_quad(quotient, 3);
+    const float im = some_m ? up_m : 0.0f, ir = some_r ? up_r : 0.0f;
     if (!(fine_m && fine_r)) {                        // codes 0 in what is not finite
 #pragma unroll
         for (int k = 0; k < K; ++k)
@@ -265,7 +268,15 @@ __device__ __forceinline__ void adamw8_body(const Adamw8Args& a, const AdamwHype
                 if (!fine_r) r[k][j] = 0.0f;
             }
     }
-    const unsigned kb = aw_mix((a.key[s] + (unsigned)step * AW_GOLD) ^ aw_mix((unsigned)b)) + (unsigned)(l * N) * AW_GOLD;
+    // (the blocks of a wave one after the other: their numbers are the wave's, so the scalar unit does this)
+    const unsigned key = a.key[s] + (unsigned)step * AW_GOLD, b0 = (unsigned)mne_first_lane((int)b);
+    unsigned kb = aw_mix(key ^ aw_mix(b0));
+#pragma unroll
+    for (int k = 1; k < 64 / LANES; ++k) {
+        const unsigned other = aw_mix(key ^ aw_mix(b0 + (unsigned)k));
+        kb = (threadIdx.x & 63) / LANES == k ? other : kb;
+    }
+    kb += (unsigned)(l * N) * AW_GOLD;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         const long long i = i0 + k * (LANES * N);
@@ -293,11 +304,11 @@ __device__ __forceinline__ void adamw8_body(const Adamw8Args& a, const AdamwHype
     }
     if (l == 0 && there) {
         const float nan = __uint_as_float(0x7FC00000u);
-        ((float2*)a.scales[s])[b] = make_float2(fine_m ? (some_m ? fm / 16129.0f : 0.0f) : nan, fine_r ? (some_r ? fr / 65025.0f : 0.0f) : nan);
+        ((float2*)a.scales[s])[b] = make_float2(fine_m ? (some_m ? scale_m : 0.0f) : nan, fine_r ? (some_r ? scale_r : 0.0f) : nan);
     }
 }
 
-template <int PT, int GT, int LANES>
+template <int PT, int GT>
 __global__ __launch_bounds__(AW_THREADS) void adamw8_kernel(Adamw8Args a) {
     const int s = aw_segment(a.first, a.n_seg, (int)blockIdx.x);
     AdamwHyper h = a.h;
@@ -306,10 +317,10 @@ __global__ __launch_bounds__(AW_THREADS) void adamw8_kernel(Adamw8Args a) {
         clock_bias(a.clk, h.lr, h.step, h.step_size, h.root_bc2);
         step += *a.clk.step_offset;
     }
-    constexpr int BLOCKS = AW_THREADS / LANES;
-    const long long wg = (int)blockIdx.x - a.first[s], b = wg * BLOCKS + threadIdx.x / LANES;
-    if (a.aligned[s] && (wg + 1) * (BLOCKS * AW_BLOCK) <= a.n[s]) adamw8_body<PT, GT, LANES, true>(a, h, step, s, b);
-    else adamw8_body<PT, GT, LANES, false>(a, h, step, s, b);
+    constexpr int BLOCKS = AW_THREADS / AW_LANES8;
+    const long long wg = (int)blockIdx.x - a.first[s], b = wg * BLOCKS + threadIdx.x / AW_LANES8;
+    if (a.aligned[s] && (wg + 1) * AW_WG8 <= a.n[s]) adamw8_body<PT, GT, true>(a, h, step, s, b);
+    else adamw8_body<PT, GT, false>(a, h, step, s, b);
 }
 
 // what 8-bit moments stand for, in 32 bits: exp_avg and exp_avg_sq, four elements a thread
@@ -347,44 +358,36 @@ __global__ __launch_bounds__(AW_THREADS) void adamw_moments_kernel(const signed 
 }
 
 template <class Args, template <int, int> class Launch>
-static int aw_by_type(const Args& a, int pt, int gt, int per_wg, unsigned blocks, hipStream_t st) {
-    if (pt == MNE_T_F32 && gt == MNE_T_F32) Launch<MNE_T_F32, MNE_T_F32>::go(a, per_wg, blocks, st);
-    else if (pt == MNE_T_F32 && gt == MNE_T_BF16) Launch<MNE_T_F32, MNE_T_BF16>::go(a, per_wg, blocks, st);
-    else if (pt == MNE_T_F32 && gt == MNE_T_F16) Launch<MNE_T_F32, MNE_T_F16>::go(a, per_wg, blocks, st);
-    else if (pt == MNE_T_BF16 && gt == MNE_T_F32) Launch<MNE_T_BF16, MNE_T_F32>::go(a, per_wg, blocks, st);
-    else if (pt == MNE_T_BF16 && gt == MNE_T_BF16) Launch<MNE_T_BF16, MNE_T_BF16>::go(a, per_wg, blocks, st);
-    else if (pt == MNE_T_F16 && gt == MNE_T_F32) Launch<MNE_T_F16, MNE_T_F32>::go(a, per_wg, blocks, st);
-    else if (pt == MNE_T_F16 && gt == MNE_T_F16) Launch<MNE_T_F16, MNE_T_F16>::go(a, per_wg, blocks, st);
+static int aw_by_type(const Args& a, int pt, int gt, unsigned blocks, hipStream_t st) {
+    if (pt == MNE_T_F32 && gt == MNE_T_F32) Launch<MNE_T_F32, MNE_T_F32>::go(a, blocks, st);
+    else if (pt == MNE_T_F32 && gt == MNE_T_BF16) Launch<MNE_T_F32, MNE_T_BF16>::go(a, blocks, st);
+    else if (pt == MNE_T_F32 && gt == MNE_T_F16) Launch<MNE_T_F32, MNE_T_F16>::go(a, blocks, st);
+    else if (pt == MNE_T_BF16 && gt == MNE_T_F32) Launch<MNE_T_BF16, MNE_T_F32>::go(a, blocks, st);
+    else if (pt == MNE_T_BF16 && gt == MNE_T_BF16) Launch<MNE_T_BF16, MNE_T_BF16>::go(a, blocks, st);
+    else if (pt == MNE_T_F16 && gt == MNE_T_F32) Launch<MNE_T_F16, MNE_T_F32>::go(a, blocks, st);
+    else if (pt == MNE_T_F16 && gt == MNE_T_F16) Launch<MNE_T_F16, MNE_T_F16>::go(a, blocks, st);
     else return -1;
     return 0;
 }
 template <int PT, int GT> struct Launch32 {
-    static void go(const Adamw32Args& a, int per_wg, unsigned blocks, hipStream_t st) {
-        if (per_wg == AW_SMALL_WG) MNE_LAUNCH((adamw32_kernel<PT, GT, AW_SMALL_WG / AW_THREADS>), blocks, AW_THREADS, 0, st, a);
-        else MNE_LAUNCH((adamw32_kernel<PT, GT, AW32_WG / AW_THREADS>), blocks, AW_THREADS, 0, st, a);
-    }
+    static void go(const Adamw32Args& a, unsigned blocks, hipStream_t st) { MNE_LAUNCH((adamw32_kernel<PT, GT>), blocks, AW_THREADS, 0, st, a); }
 };
 template <int PT, int GT> struct Launch8 {
-    static void go(const Adamw8Args& a, int per_wg, unsigned blocks, hipStream_t st) {
-        if (per_wg == AW_SMALL_WG) MNE_LAUNCH((adamw8_kernel<PT, GT, AW_THREADS * AW_BLOCK / AW_SMALL_WG>), blocks, AW_THREADS, 0, st, a);
-        else MNE_LAUNCH((adamw8_kernel<PT, GT, AW_THREADS * AW_BLOCK / AW8_WG>), blocks, AW_THREADS, 0, st, a);
-    }
+    static void go(const Adamw8Args& a, unsigned blocks, hipStream_t st) { MNE_LAUNCH((adamw8_kernel<PT, GT>), blocks, AW_THREADS, 0, st, a); }
 };
 
-int mne_launch_adamw32(const Adamw32Args& a, int p_type, int g_type, int per_wg, unsigned blocks, hipStream_t st) {
-    return aw_by_type<Adamw32Args, Launch32>(a, p_type, g_type, per_wg, blocks, st);
+int mne_launch_adamw32(const Adamw32Args& a, int p_type, int g_type, unsigned blocks, hipStream_t st) {
+    return aw_by_type<Adamw32Args, Launch32>(a, p_type, g_type, blocks, st);
 }
-int mne_launch_adamw8(const Adamw8Args& a, int p_type, int g_type, int per_wg, unsigned blocks, hipStream_t st) {
-    return aw_by_type<Adamw8Args, Launch8>(a, p_type, g_type, per_wg, blocks, st);
+int mne_launch_adamw8(const Adamw8Args& a, int p_type, int g_type, unsigned blocks, hipStream_t st) {
+    return aw_by_type<Adamw8Args, Launch8>(a, p_type, g_type, blocks, st);
 }
 int mne_launch_adamw_moments(const signed char* mc, const unsigned char* rc, const float* scales, long long n, float* m, float* v, hipStream_t st) {
     const int aligned = ((uintptr_t)mc % 4 | (uintptr_t)rc % 4 | (uintptr_t)m % 16 | (uintptr_t)v % 16) == 0;
     MNE_LAUNCH(adamw_moments_kernel, (unsigned)((n + 4 * AW_THREADS - 1) / (4 * AW_THREADS)), AW_THREADS, 0, st, mc, rc, scales, n, m, v, aligned);
     return 0;
 }
-int mne_adamw_per_wg(long long elements, int state_bits) {
-    return elements <= AW_SMALL ? AW_SMALL_WG : state_bits == 8 ? AW8_WG : AW32_WG;
-}
+int mne_adamw_per_wg(int state_bits) { return state_bits == 8 ? AW_WG8 : AW_WG32; }
 unsigned mne_adamw_key(unsigned seed, unsigned ordinal) {
     unsigned h = seed + ordinal * AW_GOLD;
     h = (h ^ (h >> 16)) * 0x7FEB352Du;

@@ -719,14 +719,12 @@ int mne_adamw_step(const int64_t* table, int64_t n_tensors, const mne_adamw_cfg_
     if (!adamw_types(cfg->p_type, cfg->g_type)) return fail(-1, "mne_adamw_step: unsupported types of parameter and gradient");
     if (cfg->step < 1) return fail(-1, "mne_adamw_step: step counts from 1");
     const bool small = cfg->state_bits == 8;
-    long long all = 0;
     const int64_t psize = cfg->p_type == MNE_T_F32 ? 4 : 2, gsize = cfg->g_type == MNE_T_F32 ? 4 : 2;
     for (int64_t i = 0; i < n_tensors; ++i) {               // nothing is launched unless every row is sound
         const int64_t* t = table + 7 * i;
         if (t[5] < 0 || t[5] > (1ll << 42)) return fail(-1, "mne_adamw_step: bad number of elements");
         if (t[5] && (!t[0] || !t[1] || !t[2] || !t[3] || (small && !t[4]))) return fail(-1, "mne_adamw_step: NULL address");
         if (t[0] % psize || t[1] % gsize || (small ? t[4] % 8 : t[2] % 4 || t[3] % 4)) return fail(-1, "mne_adamw_step: misaligned address");
-        all += t[5];
     }
     AdamwHyper h = {};
     const double bc1 = 1.0 - std::pow(cfg->beta1, (double)cfg->step), bc2 = 1.0 - std::pow(cfg->beta2, (double)cfg->step);
@@ -742,7 +740,7 @@ int mne_adamw_step(const int64_t* table, int64_t n_tensors, const mne_adamw_cfg_
     Adamw32Args a32;
     Adamw8Args a8;
     a32.h = a8.h = h; a32.clk = a8.clk = clk; a32.zero_grad = a8.zero_grad = cfg->zero_grad;
-    const int per_wg = mne_adamw_per_wg(all, cfg->state_bits);
+    const int per_wg = mne_adamw_per_wg(cfg->state_bits);
     int n_seg = 0;
     long long blocks = 0;
     for (int64_t i = 0; i <= n_tensors; ++i) {
@@ -750,8 +748,8 @@ int mne_adamw_step(const int64_t* table, int64_t n_tensors, const mne_adamw_cfg_
         const long long more = i < n_tensors ? (t[5] + per_wg - 1) / per_wg : 0;
         if (n_seg && (i == n_tensors || n_seg == (small ? MNE_ADAMW8_SEGS : MNE_ADAMW32_SEGS) || blocks + more > 0x7FFFFFFFll)) {
             a32.n_seg = a8.n_seg = n_seg;
-            if (small) mne_launch_adamw8(a8, cfg->p_type, cfg->g_type, per_wg, (unsigned)blocks, (hipStream_t)stream);
-            else mne_launch_adamw32(a32, cfg->p_type, cfg->g_type, per_wg, (unsigned)blocks, (hipStream_t)stream);
+            if (small) mne_launch_adamw8(a8, cfg->p_type, cfg->g_type, (unsigned)blocks, (hipStream_t)stream);
+            else mne_launch_adamw32(a32, cfg->p_type, cfg->g_type, (unsigned)blocks, (hipStream_t)stream);
             if (check_launch("adamw_step")) return -10;
             n_seg = 0; blocks = 0;
         }

@@ -11,6 +11,8 @@ static inline unsigned mne_max16(unsigned v) {                    // largest val
     for (int d = 1; d < 16; d <<= 1) { const unsigned o = __shfl_xor(v, d); v = o > v ? o : v; }
     return v;
 }
+static inline float mne_quad(float v, int k) { return __shfl(v, (int)(threadIdx.x & 60u) | k); }      // lane k's of every four lanes
+static inline int mne_first_lane(int v) { return __shfl(v, 0); }
 // bf16 <-> fp32, rounded to nearest even
 static inline float mne_bf16_to_float(unsigned short x) { return __uint_as_float((unsigned)x << 16); }
 static inline unsigned short mne_float_to_bf16(float x) {
@@ -66,6 +68,17 @@ template <int CTRL> static __device__ __forceinline__ unsigned mne_max_ror(unsig
     const unsigned o = (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true);
     return o > v ? o : v;
 }
+// lane k's value (a constant) of every four lanes
+static __device__ __forceinline__ float mne_quad(float v, int k) {
+    const int x = __float_as_int(v);
+    switch (k) {
+        case 0: return __int_as_float(__builtin_amdgcn_update_dpp(0, x, 0x00, 0xF, 0xF, true));
+        case 1: return __int_as_float(__builtin_amdgcn_update_dpp(0, x, 0x55, 0xF, 0xF, true));
+        case 2: return __int_as_float(__builtin_amdgcn_update_dpp(0, x, 0xAA, 0xF, 0xF, true));
+        default: return __int_as_float(__builtin_amdgcn_update_dpp(0, x, 0xFF, 0xF, 0xF, true));
+    }
+}
+static __device__ __forceinline__ int mne_first_lane(int v) { return __builtin_amdgcn_readfirstlane(v); }
 static __device__ __forceinline__ unsigned mne_max16(unsigned v) {
     return mne_max_ror<0x121>(mne_max_ror<0x122>(mne_max_ror<0x124>(mne_max_ror<0x128>(v))));
 }

@@ -158,7 +158,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, scales=None, *, step, lr, b
         raise RuntimeError("adamw_step: recording a step needs a clock (the step count would be the same at every replay)")
     with _lib.device_guard(dev):
         rc = _lib.host_tensors().adamw_step(
-            _lib.address(lib, "mne_adamw_step"), params, list(grads), list(exp_avgs), list(exp_avg_sqs),
+            lib.adamw_step_address, params, list(grads), list(exp_avgs), list(exp_avg_sqs),
             None if scales is None else list(scales), None if ordinals is None else list(ordinals), lr, betas[0], betas[1], eps,
             weight_decay, step, seed, zero_grad, 0 if clock is None else C.addressof(clock), _lib.raw_stream(dev), lib.on_host)
     _lib.check(rc, "mne_adamw_step")
@@ -178,8 +178,8 @@ def adamw_moments(exp_avg, exp_avg_sq, scales):
         raise ValueError("adamw_moments: scales must be contiguous float32 [ceil(n / 256), 2]")
     dev = _lib.one_device([exp_avg, exp_avg_sq, scales], "adamw_moments")
     with _lib.device_guard(dev):
-        _lib.check(_lib.load().mne_adamw_moments(_lib.ptr(exp_avg), _lib.ptr(exp_avg_sq), _lib.ptr(scales), n, _lib.ptr(m), _lib.ptr(v),
-                                                 _lib.stream_for(exp_avg)), "mne_adamw_moments")
+        _lib.check(_lib.load().mne_adamw_moments(exp_avg.data_ptr(), exp_avg_sq.data_ptr(), scales.data_ptr(), n, m.data_ptr(),
+                                                 v.data_ptr(), _lib.raw_stream(dev)), "mne_adamw_moments")
     return m, v
 
 
