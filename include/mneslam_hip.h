@@ -529,6 +529,30 @@ int mne_adamw_step(const int64_t* table, int64_t n_tensors, const mne_adamw_cfg_
 /* exp_avg [n] and exp_avg_sq [n] in fp32 of n elements' codes and scales (as above; one run that starts with a block). */
 int mne_adamw_moments(const int8_t* m, const uint8_t* v, const float* scales, int64_t n, float* exp_avg, float* exp_avg_sq, void* stream);
 
+/* ---- tokens sorted by expert, dealt to its rows, and blended back ----------------------------- */
+/* Slot n * k + j holds the expert of token n's choice j (int32, or int64 with wide != 0); m = n * k slots.  An id outside
+ * 0 .. experts - 1 names no expert: its slot has no row.
+ * mne_expert_sort: stable sort of the slots by expert.  offsets [experts + 1]: the rows of expert e are offsets[e] .. offsets[e + 1] - 1;
+ * order [m]: the slot of a row, -1 behind the last live row;  position [m]: the row of a slot, -1 where it has none.
+ * `workspace` is scratch of mne_expert_sort_workspace_bytes(m, experts) bytes.  experts 1 .. 4096, m < 2^31. */
+size_t mne_expert_sort_workspace_bytes(int64_t m, int experts);
+int mne_expert_sort(const void* ids, int wide, int64_t m, int experts, int32_t* order, int32_t* position, int32_t* offsets,
+                    void* workspace, size_t workspace_bytes, void* stream);
+/* Rows of `width` elements of one type (MNE_T_*); strides are elements between rows of what is read, what is written is dense.
+ * `position` [n][k] and `live` (= offsets + experts: the number of live rows, on the device) are what mne_expert_sort left for these
+ * n * k slots.
+ * dispatch: out [n*k][width]: out[position[n][j]] = x[n]; rows behind the live ones are zero.
+ * combine:  out [n][width] = sum_j w[n][j] y[position[n][j]] in fp32, j = 0, 1, ... (weights NULL: all 1; the gradient of dispatch).
+ * combine_backward: dy [n*k][width]: dy[position[n][j]] = w[n][j] dout[n], zero behind the live rows; dw [n][j] = <dout[n],
+ * y[position[n][j]]>, 0 without a row.  dy or dw (and then y) may be NULL. */
+int mne_expert_dispatch(const void* x, int64_t x_stride, int type, int64_t n, int k, int64_t width, const int32_t* position,
+                        const int32_t* live, void* out, void* stream);
+int mne_expert_combine(const void* y, int64_t y_stride, int type, int64_t n, int k, int64_t width, const int32_t* position,
+                       const float* weights, void* out, void* stream);
+int mne_expert_combine_backward(const void* dout, int64_t dout_stride, const void* y, int64_t y_stride, int type, int64_t n, int k,
+                                int64_t width, const int32_t* position, const int32_t* live, const float* weights, void* dy,
+                                float* dw, void* stream);
+
 /* ---- point queries (forward only) -------------------------------------------------------- */
 /* Replaces JointEncoding.query_color_sdf / query_sdf / run_network_flat (scene_rep.py:232-331):
  * raw [N][4] for arbitrary points [N][3]; geo (optional) [N][geo_feat_dim]; feat (optional)

@@ -128,6 +128,12 @@ _PROTOS = {
     "mne_runs_on_host": (C.c_int, []),
     "mne_adamw_step": (C.c_int, [C.c_void_p, C.c_int64, C.POINTER(AdamwCfg), C.POINTER(Clock), C.c_void_p]),
     "mne_adamw_moments": (C.c_int, [C.c_void_p] * 3 + [C.c_int64] + [C.c_void_p] * 3),
+    "mne_expert_sort_workspace_bytes": (C.c_size_t, [C.c_int64, C.c_int]),
+    "mne_expert_sort": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_int] + [C.c_void_p] * 4 + [C.c_size_t, C.c_void_p]),
+    "mne_expert_dispatch": (C.c_int, [C.c_void_p, C.c_int64, C.c_int, C.c_int64, C.c_int, C.c_int64] + [C.c_void_p] * 4),
+    "mne_expert_combine": (C.c_int, [C.c_void_p, C.c_int64, C.c_int, C.c_int64, C.c_int, C.c_int64] + [C.c_void_p] * 4),
+    "mne_expert_combine_backward": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int, C.c_int64, C.c_int, C.c_int64]
+                                    + [C.c_void_p] * 6),
     "mne_sample_batch": (C.c_int, [C.c_void_p, C.c_int64, C.c_int, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_int,
                                    C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_uint64, C.c_uint64] + [C.c_void_p] * 5
                          + [C.POINTER(RenderCfg), C.c_void_p, C.c_void_p, C.c_uint64] + [C.c_void_p] * 5 + [C.POINTER(Clock), C.c_void_p]),

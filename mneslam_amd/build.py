@@ -27,8 +27,8 @@ INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 LIB = os.path.join(HERE, "libmneslam_hip.so")
 HOST_LIB = os.path.join(HERE, "_host_tensors.so")
 FUZZ_DIR = os.path.join(HERE, "_fuzz")
-SOURCES = ["capi.hip", "render.hip", "wgrad.hip", "adam.hip", "adamw.hip", "sampler.hip", "tile_adam.hip", "gridenc.hip", "pose.hip", "encodings.hip"]
-HEADERS = ["mne_device.h", "mne_launch.h", "mne_platform.h", "mlp_mfma.h"]
+SOURCES = ["capi.hip", "render.hip", "wgrad.hip", "adam.hip", "adamw.hip", "sampler.hip", "tile_adam.hip", "gridenc.hip", "pose.hip", "encodings.hip", "routing.hip"]
+HEADERS = ["mne_device.h", "mne_elem.h", "mne_launch.h", "mne_platform.h", "mlp_mfma.h"]
 
 # -packed-fp32-ops: no v_pk_{add,mul,fma}_f32 in the device code (some of their forms have given wrong results now and then); the
 # host pass of hipcc does not know the feature and says so, which is harmless

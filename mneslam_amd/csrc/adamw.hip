@@ -18,6 +18,7 @@
 // What enters the codes is plain IEEE fp32 in the order written here (the build forbids contraction), so the codes do not depend on
 // the launch or on the machine.
 #include "mne_device.h"
+#include "mne_elem.h"
 #include "mne_launch.h"
 
 #define AW_THREADS 256
@@ -38,23 +39,6 @@ __device__ __forceinline__ unsigned aw_mix(unsigned h) {      // a multiply-xors
 }
 #define AW_GOLD 0x9E3779B1u
 
-template <int T> struct AwType;                      // how an element is held: MNE_T_F32 / _BF16 / _F16
-template <> struct AwType<MNE_T_F32> {
-    typedef float mem;
-    static __device__ __forceinline__ float get(mem x) { return x; }
-    static __device__ __forceinline__ mem put(float x) { return x; }
-};
-template <> struct AwType<MNE_T_BF16> {
-    typedef unsigned short mem;
-    static __device__ __forceinline__ float get(mem x) { return mne_bf16_to_float(x); }
-    static __device__ __forceinline__ mem put(float x) { return mne_float_to_bf16(x); }
-};
-template <> struct AwType<MNE_T_F16> {
-    typedef _Float16 mem;
-    static __device__ __forceinline__ float get(mem x) { return (float)x; }
-    static __device__ __forceinline__ mem put(float x) { return (_Float16)x; }
-};
-
 // the tensor that workgroup `blk` works on: first[s] <= blk < first[s + 1]
 __device__ __forceinline__ int aw_segment(const int* first, int n, int blk) {
     int lo = 0, hi = n - 1;
@@ -69,7 +53,7 @@ __device__ __forceinline__ int aw_segment(const int* first, int n, int blk) {
 // and only those below n (zeros stand for the others).
 template <int T, int N, bool FULL>
 __device__ __forceinline__ void aw_load(float* out, const void* base, long long i, long long n) {
-    typedef typename AwType<T>::mem mem;
+    typedef typename MneElem<T>::mem mem;
     const mem* q = (const mem*)base + i;
     if (FULL) {
         constexpr int B = N * (int)sizeof(mem) < 16 ? N * (int)sizeof(mem) : 16;
@@ -77,26 +61,26 @@ __device__ __forceinline__ void aw_load(float* out, const void* base, long long 
 #pragma unroll
         for (int k = 0; k < N * (int)sizeof(mem) / B; ++k) r.v[k] = ((const MneBytes<B>*)q)[k];
 #pragma unroll
-        for (int k = 0; k < N; ++k) out[k] = AwType<T>::get(r.e[k]);
+        for (int k = 0; k < N; ++k) out[k] = MneElem<T>::get(r.e[k]);
     } else {
 #pragma unroll
-        for (int k = 0; k < N; ++k) out[k] = i + k < n ? AwType<T>::get(q[k]) : 0.0f;
+        for (int k = 0; k < N; ++k) out[k] = i + k < n ? MneElem<T>::get(q[k]) : 0.0f;
     }
 }
 template <int T, int N, bool FULL>
 __device__ __forceinline__ void aw_store(const float* x, void* base, long long i, long long n) {
-    typedef typename AwType<T>::mem mem;
+    typedef typename MneElem<T>::mem mem;
     mem* q = (mem*)base + i;
     if (FULL) {
         constexpr int B = N * (int)sizeof(mem) < 16 ? N * (int)sizeof(mem) : 16;
         union { MneBytes<B> v[N * sizeof(mem) / B]; mem e[N]; } r;
 #pragma unroll
-        for (int k = 0; k < N; ++k) r.e[k] = AwType<T>::put(x[k]);
+        for (int k = 0; k < N; ++k) r.e[k] = MneElem<T>::put(x[k]);
 #pragma unroll
         for (int k = 0; k < N * (int)sizeof(mem) / B; ++k) ((MneBytes<B>*)q)[k] = r.v[k];
     } else {
 #pragma unroll
-        for (int k = 0; k < N; ++k) if (i + k < n) q[k] = AwType<T>::put(x[k]);
+        for (int k = 0; k < N; ++k) if (i + k < n) q[k] = MneElem<T>::put(x[k]);
     }
 }
 

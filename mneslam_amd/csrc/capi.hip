@@ -777,6 +777,72 @@ int mne_adamw_moments(const int8_t* m, const uint8_t* v, const float* scales, in
     return check_launch("adamw_moments");
 }
 
+#define EXPERTS_MAX 4096
+size_t mne_expert_sort_workspace_bytes(int64_t m, int experts) {
+    if (m < 0 || m > 0x7FFFFFFFll || experts < 1 || experts > EXPERTS_MAX) return 0;
+    return (size_t)mne_expert_workspace_ints(m, experts) * sizeof(int32_t);
+}
+
+int mne_expert_sort(const void* ids, int wide, int64_t m, int experts, int32_t* order, int32_t* position, int32_t* offsets,
+                    void* workspace, size_t workspace_bytes, void* stream) {
+    if (experts < 1 || experts > EXPERTS_MAX) return fail(-1, "mne_expert_sort: 1 to 4096 experts");
+    if (m < 0 || m > 0x7FFFFFFFll - 65536) return fail(-1, "mne_expert_sort: too many slots for 32-bit rows");
+    if (!offsets || (m && (!ids || !order || !position))) return fail(-1, "mne_expert_sort: NULL argument");
+    if (workspace_bytes < mne_expert_sort_workspace_bytes(m, experts) || (workspace_bytes && !workspace))
+        return fail(-1, "mne_expert_sort: workspace too small");
+    ExpertSortArgs a = {};
+    a.ids = ids; a.wide = wide; a.m = (int)m; a.experts = experts;
+    a.order = order; a.position = position; a.offsets = offsets;
+    mne_launch_expert_sort(a, workspace, (hipStream_t)stream);
+    return check_launch("expert_sort");
+}
+
+static int expert_rows(ExpertRowArgs& a, const char* what, int type, int64_t n, int k, int64_t width, const int32_t* position) {
+    if (type != MNE_T_F32 && type != MNE_T_BF16 && type != MNE_T_F16) return fail(-1, std::string(what) + ": unsupported type");
+    if (n < 0 || k < 1 || n * (int64_t)k > 0x7FFFFFFFll || n > 0x7FFFFFFFll || width < 0 || width > (1ll << 28)) return fail(-1, std::string(what) + ": bad size");
+    if (n && width && !position) return fail(-1, std::string(what) + ": NULL argument");
+    const int64_t per = type == MNE_T_F32 ? 4 : 8;
+    if (n * ((width / per + per + 63) / 64 + 1) > (1ll << 31)) return fail(-1, std::string(what) + ": too many elements for one launch");
+    a.n = (int)n; a.k = k; a.width = (int)width; a.position = position;
+    return 0;
+}
+static int64_t row_bytes(int type, int64_t elements) { return elements * (type == MNE_T_F32 ? 4 : 2); }
+
+int mne_expert_dispatch(const void* x, int64_t x_stride, int type, int64_t n, int k, int64_t width, const int32_t* position,
+                        const int32_t* live, void* out, void* stream) {
+    ExpertRowArgs a = {};
+    if (int rc = expert_rows(a, "mne_expert_dispatch", type, n, k, width, position)) return rc;
+    if (n == 0 || width == 0) return 0;
+    if (!x || !live || !out) return fail(-1, "mne_expert_dispatch: NULL argument");
+    a.a = x; a.a_stride = row_bytes(type, x_stride); a.total = live; a.out = out;
+    mne_launch_expert_dispatch(a, type, (hipStream_t)stream);
+    return check_launch("expert_dispatch");
+}
+
+int mne_expert_combine(const void* y, int64_t y_stride, int type, int64_t n, int k, int64_t width, const int32_t* position,
+                       const float* weights, void* out, void* stream) {
+    ExpertRowArgs a = {};
+    if (int rc = expert_rows(a, "mne_expert_combine", type, n, k, width, position)) return rc;
+    if (n == 0 || width == 0) return 0;
+    if (!y || !out) return fail(-1, "mne_expert_combine: NULL argument");
+    a.a = y; a.a_stride = row_bytes(type, y_stride); a.weights = weights; a.out = out;
+    mne_launch_expert_combine(a, type, (hipStream_t)stream);
+    return check_launch("expert_combine");
+}
+
+int mne_expert_combine_backward(const void* dout, int64_t dout_stride, const void* y, int64_t y_stride, int type, int64_t n, int k,
+                                int64_t width, const int32_t* position, const int32_t* live, const float* weights, void* dy,
+                                float* dw, void* stream) {
+    ExpertRowArgs a = {};
+    if (int rc = expert_rows(a, "mne_expert_combine_backward", type, n, k, width, position)) return rc;
+    if (n == 0 || width == 0 || (!dy && !dw)) return 0;
+    if (!dout || !live || (dw && !y)) return fail(-1, "mne_expert_combine_backward: NULL argument");
+    a.a = dout; a.a_stride = row_bytes(type, dout_stride); a.b = y; a.b_stride = row_bytes(type, y_stride);
+    a.total = live; a.weights = weights; a.out = dy; a.dw = dw;
+    mne_launch_expert_combine_backward(a, type, (hipStream_t)stream);
+    return check_launch("expert_combine_backward");
+}
+
 int mne_encode_oneblob(int64_t n_pts, int dims, const float* x, float* out, void* stream) {
     if (!x || !out || dims < 1) return fail(-1, "mne_encode_oneblob: bad argument");
     if (n_pts <= 0) return 0;

@@ -344,6 +344,28 @@ int mne_launch_adamw_moments(const signed char* mc, const unsigned char* rc, con
 int mne_adamw_per_wg(int state_bits);       // elements of a workgroup
 unsigned mne_adamw_key(unsigned seed, unsigned ordinal);
 
+struct ExpertSortArgs {
+    const void* ids;
+    int wide, m, experts;          // ids of 64 bits; slots; experts 0 .. experts - 1
+    int per_wave, chunks;          // slots of a wave, workgroups
+    int *count, *total;            // workspace: [chunks][experts + 1], [experts + 1]
+    int *order, *position, *offsets;
+};
+struct ExpertRowArgs {
+    const void *a, *b;             // rows that are read (combine_backward: of the output's gradient, and of y)
+    void* out;
+    const int *position, *total;   // [n][k]; number of live rows
+    const float* weights;          // [n][k] or NULL
+    float* dw;                     // [n][k] or NULL
+    long long a_stride, b_stride;  // bytes between rows
+    int n, k, width, cols, tiles;  // cols: 16-byte pieces and single elements of a row
+};
+long long mne_expert_workspace_ints(long long m, int experts);
+int mne_launch_expert_sort(ExpertSortArgs a, void* workspace, hipStream_t st);
+int mne_launch_expert_dispatch(ExpertRowArgs a, int type, hipStream_t st);
+int mne_launch_expert_combine(ExpertRowArgs a, int type, hipStream_t st);
+int mne_launch_expert_combine_backward(ExpertRowArgs a, int type, hipStream_t st);
+
 int mne_launch_sample_z(const ZArgs& a, hipStream_t st);
 int mne_launch_pack(const mne_scene_t& sc, float* pk, hipStream_t st);
 // mode: 0 = forward, every sample decoded (raw complete);  1 = forward with early ray termination (maps only);

@@ -111,3 +111,8 @@ template <> struct MneBytes<8> { uint2 v; };
 template <> struct MneBytes<4> { unsigned v; };
 template <> struct MneBytes<2> { unsigned short v; };
 template <> struct MneBytes<1> { unsigned char v; };
+
+// the unsigned integer of B bytes
+template <int B> struct MneWord;
+template <> struct MneWord<4> { typedef unsigned type; };
+template <> struct MneWord<2> { typedef unsigned short type; };

@@ -196,3 +196,115 @@ def check_adamw8(device, ptype, gtype, wd=0.01, eps=1e-8, betas=(0.9, 0.99), ste
                 got_m, got_v = optim.adamw_moments(*st)
                 m1, r1 = values8(want_mc, want_rc, want_sc)
                 assert np.array_equal(_np(got_m), m1.astype(np.float64)) and np.array_equal(_np(got_v), (r1 * r1).astype(np.float64))
+
+
+# -------------------------------------------------------------------------------------------------------------- routing
+def plan64(ids, experts):
+    """order, position, offsets of int64 ids [N, K] (numpy)."""
+    flat = ids.reshape(-1)
+    live = (flat >= 0) & (flat < experts)
+    slots = np.nonzero(live)[0]
+    slots = slots[np.argsort(flat[slots], kind="stable")]
+    order = np.full(flat.size, -1, np.int64)
+    order[:slots.size] = slots
+    position = np.full(flat.size, -1, np.int64)
+    position[slots] = np.arange(slots.size)
+    offsets = np.concatenate([[0], np.cumsum(np.bincount(flat[slots], minlength=experts))])
+    return order, position.reshape(ids.shape), offsets
+
+
+def make_ids(kind, n, k, experts, gen):
+    """Batches that routing goes wrong on: one hot expert, the same expert twice for a token, none at all, ids out of range."""
+    if kind == "hot":
+        ids = torch.full((n, k), experts // 2, dtype=torch.int64)
+    elif kind == "none":
+        ids = torch.full((n, k), -1, dtype=torch.int64)
+    elif kind == "last":
+        ids = torch.full((n, k), experts - 1, dtype=torch.int64)
+    else:
+        ids = torch.randint(0, experts, (n, k), generator=gen)
+        if kind == "masked":
+            ids[torch.rand(n, k, generator=gen) < 0.4] = -1
+            ids[n // 3:n // 2] = -1                       # whole tokens without an expert
+        if kind == "outside" and n:
+            ids[::3] = experts
+            ids[1::5, 0] = -(1 << 40)
+            ids[2::7, -1] = (1 << 33) + 1                 # 32 bits of it would be a valid id
+    return ids
+
+
+def check_expert_sort(device, n, k, experts, kind, wide):
+    from mneslam_amd.routing import expert_sort
+    gen = torch.Generator().manual_seed(n + 7 * k + experts)
+    ids = make_ids(kind, n, k, experts, gen)
+    if not wide:
+        ids = ids.clamp(-(1 << 31), (1 << 31) - 1).to(torch.int32)
+    plan = expert_sort(ids.to(device), experts)
+    order, position, offsets = plan64(ids.to(torch.int64).numpy(), experts)
+    assert np.array_equal(plan.offsets.cpu().numpy(), offsets)
+    assert np.array_equal(plan.order.cpu().numpy(), order)
+    assert np.array_equal(plan.position.cpu().numpy(), position)
+    assert plan.sizes() == np.diff(offsets).tolist() and int(plan.live) == offsets[-1]
+
+
+def _rows_of(shape, dtype, gen, device, odd):
+    """Rows with a stride and an odd start, or dense ones."""
+    n, d = shape
+    t = torch.randn(n, d + (3 if odd else 0), generator=gen).to(dtype).to(device)
+    return t[:, 1:1 + d] if odd else t
+
+
+def check_expert_rows(device, dtype, n, k, experts, width, out_width, kind, odd, wtype="f32", need=("x", "y", "w")):
+    """dispatch, combine and their gradients against float64; masked slots carry NaN weights and dead rows NaN."""
+    from mneslam_amd.routing import expert_combine, expert_dispatch, expert_sort
+    dt, wt = NAMES[dtype], NAMES[wtype]
+    gen = torch.Generator().manual_seed(n + 31 * k + width)
+    ids = make_ids(kind, n, k, experts, gen)
+    order, position, offsets = plan64(ids.numpy(), experts)
+    live = int(offsets[-1])
+    plan = expert_sort(ids.to(device), experts)
+    x, y = _rows_of((n, width), dt, gen, device, odd), _rows_of((n * k, out_width), dt, gen, device, odd)
+    w = torch.randn(n, k, generator=gen).to(wt)
+    w[torch.from_numpy(position) < 0] = float("nan")
+    w = w.to(device)
+    with torch.no_grad():
+        y[live:] = float("nan")
+    x, y, w = (t.requires_grad_(name in need) for name, t in (("x", x), ("y", y), ("w", w)))
+    xs, out = expert_dispatch(x, plan), expert_combine(y, plan, w)
+    gxs, gout = _rows_of((n * k, width), dt, gen, device, odd), _rows_of((n, out_width), dt, gen, device, odd)
+    gxs[live:] = float("nan")
+    outs = [t for t in (xs, out) if t.requires_grad]
+    ins = [t for t in (x, y, w) if t.requires_grad]
+    got = dict(zip(need, torch.autograd.grad(outs, ins, [g for t, g in ((xs, gxs), (out, gout)) if t.requires_grad]))) if ins else {}
+
+    f = lambda t: t.detach().cpu().double().numpy()                                   # noqa: E731
+    half = lambda t, want: (torch.finfo(t).eps / 2 * np.abs(want) + torch.finfo(t).smallest_normal * torch.finfo(t).eps / 2) * (t != torch.float32)  # noqa: E731
+    slot = order[:live]
+    tok, w64 = slot // k, f(w).reshape(-1)
+    X, Y, GX, GO = f(x), f(y)[:live], f(gxs)[:live], f(gout)
+
+    def near(t, want, scale, terms, what):
+        # `terms` roundings of fp32 on sums of magnitudes up to `scale`, and the rounding to the result's type
+        tol = terms * EPS32 * scale * 1.01 + half(t.dtype, want) * 1.01 + 1e-44
+        assert t.shape == want.shape and (np.abs(f(t) - want) <= tol).all(), what
+
+    def summed(rows, width):
+        total = np.zeros((n, width))
+        np.add.at(total, tok, rows)
+        return total
+
+    def full(rows):
+        return np.concatenate([rows, np.zeros((n * k - live, rows.shape[1]))])
+
+    assert xs.dtype == dt and np.array_equal(f(xs), full(X[tok]))
+    near(out, summed(w64[slot][:, None] * Y, out_width), summed(np.abs(w64[slot][:, None] * Y), out_width), k, "out")
+    if "x" in need:
+        near(got["x"], summed(GX, width), summed(np.abs(GX), width), k, "dx")
+    if "y" in need:
+        want = full(w64[slot][:, None] * GO[tok])
+        near(got["y"], want, np.abs(want), 1, "dy")
+    if "w" in need:
+        want, scale = np.zeros(n * k), np.zeros(n * k)
+        want[slot], scale[slot] = (GO[tok] * Y).sum(1), np.abs(GO[tok] * Y).sum(1)
+        near(got["w"], want.reshape(n, k), scale.reshape(n, k), out_width, "dw")
+        assert got["w"].dtype == wt

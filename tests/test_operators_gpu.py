@@ -34,3 +34,36 @@ def test_adamw_32(ptype, gtype):
 @pytest.mark.parametrize("ptype,gtype", TYPES)
 def test_adamw_8(ptype, gtype):
     oc.check_adamw8(DEV, ptype, gtype)
+
+
+SORTS = [(1, 1, 1), (1, 2, 8), (3, 2, 1), (0, 2, 5), (64, 1, 64), (65, 3, 7), (1000, 2, 129), (4097, 4, 33), (777, 8, 2000), (300, 2, 2001),
+         (5000, 4, 4096)]
+
+
+@pytest.mark.parametrize("kind", ["even", "hot", "none", "last", "masked", "outside"])
+@pytest.mark.parametrize("n,k,experts", SORTS)
+def test_expert_sort(n, k, experts, kind):
+    oc.check_expert_sort(DEV, n, k, experts, kind, wide=(n + experts) % 2 == 0 or kind == "outside")
+
+
+# widths of one element, below and beyond a piece, odd, one wave's columns and more
+ROWS = [(1, 2, 8, 1024, 1024), (5, 1, 3, 1, 1), (33, 3, 4, 3, 4), (70, 2, 9, 8, 7), (129, 2, 6, 65, 65), (17, 8, 40, 130, 129),
+        (9, 5, 4, 520, 257), (6, 4, 3, 2051, 1030), (40, 6, 5, 16, 16), (0, 2, 3, 8, 8), (4, 2, 3, 0, 0)]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("kind", ["even", "masked"])
+@pytest.mark.parametrize("n,k,experts,width,out_width", ROWS)
+def test_expert_rows(dtype, kind, n, k, experts, width, out_width):
+    oc.check_expert_rows(DEV, dtype, n, k, experts, width, out_width, kind, odd=(n + width) % 2 == 1 and n > 1)
+
+
+@pytest.mark.parametrize("dtype,wtype", [("f32", "bf16"), ("bf16", "bf16"), ("f16", "f32")])
+@pytest.mark.parametrize("need", [("x",), ("y",), ("w",), ("x", "w"), ("y", "w"), ()])
+def test_expert_rows_needed_gradients(dtype, wtype, need):
+    oc.check_expert_rows(DEV, dtype, 50, 3, 5, 24, 33, "masked", odd=True, wtype=wtype, need=need)
+
+
+@pytest.mark.parametrize("kind", ["hot", "none", "outside"])
+def test_expert_rows_batches(kind):
+    oc.check_expert_rows(DEV, "bf16", 130, 2, 7, 40, 24, kind, odd=False)
