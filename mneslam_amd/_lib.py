@@ -3,7 +3,6 @@
 The library is the only compute backend of this package.  If it is missing the import of any hot
 path raises -- there is deliberately no CPU/PyTorch fallback.
 """
-import contextlib
 import ctypes as C
 import importlib.util
 import os
@@ -246,8 +245,6 @@ def load(path=None):
                        (lib.mne_sizeof_tile_overlap, TileOverlap), (lib.mne_sizeof_pose_state, PoseState)):
             if fn() != C.sizeof(st):
                 raise RuntimeError(f"struct layout mismatch for {st.__name__}: C {fn()} vs ctypes {C.sizeof(st)}")
-        lib.on_host = bool(lib.mne_runs_on_host())
-        lib.adamw_step_address = C.cast(lib.mne_adamw_step, C.c_void_p).value      # (called from host_tensors.cpp)
         _lib = lib
         return lib
 
@@ -279,45 +276,30 @@ def stream_for(t):
     return None
 
 
-T_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}       # MNE_T_*
 
 
-def one_device(tensors, what):
-    """The device that all of ``tensors`` are on; raises if there are several, or if the library cannot reach it (a kernel that
-    is given an address of host memory would fault)."""
-    dev = tensors[0].device
-    for t in tensors:
-        if t.device != dev:
-            raise ValueError(f"{what}: tensors on {dev} and on {t.device}")
-    if dev.type != ("cpu" if load().on_host else "cuda"):
-        raise ValueError(f"{what}: tensors on {dev}: the HIP kernels need them on the GPU")
-    return dev
-
-
-def device_guard(dev):
-    """Makes ``dev`` the current device for a launch (the streams of another device are not the current one's)."""
-    return torch.cuda.device(dev) if dev.type == "cuda" and dev.index != torch.cuda.current_device() else contextlib.nullcontext()
-
-
-def raw_stream(dev):
-    """Handle of the current stream of ``dev`` as a number."""
-    return torch.cuda.current_stream(dev).cuda_stream if dev.type == "cuda" else 0
-
-
-_host = None
+_host, _host_library = None, None
+_HOST_ENTRIES = ("mne_last_error", "mne_adamw_step", "mne_adamw_moments", "mne_expert_sort_workspace_bytes", "mne_expert_sort",
+                 "mne_expert_dispatch", "mne_expert_combine", "mne_expert_combine_backward")       # the order of struct Library there
 
 
 def host_tensors():
-    """The in-tree extension module of csrc/host_tensors.cpp."""
-    global _host
-    if _host is None:
-        path = os.path.join(_HERE, "_host_tensors.so")
-        if not os.path.exists(path):
-            raise RuntimeError(f"{path} not found. Build it with `python -m mneslam_amd.build`.")
-        spec = importlib.util.spec_from_file_location("mneslam_amd._host_tensors", path)
-        mod = importlib.util.module_from_spec(spec)
-        spec.loader.exec_module(mod)
-        if mod.ABI_VERSION != ABI_VERSION:
-            raise RuntimeError("_host_tensors ABI version mismatch")
-        _host = mod
+    """The in-tree extension module of csrc/host_tensors.cpp, calling the library that is loaded."""
+    global _host, _host_library
+    lib = _lib if _lib is not None else load()
+    if _host_library is lib:
+        return _host
+    with _lock:
+        if _host is None:
+            path = os.path.join(_HERE, "_host_tensors.so")
+            if not os.path.exists(path):
+                raise RuntimeError(f"{path} not found. Build it with `python -m mneslam_amd.build`.")
+            spec = importlib.util.spec_from_file_location("mneslam_amd._host_tensors", path)
+            mod = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(mod)
+            if mod.ABI_VERSION != ABI_VERSION:
+                raise RuntimeError("_host_tensors ABI version mismatch")
+            _host = mod
+        _host.bind([C.cast(getattr(lib, name), C.c_void_p).value for name in _HOST_ENTRIES], bool(lib.mne_runs_on_host()))
+        _host_library = lib
     return _host

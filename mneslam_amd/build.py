@@ -136,10 +136,11 @@ def build_host(force=False, verbose=False):
     import torch
     from torch.utils import cpp_extension
     lib_dir = os.path.join(os.path.dirname(torch.__file__), "lib")
-    inc = [INCLUDE, *cpp_extension.include_paths(), sysconfig.get_paths()["include"]]
+    rocm = os.path.dirname(os.path.dirname(os.path.realpath(_hipcc())))
+    inc = [INCLUDE, os.path.join(rocm, "include"), *cpp_extension.include_paths(), sysconfig.get_paths()["include"]]
     cmd = [shutil.which("g++") or "c++", "-std=c++17", "-O2", "-shared", "-fPIC", "-fvisibility=hidden",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[f"-I{i}" for i in inc], src, "-o", HOST_LIB,
-           f"-L{lib_dir}", "-ltorch_python", "-ltorch_cpu", "-lc10"]
+           "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[f"-I{i}" for i in inc], src, "-o", HOST_LIB,
+           f"-L{lib_dir}", "-ltorch_python", "-ltorch_cpu", "-lc10_hip", "-lc10"]
     if verbose:
         print(" ".join(cmd), flush=True)
     subprocess.check_call(cmd)

@@ -1,8 +1,12 @@
-// host_tensors.cpp -- the host side of optim.adamw_step: lists of torch tensors checked and written into the table of
-// mne_adamw_step.  A list of several hundred small tensors is bound by this loop and not by the GPU: in python it costs 2.5 us a
-// tensor (about thirty attribute reads), here 0.1 us.
+// host_tensors.cpp -- the host side of optim.adamw_step and of routing: torch tensors checked and handed to the C ABI, and the autograd
+// nodes of the row movements.  Calls that take a few microseconds on the GPU are bound by what runs before and between them: a list of
+// several hundred tensors costs 2.5 us a tensor in python (about thirty attribute reads) and 0.1 us here, and a backward pass through two
+// python nodes 140 us and 30 us.
 #include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <algorithm>
@@ -14,7 +18,47 @@
 namespace {
 
 typedef std::vector<at::Tensor> Tensors;
-typedef int (*adamw_step_fn)(const int64_t*, int64_t, const mne_adamw_cfg_t*, const mne_clock_t*, void*);
+using torch::autograd::AutogradContext;
+using torch::autograd::Variable;
+using torch::autograd::variable_list;
+
+// The entry points of the library that the package has loaded (a table by value: a node of a graph keeps the one it was made with).
+struct Library {
+    decltype(&mne_last_error) last_error;
+    decltype(&mne_adamw_step) adamw_step;
+    decltype(&mne_adamw_moments) adamw_moments;
+    decltype(&mne_expert_sort_workspace_bytes) sort_bytes;
+    decltype(&mne_expert_sort) sort;
+    decltype(&mne_expert_dispatch) dispatch;
+    decltype(&mne_expert_combine) combine;
+    decltype(&mne_expert_combine_backward) combine_backward;
+    int64_t on_host;
+};
+Library g_lib;
+
+void bind(const std::vector<uintptr_t>& addresses, bool on_host) {
+    if (addresses.size() * sizeof(uintptr_t) + sizeof(int64_t) != sizeof(Library)) throw py::value_error("bind: wrong number of entry points");
+    memcpy((void*)&g_lib, addresses.data(), addresses.size() * sizeof(uintptr_t));
+    g_lib.on_host = on_host;
+}
+
+void check(int rc, const char* what) {
+    if (rc) throw std::runtime_error(std::string("libmneslam_hip ") + what + " failed (" + std::to_string(rc) + "): " + g_lib.last_error());
+}
+
+// All on one device that the library reaches (a kernel that is given an address of host memory would fault).
+void one_device(const char* what, std::initializer_list<const at::Tensor*> tensors) {
+    const at::Device dev = (*tensors.begin())->device();
+    for (const at::Tensor* t : tensors) {
+        if (!t->defined()) continue;
+        if (t->layout() != at::kStrided) throw py::value_error(std::string(what) + ": sparse tensors are not supported");
+        if (t->device() != dev) throw py::value_error(std::string(what) + ": tensors on " + dev.str() + " and on " + t->device().str());
+    }
+    if (dev.type() != (g_lib.on_host ? at::kCPU : at::kCUDA))
+        throw py::value_error(std::string(what) + ": tensors on " + dev.str() + ": the HIP kernels need them on the GPU");
+}
+
+void* stream_of(const at::Device& dev) { return dev.is_cuda() ? (void*)c10::hip::getCurrentHIPStream(dev.index()).stream() : nullptr; }
 
 int type_code(at::ScalarType t) {
     return t == at::kFloat ? MNE_T_F32 : t == at::kBFloat16 ? MNE_T_BF16 : t == at::kHalf ? MNE_T_F16 : -1;
@@ -27,19 +71,19 @@ bool laid_out_alike(const at::Tensor& a, const at::Tensor& b) {
     return true;
 }
 
-int adamw_step(uintptr_t fn, const Tensors& params, const Tensors& grads, const Tensors& exp_avgs, const Tensors& exp_avg_sqs,
+void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& exp_avgs, const Tensors& exp_avg_sqs,
                const c10::optional<Tensors>& scales, const c10::optional<std::vector<int64_t>>& ordinals, double lr, double beta1,
-               double beta2, double eps, double weight_decay, int64_t step, int64_t seed, bool zero_grad, uintptr_t clock,
-               uintptr_t stream, bool on_host) {
+               double beta2, double eps, double weight_decay, int64_t step, int64_t seed, bool zero_grad, uintptr_t clock) {
     const size_t n = params.size();
     const bool small = scales.has_value();
     if (grads.size() != n || exp_avgs.size() != n || exp_avg_sqs.size() != n || (small && scales->size() != n) ||
         (ordinals && ordinals->size() != n))
         throw py::value_error("adamw_step: lists of different lengths");
-    if (!n) return 0;
+    if (!n) return;
+    if (!params[0].defined()) throw py::value_error("adamw_step: undefined tensors");
+    one_device("adamw_step", {&params[0]});
     const at::Device dev = params[0].device();
-    if (dev.type() != (on_host ? at::kCPU : at::kCUDA))
-        throw py::value_error("adamw_step: tensors on " + dev.str() + ": the HIP kernels need them on the GPU");
+    const c10::DeviceGuard guard(dev);
     std::map<std::pair<int, int>, std::vector<int64_t>> tables;          // by the types of parameter and gradient
     std::vector<std::pair<int64_t, int64_t>> ranges;
     Tensors keep;
@@ -89,17 +133,161 @@ int adamw_step(uintptr_t fn, const Tensors& params, const Tensors& grads, const 
         cfg.lr = lr; cfg.beta1 = beta1; cfg.beta2 = beta2; cfg.eps = eps; cfg.weight_decay = weight_decay;
         cfg.step = (int32_t)step; cfg.state_bits = small ? 8 : 32; cfg.p_type = t.first.first; cfg.g_type = t.first.second;
         cfg.zero_grad = zero_grad; cfg.seed = (uint32_t)seed;
-        const int rc = ((adamw_step_fn)fn)(t.second.data(), (int64_t)t.second.size() / 7, &cfg, (const mne_clock_t*)clock, (void*)stream);
-        if (rc) return rc;
+        check(g_lib.adamw_step(t.second.data(), (int64_t)t.second.size() / 7, &cfg, (const mne_clock_t*)clock, stream_of(dev)), "mne_adamw_step");
     }
     for (const at::Tensor& p : params)              // what autograd has saved of a parameter is out of date, as after p.add_()
         if (!p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
-    return 0;
+}
+
+std::vector<at::Tensor> adamw_moments(const at::Tensor& m, const at::Tensor& v, const at::Tensor& scales) {
+    one_device("adamw_moments", {&m, &v, &scales});
+    if (m.scalar_type() != at::kChar || v.scalar_type() != at::kByte) throw py::type_error("adamw_moments: the codes are int8 and uint8");
+    if (m.sizes() != v.sizes() || !m.is_non_overlapping_and_dense() || !laid_out_alike(m, v))
+        throw py::value_error("adamw_moments: the codes must be dense and laid out alike");
+    const int64_t n = m.numel();
+    if (scales.scalar_type() != at::kFloat || scales.dim() != 2 || scales.size(0) != (n + 255) / 256 || scales.size(1) != 2 || !scales.is_contiguous())
+        throw py::value_error("adamw_moments: scales must be contiguous float32 [ceil(n / 256), 2]");
+    const c10::DeviceGuard guard(m.device());
+    c10::NoGradGuard no_grad;
+    at::Tensor a = at::empty_like(m, m.options().dtype(at::kFloat)), b = at::empty_like(a);
+    check(g_lib.adamw_moments((const int8_t*)m.data_ptr(), (const uint8_t*)v.data_ptr(), (const float*)scales.data_ptr(), n,
+                              (float*)a.data_ptr(), (float*)b.data_ptr(), stream_of(m.device())), "mne_adamw_moments");
+    return {a, b};
+}
+
+// ---- routing ---------------------------------------------------------------------------------------------------------
+// order [m], position [n, k], offsets [experts + 1]
+std::vector<at::Tensor> expert_sort(const at::Tensor& given, int64_t experts) {
+    one_device("expert_sort", {&given});
+    if ((given.scalar_type() != at::kInt && given.scalar_type() != at::kLong) || (given.dim() != 1 && given.dim() != 2))
+        throw py::type_error("expert_sort: ids must be int32 or int64 [N, K] or [N]");
+    if (experts < 1 || experts > 4096) throw py::value_error("expert_sort: 1 to 4096 experts, got " + std::to_string(experts));
+    const int64_t n = given.size(0), k = given.dim() == 2 ? given.size(1) : 1, m = n * k;
+    if (k < 1) throw py::value_error("expert_sort: ids without a choice");
+    if (m >= (1ll << 31) - 65536) throw py::value_error("expert_sort: too many choices for 32-bit rows");
+    const c10::DeviceGuard guard(given.device());
+    c10::NoGradGuard no_grad;
+    const at::Tensor ids = given.contiguous();
+    const size_t bytes = g_lib.sort_bytes(m, (int)experts);
+    // one allocation: order, position, offsets, workspace
+    const at::Tensor all = at::empty({2 * m + experts + 1 + (int64_t)bytes / 4}, ids.options().dtype(at::kInt));
+    int32_t* base = (int32_t*)all.data_ptr();
+    check(g_lib.sort(ids.data_ptr(), ids.scalar_type() == at::kLong, m, (int)experts, base, base + m, base + 2 * m, base + 2 * m + experts + 1,
+                     bytes, stream_of(ids.device())), "mne_expert_sort");
+    return {all.narrow(0, 0, m), all.narrow(0, m, m).view({n, k}), all.narrow(0, 2 * m, experts + 1)};
+}
+
+// a row's elements next to each other (a copy where they are not)
+at::Tensor rows(const at::Tensor& t, const char* what) {
+    if (t.dim() != 2) throw py::value_error(std::string(what) + ": rows must be [rows, width]");
+    if (type_code(t.scalar_type()) < 0)
+        throw py::type_error(std::string(what) + ": " + c10::toString(t.scalar_type()) + " is not supported (float32, bfloat16, float16)");
+    return t.stride(1) == 1 || t.size(1) <= 1 ? t : t.contiguous();
+}
+const int32_t* ints(const at::Tensor& t) { return (const int32_t*)t.data_ptr(); }
+const int32_t* live_rows(const at::Tensor& offsets) { return ints(offsets) + offsets.size(0) - 1; }
+const float* floats(const at::Tensor& t) { return t.defined() ? (const float*)t.data_ptr() : nullptr; }
+
+at::Tensor dispatch(const Library& lib, const at::Tensor& given, const at::Tensor& position, const at::Tensor& offsets) {
+    const at::Tensor x = rows(given, "expert_dispatch");
+    const c10::DeviceGuard guard(x.device());
+    const int64_t n = position.size(0), k = position.size(1), width = x.size(1);
+    at::Tensor out = at::empty({n * k, width}, x.options());
+    check(lib.dispatch(x.data_ptr(), x.stride(0), type_code(x.scalar_type()), n, (int)k, width, ints(position), live_rows(offsets), out.data_ptr(),
+                       stream_of(x.device())), "mne_expert_dispatch");
+    return out;
+}
+
+at::Tensor combine(const Library& lib, const at::Tensor& given, const at::Tensor& position, const at::Tensor& weights) {
+    const at::Tensor y = rows(given, "expert_combine"), w = weights.defined() ? weights.to(at::kFloat).contiguous() : weights;
+    const c10::DeviceGuard guard(y.device());
+    const int64_t n = position.size(0), k = position.size(1), width = y.size(1);
+    at::Tensor out = at::empty({n, width}, y.options());
+    check(lib.combine(y.data_ptr(), y.stride(0), type_code(y.scalar_type()), n, (int)k, width, ints(position), floats(w), out.data_ptr(),
+                      stream_of(y.device())), "mne_expert_combine");
+    return out;
+}
+
+// A gradient of a gradient would come out as zero, unnoticed: refused.
+void once(const char* what) {
+    if (c10::GradMode::is_enabled()) throw std::runtime_error(std::string(what) + ": differentiable once (create_graph=True is not supported)");
+}
+
+Library library_of(AutogradContext* ctx) {
+    Library lib;
+    const std::string bytes = ctx->saved_data["library"].toStringRef();
+    memcpy((void*)&lib, bytes.data(), sizeof(lib));
+    return lib;
+}
+
+struct DispatchNode : torch::autograd::Function<DispatchNode> {
+    static Variable forward(AutogradContext* ctx, const Variable& x, const Variable& position, const Variable& offsets) {
+        ctx->save_for_backward({position});
+        ctx->saved_data["library"] = std::string((const char*)&g_lib, sizeof(g_lib));
+        return dispatch(g_lib, x, position, offsets);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        once("expert_dispatch");
+        if (!grads[0].defined()) return {Variable(), Variable(), Variable()};
+        return {combine(library_of(ctx), grads[0], ctx->get_saved_variables()[0], at::Tensor()), Variable(), Variable()};
+    }
+};
+
+struct CombineNode : torch::autograd::Function<CombineNode> {
+    static Variable forward(AutogradContext* ctx, const Variable& y, const Variable& position, const Variable& offsets, const Variable& weights) {
+        ctx->save_for_backward({y, position, offsets, weights});
+        ctx->saved_data["library"] = std::string((const char*)&g_lib, sizeof(g_lib));
+        return combine(g_lib, y, position, weights);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        once("expert_combine");
+        if (!grads[0].defined()) return {Variable(), Variable(), Variable(), Variable()};
+        const Library lib = library_of(ctx);
+        const variable_list saved = ctx->get_saved_variables();
+        const at::Tensor y = rows(saved[0], "expert_combine"), &position = saved[1], &offsets = saved[2], &weights = saved[3];
+        const at::Tensor dout = rows(grads[0], "expert_combine"), w = weights.defined() ? weights.to(at::kFloat).contiguous() : weights;
+        const c10::DeviceGuard guard(y.device());
+        const int64_t n = position.size(0), k = position.size(1), width = y.size(1);
+        const bool want_dw = weights.defined() && ctx->needs_input_grad(3), want_dy = ctx->needs_input_grad(0);
+        at::Tensor dy, dw;
+        if (want_dy) dy = at::empty({n * k, width}, y.options());
+        if (want_dw) dw = width ? at::empty({n, k}, w.options()) : at::zeros({n, k}, w.options());
+        check(lib.combine_backward(dout.data_ptr(), dout.stride(0), y.data_ptr(), y.stride(0), type_code(y.scalar_type()), n, (int)k, width,
+                                   ints(position), live_rows(offsets), floats(w), want_dy ? dy.data_ptr() : nullptr,
+                                   want_dw ? (float*)dw.data_ptr() : nullptr, stream_of(y.device())), "mne_expert_combine_backward");
+        return {dy, Variable(), Variable(), want_dw ? dw.to(weights.scalar_type()) : dw};
+    }
+};
+
+at::Tensor expert_dispatch(const at::Tensor& x, const at::Tensor& position, const at::Tensor& offsets) {
+    one_device("expert_dispatch", {&x, &position, &offsets});
+    if (x.dim() != 2 || x.size(0) != position.size(0))
+        throw py::value_error("expert_dispatch: x must be [" + std::to_string(position.size(0)) + " tokens, width]");
+    rows(x, "expert_dispatch");
+    return DispatchNode::apply(x, position, offsets);
+}
+
+at::Tensor expert_combine(const at::Tensor& y, const at::Tensor& position, const at::Tensor& offsets, const c10::optional<at::Tensor>& weights) {
+    const at::Tensor w = weights ? *weights : at::Tensor();
+    one_device("expert_combine", {&y, &position, &offsets, &w});
+    if (y.dim() != 2 || y.size(0) != position.numel())
+        throw py::value_error("expert_combine: y must be [" + std::to_string(position.numel()) + " rows, width]");
+    if (w.defined()) {
+        if (w.sizes() != position.sizes()) throw py::value_error("expert_combine: weights must be [tokens, choices]");
+        if (type_code(w.scalar_type()) < 0) throw py::type_error("expert_combine: weights must be float32, bfloat16 or float16");
+    }
+    rows(y, "expert_combine");
+    return CombineNode::apply(y, position, offsets, w);
 }
 
 }  // namespace
 
 PYBIND11_MODULE(_host_tensors, m) {
+    m.def("bind", &bind);
     m.def("adamw_step", &adamw_step);
+    m.def("adamw_moments", &adamw_moments);
+    m.def("expert_sort", &expert_sort);
+    m.def("expert_dispatch", &expert_dispatch);
+    m.def("expert_combine", &expert_combine);
     m.attr("ABI_VERSION") = MNE_ABI_VERSION;
 }

@@ -13,9 +13,10 @@
 
 #define EX_THREADS 256
 #define EX_WAVES (EX_THREADS / 64)
-#define EX_CHUNK 4096                               // slots of a workgroup of the long form
+#define EX_CHUNKS 512                               // workgroups of the long form at most
 #define EX_SHORT 16384                              // slots up to which one workgroup of 1024 does it all
 #define EX_SHORT_EXPERTS 2000                       // its counters of 16 waves fit the LDS
+#define EX_AHEAD 8                                  // ids that a lane loads before it looks at the first
 
 // ---- sort ------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ int ex_id(const ExpertSortArgs& a, int slot) {        // what names no expert sorts behind all of them
@@ -23,42 +24,62 @@ __device__ __forceinline__ int ex_id(const ExpertSortArgs& a, int slot) {       
     return e >= 0 && e < a.experts ? (int)e : a.experts;
 }
 
+// the slots first + 64 j + lane of a wave, j = 0 .. EX_AHEAD - 1, at most `last`: loaded together, looked at one after the other
+__device__ __forceinline__ void ex_ids(const ExpertSortArgs& a, long long first, long long last, int* e) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int j = 0; j < EX_AHEAD; ++j) {
+        const long long slot = first + 64 * j + lane;
+        e[j] = slot < last ? ex_id(a, (int)slot) : -1;
+    }
+}
+
+__device__ __forceinline__ void ex_count(const ExpertSortArgs& a, long long first, long long last, int* cnt) {
+    for (long long j0 = first; j0 < last; j0 += 64 * EX_AHEAD) {
+        int e[EX_AHEAD];
+        ex_ids(a, j0, last, e);
+#pragma unroll
+        for (int j = 0; j < EX_AHEAD; ++j)
+            if (e[j] >= 0) atomicAdd(&cnt[e[j]], 1);
+    }
+}
+
 __global__ __launch_bounds__(EX_THREADS) void expert_count_kernel(ExpertSortArgs a) {
     MNE_DYN_LDS(lds);
     int* cnt = (int*)lds;
     for (int e = threadIdx.x; e <= a.experts; e += EX_THREADS) cnt[e] = 0;
     __syncthreads();
-    const int first = (int)blockIdx.x * EX_CHUNK;
-    for (int j = threadIdx.x; j < EX_CHUNK && first + j < a.m; j += EX_THREADS) atomicAdd(&cnt[ex_id(a, first + j)], 1);
+    const long long first = ((long long)blockIdx.x * EX_WAVES + (threadIdx.x >> 6)) * a.per_wave;
+    ex_count(a, first, first + a.per_wave < a.m ? first + a.per_wave : a.m, cnt);
     __syncthreads();
     for (int e = threadIdx.x; e <= a.experts; e += EX_THREADS) a.count[(long long)blockIdx.x * (a.experts + 1) + e] = cnt[e];
 }
 
 // count[chunk][e] becomes the number of e's slots in the chunks before, total[e] the number in all: 64 experts a workgroup, a
-// quarter of the chunks a wave
-__global__ __launch_bounds__(EX_THREADS) void expert_scan_kernel(ExpertSortArgs a) {
-    __shared__ int part[EX_WAVES][64];
+// sixteenth of the chunks (32 at most) a wave, in registers between the two passes
+__global__ __launch_bounds__(1024) void expert_scan_kernel(ExpertSortArgs a) {
+    __shared__ int part[16][64];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, e = (int)blockIdx.x * 64 + lane, stride = a.experts + 1;
-    const int each = (a.chunks + EX_WAVES - 1) / EX_WAVES, lo = w * each, hi = lo + each < a.chunks ? lo + each : a.chunks;
-    int sum = 0;
-    if (e <= a.experts)
-        for (int c = lo; c < hi; ++c) sum += a.count[(long long)c * stride + e];
+    const int each = (a.chunks + 15) / 16, lo = w * each, hi = lo + each < a.chunks ? lo + each : a.chunks;
+    int c[EX_CHUNKS / 16], sum = 0;
+#pragma unroll
+    for (int i = 0; i < EX_CHUNKS / 16; ++i) c[i] = e <= a.experts && lo + i < hi ? a.count[(long long)(lo + i) * stride + e] : 0;
+#pragma unroll
+    for (int i = 0; i < EX_CHUNKS / 16; ++i) sum += c[i];
     part[w][lane] = sum;
     __syncthreads();
     int run = 0, all = 0;
-    for (int i = 0; i < EX_WAVES; ++i) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
         if (i < w) run += part[i][lane];
         all += part[i][lane];
     }
-    if (e <= a.experts) {
-        for (int c = lo; c < hi; ++c) {
-            int* q = &a.count[(long long)c * stride + e];
-            const int x = *q;
-            *q = run;
-            run += x;
-        }
-        if (w == 0) a.total[e] = all;
+#pragma unroll
+    for (int i = 0; i < EX_CHUNKS / 16; ++i) {
+        if (e <= a.experts && lo + i < hi) a.count[(long long)(lo + i) * stride + e] = run;
+        run += c[i];
     }
+    if (e <= a.experts && w == 0) a.total[e] = all;
 }
 
 // Rows of a workgroup's slots: WAVES waves of a.per_wave consecutive slots.  ALONE: one workgroup has all slots.
@@ -72,8 +93,8 @@ __global__ __launch_bounds__(WAVES * 64) void expert_place_kernel(ExpertSortArgs
     for (int e = threadIdx.x; e < WAVES * bins; e += WAVES * 64) cnt[e] = 0;
     __syncthreads();
     const long long first = ((long long)blockIdx.x * WAVES + w) * a.per_wave;
-    const int n = first < a.m ? (int)(a.m - first < a.per_wave ? a.m - first : a.per_wave) : 0;
-    for (int j = lane; j < n; j += 64) atomicAdd(&mine[ex_id(a, (int)first + j)], 1);
+    const long long last = first + a.per_wave < a.m ? first + a.per_wave : a.m;
+    ex_count(a, first, last, mine);
     __syncthreads();
     // first row of every expert: a thread has a run of them, the threads' sums are scanned
     const int each = (bins + WAVES * 64 - 1) / (WAVES * 64), lo = threadIdx.x * each, hi = lo + each < bins ? lo + each : bins;
@@ -107,32 +128,49 @@ __global__ __launch_bounds__(WAVES * 64) void expert_place_kernel(ExpertSortArgs
     __syncthreads();
     int bits = 0;
     while ((1 << bits) < bins) ++bits;
-    for (int j0 = 0; j0 < n; j0 += 64) {            // 64 slots at a time, in order
-        const int slot = (int)first + j0 + lane, live = j0 + lane < n, e = live ? ex_id(a, slot) : a.experts;
-        unsigned long long peers = __ballot(live);  // the lanes with the same expert
-        for (int b = 0; b < bits; ++b) {
-            const unsigned long long set = __ballot((e >> b) & 1);
-            peers &= (e >> b) & 1 ? set : ~set;
+    for (long long j0 = first; j0 < last; j0 += 64 * EX_AHEAD) {
+        int ids[EX_AHEAD];
+        ex_ids(a, j0, last, ids);
+        for (int j = 0; j < EX_AHEAD && j0 + 64 * j < last; ++j) {        // 64 slots at a time, in order
+            int e = -1;
+#pragma unroll
+            for (int i = 0; i < EX_AHEAD; ++i) e = i == j ? ids[i] : e;
+            const bool live = e >= 0;
+            const int key = live ? e : a.experts;
+            unsigned long long peers = __ballot(live);                    // the lanes with the same expert
+            for (int b = 0; b < bits; ++b) {
+                const unsigned long long set = __ballot((key >> b) & 1);
+                peers &= (key >> b) & 1 ? set : ~set;
+            }
+            const int before = __popcll(peers & ((1ull << lane) - 1ull)), all = __popcll(peers);
+            const int start = mine[key];
+            MNE_WAVE_SYNC();
+            if (live) {
+                const int slot = (int)(j0 + 64 * j) + lane, r = start + before;
+                const bool named = e < a.experts;
+                if (before == all - 1) mine[e] = r + 1;
+                a.position[slot] = named ? r : -1;
+                a.order[r] = named ? slot : -1;
+            }
+            MNE_WAVE_SYNC();
         }
-        const int before = __popcll(peers & ((1ull << lane) - 1ull)), all = __popcll(peers);
-        const int start = mine[e];
-        MNE_WAVE_SYNC();
-        if (live) {
-            const int r = start + before;
-            if (before == all - 1) mine[e] = r + 1;
-            const bool named = e < a.experts;
-            a.position[slot] = named ? r : -1;
-            a.order[r] = named ? slot : -1;
-        }
-        MNE_WAVE_SYNC();
     }
 }
 
-static int ex_chunks(long long m) { return (int)((m + EX_CHUNK - 1) / EX_CHUNK); }
+// Slots of a wave of the long form, in 64s: as few as make 512 workgroups, and so many that a workgroup's counters are not more than
+// twice its slots.
+static int ex_per_wave(long long m, int experts) {
+    const long long by_size = (m + EX_CHUNKS * EX_THREADS - 1) / (EX_CHUNKS * EX_THREADS), by_experts = (experts + 2 * EX_THREADS) / (2 * EX_THREADS);
+    return (int)(64 * (by_size > by_experts ? by_size : by_experts));
+}
+static int ex_chunks(long long m, int experts) {
+    const long long chunk = (long long)EX_WAVES * ex_per_wave(m, experts);
+    return (int)((m + chunk - 1) / chunk);
+}
 static bool ex_short(long long m, int experts) { return m <= EX_SHORT && experts <= EX_SHORT_EXPERTS; }
 
 long long mne_expert_workspace_ints(long long m, int experts) {
-    return ex_short(m, experts) ? 0 : ((long long)ex_chunks(m) + 1) * (experts + 1);
+    return ex_short(m, experts) ? 0 : ((long long)ex_chunks(m, experts) + 1) * (experts + 1);
 }
 
 int mne_launch_expert_sort(ExpertSortArgs a, void* workspace, hipStream_t st) {
@@ -144,12 +182,12 @@ int mne_launch_expert_sort(ExpertSortArgs a, void* workspace, hipStream_t st) {
         MNE_LAUNCH((expert_place_kernel<16, true>), 1, 1024, lds, st, a);
         return 0;
     }
-    a.chunks = ex_chunks(a.m);
-    a.per_wave = EX_CHUNK / EX_WAVES;
+    a.chunks = ex_chunks(a.m, a.experts);
+    a.per_wave = ex_per_wave(a.m, a.experts);
     a.count = (int*)workspace;
     a.total = a.count + (long long)a.chunks * bins;
     MNE_LAUNCH(expert_count_kernel, a.chunks, EX_THREADS, bins * sizeof(int), st, a);
-    MNE_LAUNCH(expert_scan_kernel, (bins + 63) / 64, EX_THREADS, 0, st, a);
+    MNE_LAUNCH(expert_scan_kernel, (bins + 63) / 64, 1024, 0, st, a);
     const size_t lds = (size_t)EX_WAVES * bins * sizeof(int);
     MNE_SET_MAX_LDS((expert_place_kernel<EX_WAVES, false>), lds);
     MNE_LAUNCH((expert_place_kernel<EX_WAVES, false>), a.chunks, EX_THREADS, lds, st, a);
@@ -261,8 +299,8 @@ __global__ __launch_bounds__(EX_THREADS) void expert_combine_kernel(ExpertRowArg
         }
 }
 
-// GROUP lanes have a token: its row of dout against its rows of y, K slots at a time.
-template <int T, int K>
+// GROUP lanes have a token: its row of dout against its rows of y, K slots and U columns of a lane at a time.
+template <int T, int K, int U>
 __global__ __launch_bounds__(EX_THREADS) void expert_combine_backward_kernel(ExpertRowArgs a, int group) {
     typedef ExCol<T> Col;
     const long long n = ((long long)blockIdx.x * EX_THREADS + threadIdx.x) / group;
@@ -281,35 +319,51 @@ __global__ __launch_bounds__(EX_THREADS) void expert_combine_backward_kernel(Exp
             dot[i] = 0.0f;
         }
         if (there)
-            for (int c = l; c < a.cols; c += group) {
-                Col d;
-                d.load((const char*)a.a + n * a.a_stride, c, a.width);
-                const int live = c < a.width / Col::N ? Col::N : 1;
+            for (int c0 = l; c0 < a.cols; c0 += group * U) {
+                Col d[U], y[K][U];
 #pragma unroll
-                for (int i = 0; i < K; ++i) {
-                    if (k0 + i >= a.k) continue;
-                    if (row[i] >= 0) {
-                        if (a.dw) {
-                            Col y;
-                            y.load((const char*)a.b + row[i] * a.b_stride, c, a.width);
+                for (int u = 0; u < U; ++u) {
+                    d[u].clear();
+                    if (c0 + u * group < a.cols) d[u].load((const char*)a.a + n * a.a_stride, c0 + u * group, a.width);
+                }
+                if (a.dw) {
+#pragma unroll
+                    for (int i = 0; i < K; ++i)
+#pragma unroll
+                        for (int u = 0; u < U; ++u) {
+                            y[i][u].clear();
+                            if (row[i] >= 0 && c0 + u * group < a.cols) y[i][u].load((const char*)a.b + row[i] * a.b_stride, c0 + u * group, a.width);
+                        }
+#pragma unroll
+                    for (int i = 0; i < K; ++i)
+#pragma unroll
+                        for (int u = 0; u < U; ++u) {
+                            const int live = c0 + u * group < a.width / Col::N ? Col::N : 1;     // (what is not there is zero on both sides)
 #pragma unroll
                             for (int j = 0; j < Col::N; ++j)
-                                if (j < live) dot[i] = fmaf(d.get(j), y.get(j), dot[i]);
+                                if (j < live) dot[i] = fmaf(d[u].get(j), y[i][u].get(j), dot[i]);
                         }
-                        if (a.out) {
-                            Col o;
-                            float x[Col::N];
+                }
+                if (a.out) {
 #pragma unroll
-                            for (int j = 0; j < Col::N; ++j) x[j] = w[i] * d.get(j);
-                            o.put(x);
-                            o.store((char*)a.out + row[i] * size, c, a.width);
+                    for (int i = 0; i < K; ++i)
+#pragma unroll
+                        for (int u = 0; u < U; ++u) {
+                            if (c0 + u * group >= a.cols) continue;
+                            if (row[i] >= 0) {
+                                Col o;
+                                float x[Col::N];
+#pragma unroll
+                                for (int j = 0; j < Col::N; ++j) x[j] = w[i] * d[u].get(j);
+                                o.put(x);
+                                o.store((char*)a.out + row[i] * size, c0 + u * group, a.width);
+                            }
+                            if (k0 + i < a.k && slot + k0 + i >= total) {
+                                Col zero;
+                                zero.clear();
+                                zero.store((char*)a.out + (slot + k0 + i) * size, c0 + u * group, a.width);
+                            }
                         }
-                    }
-                    if (a.out && slot + k0 + i >= total) {
-                        Col zero;
-                        zero.clear();
-                        zero.store((char*)a.out + (slot + k0 + i) * size, c, a.width);
-                    }
                 }
             }
         if (a.dw) {
@@ -322,37 +376,48 @@ __global__ __launch_bounds__(EX_THREADS) void expert_combine_backward_kernel(Exp
     }
 }
 
-// columns of a row, and the lanes that take one: a power of two, at most a wave
-static int ex_columns(ExpertRowArgs& a, int type) {
+// Lanes of a token (a power of two, at most a wave) and columns of a lane, 1 to `most`: of the forms that leave the fewest lanes without
+// a column the one with most columns a lane (more loads in flight).  Where that leaves the machine without waves, one column a lane.
+struct ExForm { int group, u; };
+static ExForm ex_form(ExpertRowArgs& a, int type, int most) {
     const int per = type == MNE_T_F32 ? 4 : 8;
     a.cols = a.width / per + a.width % per;
-    int group = 1;
-    while (group < a.cols && group < 64) group <<= 1;
-    return group;
+    ExForm best = {1, 1};
+    long long least = 1ll << 62;
+    if ((long long)a.n * a.cols < 1 << 17) most = 1;
+    for (int u = 1; u <= most; ++u) {
+        int group = 1;
+        while (group < 64 && group * u < a.cols) group <<= 1;
+        const long long used = ((long long)a.cols + group * u - 1) / (group * u) * (group * u);
+        if (used <= least) { least = used; best = {group, u}; }
+    }
+    a.tiles = (a.cols + best.group * best.u - 1) / (best.group * best.u);
+    return best;
 }
 static unsigned ex_grid(long long units, int group) { return (unsigned)((units * group + EX_THREADS - 1) / EX_THREADS); }
 
 template <int T> static void ex_dispatch(ExpertRowArgs a, hipStream_t st) {
-    const int group = ex_columns(a, T), u = a.cols > 128 ? 4 : a.cols > 64 ? 2 : 1;
-    a.tiles = (a.cols + group * u - 1) / (group * u);
-    const unsigned grid = ex_grid((long long)a.n * a.tiles, group);
-    if (u == 4) MNE_LAUNCH((expert_dispatch_kernel<T, 4>), grid, EX_THREADS, 0, st, a, group);
-    else if (u == 2) MNE_LAUNCH((expert_dispatch_kernel<T, 2>), grid, EX_THREADS, 0, st, a, group);
-    else MNE_LAUNCH((expert_dispatch_kernel<T, 1>), grid, EX_THREADS, 0, st, a, group);
+    const ExForm f = ex_form(a, T, 4);
+    const unsigned grid = ex_grid((long long)a.n * a.tiles, f.group);
+    if (f.u == 4) MNE_LAUNCH((expert_dispatch_kernel<T, 4>), grid, EX_THREADS, 0, st, a, f.group);
+    else if (f.u == 3) MNE_LAUNCH((expert_dispatch_kernel<T, 3>), grid, EX_THREADS, 0, st, a, f.group);
+    else if (f.u == 2) MNE_LAUNCH((expert_dispatch_kernel<T, 2>), grid, EX_THREADS, 0, st, a, f.group);
+    else MNE_LAUNCH((expert_dispatch_kernel<T, 1>), grid, EX_THREADS, 0, st, a, f.group);
 }
 template <int T, bool W> static void ex_combine(ExpertRowArgs a, hipStream_t st) {
-    const int group = ex_columns(a, T), u = a.cols > 64 ? 2 : 1;
-    a.tiles = (a.cols + group * u - 1) / (group * u);
-    const unsigned grid = ex_grid((long long)a.n * a.tiles, group);
-    if (u == 2) MNE_LAUNCH((expert_combine_kernel<T, 2, W>), grid, EX_THREADS, 0, st, a, group);
-    else MNE_LAUNCH((expert_combine_kernel<T, 1, W>), grid, EX_THREADS, 0, st, a, group);
+    const ExForm f = ex_form(a, T, 4);
+    const unsigned grid = ex_grid((long long)a.n * a.tiles, f.group);
+    if (f.u == 4) MNE_LAUNCH((expert_combine_kernel<T, 4, W>), grid, EX_THREADS, 0, st, a, f.group);
+    else if (f.u == 3) MNE_LAUNCH((expert_combine_kernel<T, 3, W>), grid, EX_THREADS, 0, st, a, f.group);
+    else if (f.u == 2) MNE_LAUNCH((expert_combine_kernel<T, 2, W>), grid, EX_THREADS, 0, st, a, f.group);
+    else MNE_LAUNCH((expert_combine_kernel<T, 1, W>), grid, EX_THREADS, 0, st, a, f.group);
 }
 template <int T> static void ex_backward(ExpertRowArgs a, hipStream_t st) {
-    const int group = ex_columns(a, T);
-    const unsigned grid = ex_grid(a.n, group);
-    if (a.k == 1) MNE_LAUNCH((expert_combine_backward_kernel<T, 1>), grid, EX_THREADS, 0, st, a, group);
-    else if (a.k == 2) MNE_LAUNCH((expert_combine_backward_kernel<T, 2>), grid, EX_THREADS, 0, st, a, group);
-    else MNE_LAUNCH((expert_combine_backward_kernel<T, 4>), grid, EX_THREADS, 0, st, a, group);
+    const ExForm f = ex_form(a, T, 4);
+    const unsigned grid = ex_grid(a.n, f.group);
+    if (a.k == 1) MNE_LAUNCH((expert_combine_backward_kernel<T, 1, 4>), grid, EX_THREADS, 0, st, a, f.group);
+    else if (a.k == 2) MNE_LAUNCH((expert_combine_backward_kernel<T, 2, 2>), grid, EX_THREADS, 0, st, a, f.group);
+    else MNE_LAUNCH((expert_combine_backward_kernel<T, 4, 1>), grid, EX_THREADS, 0, st, a, f.group);
 }
 
 int mne_launch_expert_dispatch(ExpertRowArgs a, int type, hipStream_t st) {

@@ -153,34 +153,17 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, scales=None, *, step, lr, b
     params = list(params)
     if not params:
         return
-    lib, dev = _lib.load(), params[0].device
-    if clock is None and dev.type == "cuda" and torch.cuda.is_current_stream_capturing():
+    if clock is None and params[0].is_cuda and torch.cuda.is_current_stream_capturing():
         raise RuntimeError("adamw_step: recording a step needs a clock (the step count would be the same at every replay)")
-    with _lib.device_guard(dev):
-        rc = _lib.host_tensors().adamw_step(
-            lib.adamw_step_address, params, list(grads), list(exp_avgs), list(exp_avg_sqs),
-            None if scales is None else list(scales), None if ordinals is None else list(ordinals), lr, betas[0], betas[1], eps,
-            weight_decay, step, seed, zero_grad, 0 if clock is None else C.addressof(clock), _lib.raw_stream(dev), lib.on_host)
-    _lib.check(rc, "mne_adamw_step")
+    _lib.host_tensors().adamw_step(params, list(grads), list(exp_avgs), list(exp_avg_sqs), None if scales is None else list(scales),
+                                   None if ordinals is None else list(ordinals), lr, betas[0], betas[1], eps, weight_decay, step, seed,
+                                   zero_grad, 0 if clock is None else C.addressof(clock))
 
 
-@torch.no_grad()
 def adamw_moments(exp_avg, exp_avg_sq, scales):
     """The fp32 moments (exp_avg, exp_avg_sq) that 8-bit codes and their ``scales`` stand for (see ``adamw_step``), in the codes'
     shape and layout."""
-    n = exp_avg.numel()
-    if exp_avg.dtype != torch.int8 or exp_avg_sq.dtype != torch.uint8:
-        raise TypeError("adamw_moments: the codes are int8 and uint8")
-    m, v = torch.empty_like(exp_avg, dtype=torch.float32), torch.empty_like(exp_avg_sq, dtype=torch.float32)
-    if exp_avg_sq.shape != exp_avg.shape or not m.stride() == v.stride() == exp_avg.stride() == exp_avg_sq.stride():
-        raise ValueError("adamw_moments: the codes must be dense and laid out alike")       # (what is not dense is laid out anew)
-    if scales.dtype != torch.float32 or scales.shape != (-(-n // MOMENT_BLOCK), 2) or not scales.is_contiguous():
-        raise ValueError("adamw_moments: scales must be contiguous float32 [ceil(n / 256), 2]")
-    dev = _lib.one_device([exp_avg, exp_avg_sq, scales], "adamw_moments")
-    with _lib.device_guard(dev):
-        _lib.check(_lib.load().mne_adamw_moments(exp_avg.data_ptr(), exp_avg_sq.data_ptr(), scales.data_ptr(), n, m.data_ptr(),
-                                                 v.data_ptr(), _lib.raw_stream(dev)), "mne_adamw_moments")
-    return m, v
+    return tuple(_lib.host_tensors().adamw_moments(exp_avg, exp_avg_sq, scales))
 
 
 class FusedAdamW(torch.optim.Optimizer):

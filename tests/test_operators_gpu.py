@@ -67,3 +67,16 @@ def test_expert_rows_needed_gradients(dtype, wtype, need):
 @pytest.mark.parametrize("kind", ["hot", "none", "outside"])
 def test_expert_rows_batches(kind):
     oc.check_expert_rows(DEV, "bf16", 130, 2, 7, 40, 24, kind, odd=False)
+
+
+# enough tokens for several columns a lane (forms of one to four), with one, two and more choices
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n,k,width,out_width", [(9001, 1, 65, 65), (16000, 2, 100, 33), (3001, 5, 512, 1027), (140000, 2, 3, 4), (1025, 3, 1024, 2050)])
+def test_expert_rows_large(dtype, n, k, width, out_width):
+    oc.check_expert_rows(DEV, dtype, n, k, 37, width, out_width, "masked", odd=width % 2 == 1)
+
+
+@pytest.mark.parametrize("kind", ["even", "hot", "masked"])
+@pytest.mark.parametrize("n,k,experts", [(275200, 2, 8), (1 << 20, 1, 4096), (700001, 3, 100)])
+def test_expert_sort_large(n, k, experts, kind):
+    oc.check_expert_sort(DEV, n, k, experts, kind, wide=k == 1)
