@@ -59,7 +59,7 @@ __device__ __forceinline__ void aw_load(float* out, const void* base, long long 
         constexpr int B = N * (int)sizeof(mem) < 16 ? N * (int)sizeof(mem) : 16;
         union { MneBytes<B> v[N * sizeof(mem) / B]; mem e[N]; } r;
 #pragma unroll
-        for (int k = 0; k < N * (int)sizeof(mem) / B; ++k) r.v[k] = ((const MneBytes<B>*)q)[k];
+        for (int k = 0; k < N * (int)sizeof(mem) / B; ++k) r.v[k] = mne_load_once((const MneBytes<B>*)q + k);
 #pragma unroll
         for (int k = 0; k < N; ++k) out[k] = MneElem<T>::get(r.e[k]);
     } else {
@@ -77,7 +77,7 @@ __device__ __forceinline__ void aw_store(const float* x, void* base, long long i
 #pragma unroll
         for (int k = 0; k < N; ++k) r.e[k] = MneElem<T>::put(x[k]);
 #pragma unroll
-        for (int k = 0; k < N * (int)sizeof(mem) / B; ++k) ((MneBytes<B>*)q)[k] = r.v[k];
+        for (int k = 0; k < N * (int)sizeof(mem) / B; ++k) mne_store_once((MneBytes<B>*)q + k, r.v[k]);
     } else {
 #pragma unroll
         for (int k = 0; k < N; ++k) if (i + k < n) q[k] = MneElem<T>::put(x[k]);

@@ -719,10 +719,12 @@ int mne_adamw_step(const int64_t* table, int64_t n_tensors, const mne_adamw_cfg_
     if (!adamw_types(cfg->p_type, cfg->g_type)) return fail(-1, "mne_adamw_step: unsupported types of parameter and gradient");
     if (cfg->step < 1) return fail(-1, "mne_adamw_step: step counts from 1");
     const bool small = cfg->state_bits == 8;
+    const int per_wg = mne_adamw_per_wg(cfg->state_bits);
+    const int64_t most = 0xFFFFFFFFll / 256;                // workgroups of a launch: its threads are counted in 32 bits
     const int64_t psize = cfg->p_type == MNE_T_F32 ? 4 : 2, gsize = cfg->g_type == MNE_T_F32 ? 4 : 2;
     for (int64_t i = 0; i < n_tensors; ++i) {               // nothing is launched unless every row is sound
         const int64_t* t = table + 7 * i;
-        if (t[5] < 0 || t[5] > (1ll << 42)) return fail(-1, "mne_adamw_step: bad number of elements");
+        if (t[5] < 0 || t[5] > most * per_wg) return fail(-1, "mne_adamw_step: bad number of elements");
         if (t[5] && (!t[0] || !t[1] || !t[2] || !t[3] || (small && !t[4]))) return fail(-1, "mne_adamw_step: NULL address");
         if (t[0] % psize || t[1] % gsize || (small ? t[4] % 8 : t[2] % 4 || t[3] % 4)) return fail(-1, "mne_adamw_step: misaligned address");
     }
@@ -740,13 +742,12 @@ int mne_adamw_step(const int64_t* table, int64_t n_tensors, const mne_adamw_cfg_
     Adamw32Args a32;
     Adamw8Args a8;
     a32.h = a8.h = h; a32.clk = a8.clk = clk; a32.zero_grad = a8.zero_grad = cfg->zero_grad;
-    const int per_wg = mne_adamw_per_wg(cfg->state_bits);
     int n_seg = 0;
     long long blocks = 0;
     for (int64_t i = 0; i <= n_tensors; ++i) {
         const int64_t* t = table + 7 * i;
         const long long more = i < n_tensors ? (t[5] + per_wg - 1) / per_wg : 0;
-        if (n_seg && (i == n_tensors || n_seg == (small ? MNE_ADAMW8_SEGS : MNE_ADAMW32_SEGS) || blocks + more > 0x7FFFFFFFll)) {
+        if (n_seg && (i == n_tensors || n_seg == (small ? MNE_ADAMW8_SEGS : MNE_ADAMW32_SEGS) || blocks + more > most)) {
             a32.n_seg = a8.n_seg = n_seg;
             if (small) mne_launch_adamw8(a8, cfg->p_type, cfg->g_type, (unsigned)blocks, (hipStream_t)stream);
             else mne_launch_adamw32(a32, cfg->p_type, cfg->g_type, (unsigned)blocks, (hipStream_t)stream);
@@ -770,7 +771,7 @@ int mne_adamw_step(const int64_t* table, int64_t n_tensors, const mne_adamw_cfg_
 }
 
 int mne_adamw_moments(const int8_t* m, const uint8_t* v, const float* scales, int64_t n, float* exp_avg, float* exp_avg_sq, void* stream) {
-    if (n < 0 || n > (1ll << 38)) return fail(-1, "mne_adamw_moments: bad number of elements");
+    if (n < 0 || n > (1ll << 34) - 4096) return fail(-1, "mne_adamw_moments: bad number of elements");
     if (n == 0) return 0;
     if (!m || !v || !scales || !exp_avg || !exp_avg_sq) return fail(-1, "mne_adamw_moments: NULL argument");
     mne_launch_adamw_moments(m, v, scales, n, exp_avg, exp_avg_sq, (hipStream_t)stream);
@@ -801,8 +802,6 @@ static int expert_rows(ExpertRowArgs& a, const char* what, int type, int64_t n, 
     if (type != MNE_T_F32 && type != MNE_T_BF16 && type != MNE_T_F16) return fail(-1, std::string(what) + ": unsupported type");
     if (n < 0 || k < 1 || n * (int64_t)k > 0x7FFFFFFFll || n > 0x7FFFFFFFll || width < 0 || width > (1ll << 28)) return fail(-1, std::string(what) + ": bad size");
     if (n && width && !position) return fail(-1, std::string(what) + ": NULL argument");
-    const int64_t per = type == MNE_T_F32 ? 4 : 8;
-    if (n * ((width / per + per + 63) / 64 + 1) > (1ll << 31)) return fail(-1, std::string(what) + ": too many elements for one launch");
     a.n = (int)n; a.k = k; a.width = (int)width; a.position = position;
     return 0;
 }
@@ -815,7 +814,7 @@ int mne_expert_dispatch(const void* x, int64_t x_stride, int type, int64_t n, in
     if (n == 0 || width == 0) return 0;
     if (!x || !live || !out) return fail(-1, "mne_expert_dispatch: NULL argument");
     a.a = x; a.a_stride = row_bytes(type, x_stride); a.total = live; a.out = out;
-    mne_launch_expert_dispatch(a, type, (hipStream_t)stream);
+    if (mne_launch_expert_dispatch(a, type, (hipStream_t)stream)) return fail(-1, "mne_expert_dispatch: too many elements for one launch");
     return check_launch("expert_dispatch");
 }
 
@@ -826,7 +825,7 @@ int mne_expert_combine(const void* y, int64_t y_stride, int type, int64_t n, int
     if (n == 0 || width == 0) return 0;
     if (!y || !out) return fail(-1, "mne_expert_combine: NULL argument");
     a.a = y; a.a_stride = row_bytes(type, y_stride); a.weights = weights; a.out = out;
-    mne_launch_expert_combine(a, type, (hipStream_t)stream);
+    if (mne_launch_expert_combine(a, type, (hipStream_t)stream)) return fail(-1, "mne_expert_combine: too many elements for one launch");
     return check_launch("expert_combine");
 }
 
@@ -839,7 +838,7 @@ int mne_expert_combine_backward(const void* dout, int64_t dout_stride, const voi
     if (!dout || !live || (dw && !y)) return fail(-1, "mne_expert_combine_backward: NULL argument");
     a.a = dout; a.a_stride = row_bytes(type, dout_stride); a.b = y; a.b_stride = row_bytes(type, y_stride);
     a.total = live; a.weights = weights; a.out = dy; a.dw = dw;
-    mne_launch_expert_combine_backward(a, type, (hipStream_t)stream);
+    if (mne_launch_expert_combine_backward(a, type, (hipStream_t)stream)) return fail(-1, "mne_expert_combine_backward: too many elements for one launch");
     return check_launch("expert_combine_backward");
 }
 

@@ -234,17 +234,21 @@ struct DispatchNode : torch::autograd::Function<DispatchNode> {
 };
 
 struct CombineNode : torch::autograd::Function<CombineNode> {
-    static Variable forward(AutogradContext* ctx, const Variable& y, const Variable& position, const Variable& offsets, const Variable& weights) {
+    // (a node takes no undefined tensor: without weights, `weights` is any other)
+    static Variable forward(AutogradContext* ctx, const Variable& y, const Variable& position, const Variable& offsets, const Variable& weights,
+                            bool weighted) {
         ctx->save_for_backward({y, position, offsets, weights});
         ctx->saved_data["library"] = std::string((const char*)&g_lib, sizeof(g_lib));
-        return combine(g_lib, y, position, weights);
+        ctx->saved_data["weighted"] = weighted;
+        return combine(g_lib, y, position, weighted ? weights : at::Tensor());
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         once("expert_combine");
-        if (!grads[0].defined()) return {Variable(), Variable(), Variable(), Variable()};
+        if (!grads[0].defined()) return {Variable(), Variable(), Variable(), Variable(), Variable()};
         const Library lib = library_of(ctx);
         const variable_list saved = ctx->get_saved_variables();
-        const at::Tensor y = rows(saved[0], "expert_combine"), &position = saved[1], &offsets = saved[2], &weights = saved[3];
+        const at::Tensor y = rows(saved[0], "expert_combine"), &position = saved[1], &offsets = saved[2];
+        const at::Tensor weights = ctx->saved_data["weighted"].toBool() ? saved[3] : at::Tensor();
         const at::Tensor dout = rows(grads[0], "expert_combine"), w = weights.defined() ? weights.to(at::kFloat).contiguous() : weights;
         const c10::DeviceGuard guard(y.device());
         const int64_t n = position.size(0), k = position.size(1), width = y.size(1);
@@ -255,7 +259,7 @@ struct CombineNode : torch::autograd::Function<CombineNode> {
         check(lib.combine_backward(dout.data_ptr(), dout.stride(0), y.data_ptr(), y.stride(0), type_code(y.scalar_type()), n, (int)k, width,
                                    ints(position), live_rows(offsets), floats(w), want_dy ? dy.data_ptr() : nullptr,
                                    want_dw ? (float*)dw.data_ptr() : nullptr, stream_of(y.device())), "mne_expert_combine_backward");
-        return {dy, Variable(), Variable(), want_dw ? dw.to(weights.scalar_type()) : dw};
+        return {dy, Variable(), Variable(), want_dw ? dw.to(weights.scalar_type()) : dw, Variable()};
     }
 };
 
@@ -277,7 +281,7 @@ at::Tensor expert_combine(const at::Tensor& y, const at::Tensor& position, const
         if (type_code(w.scalar_type()) < 0) throw py::type_error("expert_combine: weights must be float32, bfloat16 or float16");
     }
     rows(y, "expert_combine");
-    return CombineNode::apply(y, position, offsets, w);
+    return CombineNode::apply(y, position, offsets, w.defined() ? w : position, w.defined());
 }
 
 }  // namespace

@@ -105,12 +105,15 @@ static __device__ __forceinline__ int mne_xcc_id() {
 #endif
 
 // B bytes of memory that are loaded and stored as one
-template <int B> struct MneBytes;
-template <> struct MneBytes<16> { uint4 v; };
-template <> struct MneBytes<8> { uint2 v; };
-template <> struct MneBytes<4> { unsigned v; };
-template <> struct MneBytes<2> { unsigned short v; };
-template <> struct MneBytes<1> { unsigned char v; };
+template <int B> struct MneBytes { typedef unsigned words __attribute__((ext_vector_type(B / 4))); words v; };
+template <> struct MneBytes<4> { typedef unsigned words; words v; };
+// of data that nothing reads again soon: it leaves the caches to others
+template <int B> static __device__ __forceinline__ MneBytes<B> mne_load_once(const MneBytes<B>* p) {
+    MneBytes<B> x;
+    x.v = __builtin_nontemporal_load(&p->v);
+    return x;
+}
+template <int B> static __device__ __forceinline__ void mne_store_once(MneBytes<B>* p, const MneBytes<B>& x) { __builtin_nontemporal_store(x.v, &p->v); }
 
 // the unsigned integer of B bytes
 template <int B> struct MneWord;

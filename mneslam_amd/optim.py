@@ -177,11 +177,17 @@ class FusedAdamW(torch.optim.Optimizer):
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits, seed=int(seed)))
 
     def add_param_group(self, param_group):
-        super().add_param_group(param_group)
-        group = self.param_groups[-1]
+        group = {**self.defaults, **param_group}
         _check_hyper(group["lr"], group["betas"], group["eps"], group["weight_decay"])
         if group["state_bits"] not in (8, 32):
             raise ValueError(f"Invalid state_bits: {group['state_bits']} (8 or 32)")
+        super().add_param_group(param_group)
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        for group in self.param_groups:                 # (a state of torch.optim.AdamW has neither)
+            group.setdefault("state_bits", 32)
+            group.setdefault("seed", 0)
 
     def _state(self, p, bits):
         st = self.state[p]
@@ -235,19 +241,25 @@ class FusedAdamW(torch.optim.Optimizer):
         return loss
 
     def moments(self, p):
-        """(exp_avg, exp_avg_sq) of ``p`` in fp32."""
-        st = self.state[p]
+        """(exp_avg, exp_avg_sq) of ``p`` in fp32 (zero before its first step)."""
+        st = self.state.get(p)
+        if not st:
+            return torch.zeros_like(p, dtype=torch.float32), torch.zeros_like(p, dtype=torch.float32)
         return adamw_moments(st["exp_avg"], st["exp_avg_sq"], st["scales"]) if "scales" in st else (st["exp_avg"], st["exp_avg_sq"])
 
     def load_state_dict(self, state_dict):
-        """The base class casts floating-point state to its parameter's type: moments and scales are put back as they were saved."""
+        """Also of torch.optim.AdamW's states.  The base class casts floating-point state to its parameter's type: here moments and
+        scales are float32 or the codes they were saved as, laid out like their parameter."""
         super().load_state_dict(state_dict)
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
         for i, p in zip(saved, (p for g in self.param_groups for p in g["params"])):
             for key, value in state_dict["state"].get(i, {}).items():
-                if torch.is_tensor(value):
-                    like = p if value.shape == p.shape else value
-                    self.state[p][key] = torch.empty_like(like, dtype=value.dtype, device=p.device).copy_(value)
+                if key == "step":
+                    self.state[p][key] = int(value)
+                elif key in ("exp_avg", "exp_avg_sq", "scales"):
+                    like = value if key == "scales" else p
+                    dtype = torch.float32 if value.is_floating_point() else value.dtype
+                    self.state[p][key] = torch.empty_like(like, dtype=dtype, device=p.device, requires_grad=False).copy_(value)
 
     def zero_grad(self, set_to_none=True):
         for group in self.param_groups:

@@ -10,6 +10,7 @@ the xGMI form of the same hand-off is mneslam_amd/dist.py):
 
   save_latest_checkpoint   mneslam_mp.py:294-315      agent_<rank>/latest_checkpoint.pt
   load_foreign_model       mp_slam/mapper.py:708-726  (reader of the above)
+  load_agent_maps          several peers' maps and the own one, answering point queries as one (model/agent_maps.py)
   save_keyframe_poses / load_keyframe_poses   mp_slam/mapper.py:565-592, :344-356   key_est_poses.npy, key_timestamps.npy
 
 The rest of mneslam_mp.py (dataset, DROID tracker, threads, checkpoints, image dumps) is
@@ -149,6 +150,18 @@ def load_foreign_model(model_shared, config, other_rank, device, exchange=None):
         model_shared.bounding_box = ckpt["bounding_box"].to(device)
     model_shared.eval()
     return ckpt
+
+
+def load_agent_maps(model, config, other_ranks, new_model, device, exchange=None, top=2):
+    """This agent's ``model`` and the maps of ``other_ranks`` as one (model.agent_maps.AgentMaps): ``new_model()`` makes an empty scene
+    model for each of them, which ``load_foreign_model`` fills."""
+    from .model.agent_maps import AgentMaps
+    models = [model]
+    for rank in other_ranks:
+        foreign = new_model()
+        load_foreign_model(foreign, config, rank, device, exchange=exchange)
+        models.append(foreign)
+    return AgentMaps(models, top=top)
 
 
 def save_keyframe_poses(config, rank, poses_c2w, timestamps):

@@ -31,9 +31,9 @@ def mix(h):
     return h ^ (h >> np.uint64(16))
 
 
-def dither(seed, ordinal, step, n):
-    """u_m, u_r of the n elements of a tensor (float32, multiples of 2^-16)."""
-    i = np.arange(n, dtype=np.uint64)
+def dither(seed, ordinal, step, n, start=0):
+    """u_m, u_r of the elements start .. start + n - 1 of a tensor (float32, multiples of 2^-16)."""
+    i = np.arange(start, start + n, dtype=np.uint64)
     key = mix(np.uint64((seed + ordinal * GOLD) & U32))
     key = mix(((key + np.uint64(step * GOLD & U32)) & np.uint64(U32)) ^ mix((i >> np.uint64(8)) & np.uint64(U32)))
     h = (key + (i & np.uint64(255)) * np.uint64(GOLD)) & np.uint64(U32)
@@ -71,15 +71,15 @@ def encode8(x, u, top, most, least):
     return np.minimum(c, f(most)).reshape(-1)[:n], scale, np.repeat(some, 256)[:n]
 
 
-def adamw8_ieee(g, mc, rc, scales, seed, ordinal, step, betas):
-    """New codes and scales, bit for bit (g float32)."""
+def adamw8_ieee(g, mc, rc, scales, seed, ordinal, step, betas, start=0):
+    """New codes and scales, bit for bit (g float32), of a tensor's blocks from element `start` on."""
     f = np.float32
     b1, o1, b2, o2 = f(betas[0]), f(1.0 - betas[0]), f(betas[1]), f(1.0 - betas[1])
     with np.errstate(all="ignore"):
         m, r = values8(mc, rc, scales)
         m = m * b1 + g * o1
         r = np.sqrt((r * r) * b2 + (g * g) * o2)
-        um, ur = dither(seed, ordinal, step, g.size)
+        um, ur = dither(seed, ordinal, step, g.size, start)
         cm, sm, _ = encode8(np.abs(m), um, 16129, 127, 2.0 ** -100)
         cr, sr, some = encode8(r, ur, 65025, 255, 0)
         cr = np.where((cr == 0) & (r > 0) & some, f(1), cr)
@@ -308,3 +308,434 @@ def check_expert_rows(device, dtype, n, k, experts, width, out_width, kind, odd,
         want[slot], scale[slot] = (GO[tok] * Y).sum(1), np.abs(GO[tok] * Y).sum(1)
         near(got["w"], want.reshape(n, k), scale.reshape(n, k), out_width, "dw")
         assert got["w"].dtype == wt
+
+
+# ----------------------------------------------------------------------------------------------------------- run together
+def check_agent_maps(device, tmp_path):
+    """Two agents' maps with overlapping boxes, one of them read from its checkpoint: the union's answers against each map queried by
+    itself and blended in float64."""
+    import parity_cases as pc
+    from helpers import load_golden
+    from mneslam_amd import configs, slam_glue
+    from mneslam_amd.model.agent_maps import AgentMaps
+    g = load_golden("fwd_colorplanes")
+    cfg = configs.small_test_config(one_grid=False, depth_trunc=3.0)
+    cfg["data"]["output"], cfg["data"]["exp_name"] = str(tmp_path), "union"
+    own, other = (pc.model_from_golden(g, cfg, device).eval() for _ in range(2))
+    box = own.bounding_box.clone()
+    with torch.no_grad():
+        for p in other.decoder.parameters():
+            p.mul_(-0.5)
+    own.bounding_box = box.clone()
+    own.bounding_box[0, 1] = box[0].mean() + 0.2
+    other.bounding_box = box.clone()
+    other.bounding_box[0, 0] = box[0].mean() - 0.2
+    slam_glue.save_latest_checkpoint(other, cfg, 1)
+    union = slam_glue.load_agent_maps(own, cfg, [1], lambda: pc.model_from_golden(g, cfg, device).eval(), torch.device(device))
+    gen = torch.Generator().manual_seed(3)
+    lo, hi = box[:, 0].float().cpu(), box[:, 1].float().cpu()
+    pts = lo + (hi - lo) * (torch.rand(211, 3, generator=gen) * 1.2 - 0.1)        # some in no box
+    pts[0], pts[1] = own.bounding_box[:, 1].float().cpu(), float("nan")
+    pts = pts.to(device)
+    ids, w = union.route(pts)
+    raw = union.query_color_sdf(pts)
+    with torch.no_grad():
+        alone = torch.stack([m.query_color_sdf(torch.nan_to_num(pts)).double() for m in union.models], 1)
+    held = ids >= 0
+    want = torch.where(held[..., None], alone.gather(1, ids.clamp(min=0).long()[..., None].expand(-1, -1, 4)) * w.double()[..., None], 0.0).sum(1)
+    assert torch.equal(union.covered(pts), held[:, 0]) and 0 < int(held[:, 1].sum()) < int(held[:, 0].sum()) < len(pts)
+    assert (w.sum(1)[held[:, 0]] - 1).abs().max() < 1e-6 and (raw[~held[:, 0]] == 0).all()
+    # the same kernels on the same points (a row's answer does not depend on its neighbours), two fp32 products and their sum
+    assert ((raw.double() - want).abs() <= 4 * EPS32 * (alone.abs().amax(1) + 1e-30)).all()
+    assert torch.equal(union.query_sdf(pts), raw[:, 3]) and union.query_color(pts).shape == (211, 3)
+    assert AgentMaps([own]).top == 1
+
+
+def check_mixture_step(device, bits, ptype="f32"):
+    """A mixture of small experts on grid features, trained for some steps: routing and its gradients, the experts on their runs, one
+    AdamW call for all their tensors -- against the same model in float64 (gradients of the first step), with 32-bit moments the
+    parameters after each step too."""
+    from mneslam_amd.optim import FusedAdamW
+    from mneslam_amd.routing import expert_combine, expert_dispatch, expert_sort
+    dt = NAMES[ptype]
+    gen = torch.Generator().manual_seed(12)
+    n, k, e, d, h = 150, 2, 5, 19, 16
+    x = torch.randn(n, d, generator=gen).to(dt).to(device).requires_grad_(True)
+    target = torch.randn(n, 4, generator=gen).to(device)
+    ids = make_ids("masked", n, k, e, gen)
+    ids[ids == 3] = 1                                              # an expert without a row
+    logits = torch.nn.Parameter((torch.randn(n, k, generator=gen)).to(device))
+    experts = [[torch.nn.Parameter((torch.randn(h, d, generator=gen) / d ** 0.5).to(dt).to(device)),
+                torch.nn.Parameter((torch.randn(4, h, generator=gen) / h ** 0.5).to(dt).to(device))] for _ in range(e)]
+    flat = [p for pair in experts for p in pair]
+    opt = FusedAdamW([{"params": [logits], "state_bits": 32}, {"params": flat}], lr=0.01, betas=(0.9, 0.99), weight_decay=0.02, state_bits=bits, seed=4)
+    order, position, _ = plan64(ids.numpy(), e)
+
+    def exact_loss(xv, lv, ws):
+        out = 0.0
+        w = torch.softmax(lv, 1)
+        rows = []
+        for t in range(n):
+            acc = torch.zeros(4, dtype=torch.float64)
+            for j in range(k):
+                i = int(ids[t, j])
+                if i >= 0:
+                    acc = acc + w[t, j] * (ws[2 * i + 1] @ torch.tanh(ws[2 * i] @ xv[t]))
+            rows.append(acc)
+        return torch.square(torch.stack(rows) - target.double().cpu()).mean()
+
+    plan = expert_sort(ids.to(device), e)
+    sizes = plan.sizes()
+    for step in range(1, 4):
+        rows = expert_dispatch(x, plan)
+        ys, at = [], 0
+        for (a, b), size in zip(experts, sizes):
+            ys.append(torch.tanh(rows[at:at + size].float() @ a.float().t()) @ b.float().t())
+            at += size
+        ys.append(torch.zeros(n * k - at, 4, device=device))
+        out = expert_combine(torch.cat(ys), plan, torch.softmax(logits, 1))
+        loss = torch.square(out - target).mean()
+        opt.zero_grad()
+        x.grad = None
+        loss.backward()
+        if step == 1:
+            dbl = [t.detach().double().cpu().requires_grad_(True) for t in [x, logits] + flat]
+            want = torch.autograd.grad(exact_loss(dbl[0], dbl[1], dbl[2:]), dbl, allow_unused=True)
+            for t, g in zip([x, logits] + flat, want):
+                if g is None or not g.abs().max():
+                    assert t.grad is None or not t.grad.abs().max()      # the expert without a row
+                    continue
+                # sums of up to n k d fp32 products; a 16-bit gradient is rounded on its way (rows, and their sum over k)
+                tol = (2e-5 if t.dtype == torch.float32 and dt == torch.float32 else 4 * torch.finfo(dt).eps) * float(g.abs().max())
+                assert (t.grad.double().cpu() - g).abs().max() <= tol, t.shape
+        before = [(_np(p).copy(), _np(p.grad).copy(), [_np(v).copy() for v in opt.moments(p)]) if p.grad is not None and p in opt.state else None for p in flat]
+        opt.step()
+        for p, b in zip(flat, before):
+            if b is None or bits != 32:
+                continue
+            want_p, _, want_v = adamw64(b[0], b[1], b[2][0], b[2][1], step, 0.01, (0.9, 0.99), 1e-8, 0.02)
+            size, root_bc2, _ = constants(step, 0.01, (0.9, 0.99), 0.02)
+            upd = size * (0.9 * np.abs(b[2][0]) + 0.1 * np.abs(b[1])) / (np.sqrt(want_v) / root_bc2 + 1e-8)
+            assert_rounded(p, want_p, 16 * EPS32 * upd + 4 * EPS32 * np.abs(b[0]), step)
+    assert all(torch.isfinite(p).all() for p in flat) and opt.state[flat[0]]["step"] == 3
+
+
+# ------------------------------------------------------------------------------------------------- AdamW: the rest of its contract
+def _state_for(p, bits, device):
+    if bits == 32:
+        return [torch.zeros_like(p, dtype=torch.float32) for _ in range(2)], None
+    return [torch.zeros_like(p, dtype=torch.int8), torch.zeros_like(p, dtype=torch.uint8)], torch.zeros(-(-p.numel() // 256), 2, device=device)
+
+
+def _step(ps, gs, bits, device, step=1, state=None, **kw):
+    state = state or [_state_for(p, bits, device) for p in ps]
+    args = dict(step=step, lr=0.01, betas=(0.9, 0.99), eps=1e-8, weight_decay=0.0)
+    args.update(kw)
+    optim.adamw_step(ps, gs, [s[0][0] for s in state], [s[0][1] for s in state], [s[1] for s in state] if bits == 8 else None, **args)
+    return state
+
+
+def check_adamw_refusals(device):
+    p, g = torch.ones(300, device=device), torch.ones(300, device=device)
+    before = p.clone()
+    m, v = torch.zeros_like(p), torch.zeros_like(p)
+    c, d, s = torch.zeros(300, dtype=torch.int8, device=device), torch.zeros(300, dtype=torch.uint8, device=device), torch.zeros(2, 2, device=device)
+    ok = dict(step=1, lr=0.1)
+
+    def bad(error, *lists, scales=None, **kw):
+        with pytest.raises(error):
+            optim.adamw_step(*[[x] if torch.is_tensor(x) else x for x in lists], scales, **{**ok, **kw})
+
+    bad(ValueError, [p, p], g, m, v)
+    bad(ValueError, [p, p], [g, g], [m, m.clone()], [v, v.clone()])
+    bad(ValueError, [p[:200], p[100:]], [g[:200], g[100:]], [m[:200], m[100:]], [v[:200], v[100:]])          # overlapping
+    for kw in (dict(step=0), dict(step=-3), dict(step=1 << 31), dict(lr=-1.0), dict(lr=float("nan")), dict(betas=(1.0, 0.9)), dict(betas=(0.9, -0.1)),
+               dict(eps=-1e-8), dict(weight_decay=-1.0), dict(seed=-1), dict(seed=1 << 32), dict(ordinals=[-1]), dict(ordinals=[1 << 32]), dict(ordinals=[])):
+        bad(ValueError, p, g, m, v, **kw)
+    bad(TypeError, p.double(), g, m, v)
+    bad(TypeError, p, g.double(), m, v)
+    bad(TypeError, p.bfloat16(), g.half(), m, v)
+    bad(TypeError, p, g, m.bfloat16(), v)
+    bad(TypeError, p, g, m, v, scales=[s])                                   # 32-bit moments with scales
+    bad(TypeError, p, g, c, d)                                               # codes without
+    bad(ValueError, p, g[:299], m, v)
+    bad(ValueError, p, g, m.view(3, 100), v)
+    bad(ValueError, p, g, c, d, scales=[s[:1]])
+    bad(ValueError, p, g, c, d, scales=[s.t().contiguous().t()])
+    bad(ValueError, p, g, c, d, scales=[s.double()])
+    wide = torch.ones(300, 2, device=device)
+    bad(ValueError, wide[:, 0], g, m, v)                                     # not dense
+    bad(ValueError, p[:1].expand(300), g, m, v)
+    bad(ValueError, torch.ones(20, 15, device=device), g.view(20, 15), m.view(15, 20).t(), v.view(20, 15))
+    bad(ValueError, torch.ones(20, 15, device=device), g.view(15, 20).t(), m.view(20, 15), v.view(20, 15), zero_grad=True)
+    bad(ValueError, p, g.to_sparse(), m, v)
+    bad(TypeError, p, [None], m, v)
+    for args in ((c.float(), d, s), (c, d.to(torch.int8), s), (c, d[:299], s), (c, d, s[:1]), (c[::2], d[::2], s[:1])):
+        with pytest.raises((TypeError, ValueError)):
+            optim.adamw_moments(*args)
+    assert torch.equal(p, before) and not m.any() and not c.any()            # nothing was touched
+    optim.adamw_step([], [], [], [], **ok)
+    optim.adamw_step([p[:0]], [g[:0]], [m[:0]], [v[:0]], **ok)
+    if device != "cpu":
+        bad(ValueError, p.cpu(), g, m, v)
+        bad(ValueError, p.cpu(), g.cpu(), m.cpu(), v.cpu())
+
+
+def check_adamw_nonfinite(device, bits):
+    """A gradient that is not finite: its own element with 32-bit moments, its block's moments with 8-bit ones, nothing else."""
+    for value in (float("nan"), float("inf"), -float("inf"), 1e30):
+        p, g = torch.ones(1000, device=device), torch.full((1000,), 0.01, device=device)
+        g[300] = value
+        state = _step([p], [g], bits, device)
+        first = p.clone()
+        g[300] = 0.01
+        _step([p], [g], bits, device, step=2, state=state)
+        assert torch.isfinite(first[:256]).all() and torch.isfinite(p[512:]).all() and torch.isfinite(p[:256]).all()
+        if bits == 32:
+            m, v = state[0][0]
+            ok = torch.ones(1000, dtype=torch.bool, device=device)
+            ok[300] = False
+            assert torch.isfinite(p[ok]).all() and torch.isfinite(m[ok]).all()
+            assert torch.isnan(p[300]) if value != 1e30 else p[300] == first[300] == 1.0       # 1e30 squared is infinite: no update
+        else:
+            m, v = optim.adamw_moments(*state[0][0], state[0][1])
+            assert torch.isfinite(m[:256]).all() and torch.isfinite(v[512:]).all() and torch.isnan(v[256:512]).all()
+            assert torch.isnan(m[256:512]).all() == (value != 1e30) and torch.isnan(p[256:512]).all()
+
+
+def check_adamw8_small_and_zero(device):
+    """Zero blocks stay zero, tiny values neither overflow a scale nor lose the second moment."""
+    p, g = torch.ones(1024, device=device), torch.zeros(1024, device=device)
+    g[256:512] = 1e-20                                     # the square of its tenth is below fp32's range
+    g[512:768] = 1e-34                                     # and this one's moment below what a scale can hold
+    g[768] = 1.0
+    g[769] = 1e-9                                          # far below its block's largest
+    state = _step([p], [g], 8, device)
+    (mc, rc), sc = state[0]
+    m, v = optim.adamw_moments(mc, rc, sc)
+    assert not m[:256].any() and not v[:256].any() and (p[:256] == 1).all() and torch.isfinite(p).all()
+    assert (sc[2] == 0).all() and not mc[512:768].any() and float(v[769]) > 0
+    want = adamw64(np.ones(256), g[768:].cpu().double().numpy(), np.zeros(256), np.zeros(256), 1, 0.01, (0.9, 0.99), 1e-8, 0.0)[0]
+    assert np.abs(p[768:].cpu().double().numpy() - want).max() <= 40 * EPS32
+    for step in range(2, 30):
+        _step([p], [g], 8, device, step=step, state=state)
+    assert torch.isfinite(p).all() and (p[:256] == 1).all()
+    assert float((1 - p[769]).abs()) < 0.31                # thirty steps of at most lr each
+
+
+def check_adamw8_dither(device):
+    """Moments that change by less than a code a step still move, by the right amount on average; the codes are a function of seed,
+    ordinal, step and element alone."""
+    n = 256 * 64
+    p, g = torch.zeros(n, device=device), torch.full((n,), 0.5, device=device)
+    g[::256] = 1.0                                         # the block's largest, held up by its own gradient
+    state = _step([p], [g], 8, device, betas=(0.0, 0.0))   # m = g, sqrt(v) = g
+    rest = torch.arange(n, device=device) % 256 != 0
+    hold = torch.where(rest, 0.0, 1.0)
+    for step in range(2, 202):
+        _step([p], [hold], 8, device, step=step, state=state, betas=(0.999, 0.999))
+    m, v = optim.adamw_moments(*state[0][0], state[0][1])
+    # unbiased: the mean of m over 16320 elements follows 0.5 * 0.999^200.  One step's rounding has at most half a code's standard
+    # deviation, (2 c + 1) / (2 * 127^2) with c = 90: 200 steps, 16320 elements, five standard deviations
+    want, sd = 0.5 * 0.999 ** 200, 181 / (2 * 16129) * 200 ** 0.5 / 16320 ** 0.5
+    assert abs(float(m[rest].double().mean()) - want) < 5 * sd
+    # sqrt(v) is what is unbiased: v's mean is above by the variance of sqrt(v), at most 200 codes' of (2 * 180 + 1) / (2 * 255^2) each
+    want_r, sd_r = 0.5 * 0.999 ** 100, 361 / (2 * 65025) * 200 ** 0.5
+    assert abs(float(v[rest].double().sqrt().mean()) - want_r) < 5 * sd_r / 16320 ** 0.5 + sd_r ** 2 / want_r
+    again = {}
+    for name, kw in (("same", {}), ("same2", {}), ("seed", dict(seed=1)), ("ordinal", dict(ordinals=[5])), ("step", dict(step=2))):
+        st = _step([torch.zeros(n, device=device)], [torch.linspace(0, 1, n, device=device)], 8, device, **{"seed": 0, **kw})
+        again[name] = (st[0][0][0], st[0][0][1])
+    assert all(torch.equal(a, b) for a, b in zip(again["same"], again["same2"]))
+    for name in ("seed", "ordinal", "step"):
+        assert all(0.02 < (a != b).float().mean() for a, b in zip(again["same"], again[name])), name
+
+
+def check_fused_adamw(device):
+    """The optimizer against torch.optim.AdamW: groups, steps that skip a tensor, saved and loaded states."""
+    gen = torch.Generator().manual_seed(2)
+    shapes = [(7, 9), (300,), (1, 4, 6, 5), (1,)]
+    start = [torch.randn(s, generator=gen) for s in shapes]
+    start[2] = start[2].contiguous(memory_format=torch.channels_last)
+    make = lambda dev: [torch.nn.Parameter(t.clone().to(dev)) for t in start]        # noqa: E731
+    ours, theirs = make(device), make("cpu")
+    groups = lambda ps: [{"params": ps[:2], "lr": 0.02, "weight_decay": 0.1}, {"params": ps[2:], "eps": 1e-6, "betas": (0.5, 0.9)}]  # noqa: E731
+    opt, ref = optim.FusedAdamW(groups(ours), lr=0.005), torch.optim.AdamW(groups([p for p in theirs]), lr=0.005)
+    versions = [p._version for p in ours]
+    for step in range(5):
+        for k, (p, q) in enumerate(zip(ours, theirs)):
+            grad = None if step in (1, 2) and k == 1 else torch.randn(q.shape, generator=gen)
+            q.grad, p.grad = grad, None if grad is None else grad.to(device)
+        assert opt.step(lambda: torch.tensor(3.0)) == 3.0
+        ref.step()
+        if step == 2:                                          # through a saved state, into new objects
+            saved = opt.state_dict()
+            ours2 = [torch.nn.Parameter(p.detach().clone()) for p in ours]
+            opt = optim.FusedAdamW(groups(ours2), lr=0.005)
+            opt.load_state_dict(saved)
+            ours = ours2
+            versions = [p._version for p in ours]
+    assert all(p._version > v for p, v in zip(ours, versions))        # what autograd saved of a parameter is out of date
+    for p, q in zip(ours, theirs):
+        assert (p.detach().cpu() - q.detach()).abs().max() <= 5 * 30 * EPS32 * (q.abs().max() + 1)
+    # torch.optim.AdamW's own state
+    opt2 = optim.FusedAdamW(groups([torch.nn.Parameter(p.detach().clone()) for p in ours]), lr=0.005)
+    opt2.load_state_dict(ref.state_dict())
+    for p, q in zip((p for g in opt2.param_groups for p in g["params"]), theirs):
+        assert opt2.state[p]["step"] == int(ref.state[q]["step"]) and opt2.state[p]["exp_avg"].dtype == torch.float32
+        p.grad = torch.ones_like(p)
+    opt2.step(zero_grad=True)
+    assert all(not p.grad.any() for g in opt2.param_groups for p in g["params"])
+    # 8-bit states of 16-bit parameters survive a round trip bit for bit
+    ps = [torch.nn.Parameter(t.clone().bfloat16().to(device)) for t in start]
+    opt = optim.FusedAdamW([{"params": ps[:1], "state_bits": 32}, {"params": ps[1:]}], state_bits=8, seed=9)
+    for _ in range(2):
+        for p in ps:
+            p.grad = torch.randn(p.shape, generator=gen).bfloat16().to(device)
+        opt.step()
+    saved = opt.state_dict()
+    other = [torch.nn.Parameter(p.detach().clone()) for p in ps]
+    opt_b = optim.FusedAdamW([{"params": other[:1]}, {"params": other[1:]}])
+    opt_b.load_state_dict(saved)
+    for p, q in zip(ps, other):
+        q.grad = p.grad.clone()
+        for key, value in opt.state[p].items():
+            loaded = opt_b.state[q][key]
+            assert loaded == value if key == "step" else (loaded.dtype == value.dtype and loaded.stride() == value.stride() and torch.equal(loaded, value)), key
+    opt.step()
+    opt_b.step()
+    for p, q in zip(ps, other):
+        assert torch.equal(p, q) and all(torch.equal(a, b) for a, b in zip(opt.moments(p), opt_b.moments(q)))
+    for kw in (dict(lr=-1), dict(betas=(0.9, 1.0)), dict(eps=-1), dict(weight_decay=-1), dict(state_bits=4), dict(seed=-1)):
+        with pytest.raises(ValueError):
+            optim.FusedAdamW(ps, **kw)
+    opt = optim.FusedAdamW([torch.nn.Parameter(torch.ones(3, device=device))])
+    with pytest.raises(ValueError):
+        opt.add_param_group({"params": [torch.nn.Parameter(torch.ones(2, device=device))], "state_bits": 16})
+    assert len(opt.param_groups) == 1
+    p = opt.param_groups[0]["params"][0]
+    assert not opt.moments(p)[0].any() and not opt.state
+    opt.zero_grad()
+    opt.step()                                                 # nothing has a gradient
+    assert (p == 1).all()
+
+
+def check_adamw_many(device, count, bits):
+    """More tensors than a launch holds, of mixed types and sizes."""
+    gen = torch.Generator().manual_seed(8)
+    types = [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16), (torch.float16, torch.float32)]
+    ps, gs = [], []
+    for k in range(count):
+        n, (pt, gt) = int(torch.randint(0, 700, (1,), generator=gen)), types[k % 3 if k % 5 else 0]
+        ps.append(torch.randn(n, generator=gen).to(pt).to(device))
+        gs.append(torch.randn(n, generator=gen).to(gt).to(device))
+    alone = [p.clone() for p in ps]
+    state = _step(ps, gs, bits, device, step=3)
+    for k, (p, g) in enumerate(zip(alone, gs)):
+        st = _step([p], [g], bits, device, step=3, ordinals=[k])
+        assert torch.equal(p, ps[k]) and all(torch.equal(a, b) for a, b in zip(st[0][0], state[k][0])), k
+
+
+def check_adamw_clock(device, bits):
+    """Steps that read their number from device memory equal those that are given it."""
+    import ctypes as C
+    from mneslam_amd import _lib
+    betas = (0.9, 0.99)
+    offset = torch.zeros(1, dtype=torch.int32, device=device)
+    table = torch.tensor([[1 - betas[0] ** t, 1 - betas[1] ** t] for t in range(1, 40)], dtype=torch.float64, device=device)
+    clock = _lib.Clock()
+    clock.step_offset, clock.bias_table, clock.n_table = offset.data_ptr(), table.data_ptr(), 39
+    clock.beta1, clock.beta2 = betas
+    gen = torch.Generator().manual_seed(4)
+    g = torch.randn(777, generator=gen).to(device)
+    p, q = torch.ones(777, device=device), torch.ones(777, device=device)
+    sp, sq = None, None
+    for k in range(4):
+        sp = _step([p], [g], bits, device, step=5, state=sp, clock=clock)
+        sq = _step([q], [g], bits, device, step=5 + k, state=sq)
+        offset += 1
+        assert torch.equal(p, q) and all(torch.equal(a, b) for a, b in zip(sp[0][0], sq[0][0])), k
+    with pytest.raises(RuntimeError):
+        _step([p], [g], bits, device, step=5, clock=clock, betas=(0.8, 0.99))
+    return clock, offset, table
+
+
+# ----------------------------------------------------------------------------------------------- routing: the rest of its contract
+def check_routing_refusals(device):
+    from mneslam_amd.routing import expert_combine, expert_dispatch, expert_sort
+    ids = torch.zeros(6, 2, dtype=torch.int32, device=device)
+    for bad, error in ((ids.float(), TypeError), (ids.to(torch.int16), TypeError), (ids.view(2, 3, 2), TypeError), (ids[:, :0], ValueError)):
+        with pytest.raises(error):
+            expert_sort(bad, 4)
+    for experts in (0, -1, 4097):
+        with pytest.raises(ValueError):
+            expert_sort(ids, experts)
+    plan = expert_sort(ids[:, 0], 4)
+    assert plan.position.shape == (6, 1) and plan.n_tokens == 6 and plan.top_k == 1
+    plan = expert_sort(ids, 4)
+    x, y, w = torch.ones(6, 5, device=device), torch.ones(12, 5, device=device), torch.ones(6, 2, device=device)
+    for f in (lambda: expert_dispatch(x[:5], plan), lambda: expert_dispatch(x[0], plan), lambda: expert_dispatch(x.view(6, 5, 1), plan),
+              lambda: expert_combine(y[:11], plan), lambda: expert_combine(y, plan, w[:5]), lambda: expert_combine(y, plan, w.t()),
+              lambda: expert_combine(y.view(12, 5, 1), plan), lambda: expert_combine(y, plan, w[:, :1]), lambda: expert_dispatch(x.to_sparse(), plan)):
+        with pytest.raises(ValueError):
+            f()
+    for f in (lambda: expert_dispatch(x.double(), plan), lambda: expert_dispatch(x.int(), plan), lambda: expert_combine(y.double(), plan),
+              lambda: expert_combine(y, plan, w.double()), lambda: expert_dispatch(None, plan)):
+        with pytest.raises(TypeError):
+            f()
+    if device != "cpu":
+        for f in (lambda: expert_sort(ids.cpu(), 4), lambda: expert_dispatch(x.cpu(), plan), lambda: expert_combine(y, plan, w.cpu())):
+            with pytest.raises(ValueError):
+                f()
+    # differentiable once
+    a = x.clone().requires_grad_(True)
+    out = expert_dispatch(a, plan)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(out.sum(), a, create_graph=True)
+    b = y.clone().requires_grad_(True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(expert_combine(b, plan, w).sum(), b, create_graph=True)
+    # what the backward pass reads must not have changed
+    v = w.clone().requires_grad_(True)
+    out = expert_combine(y, plan, v * 1)
+    y.add_(1)
+    with pytest.raises(RuntimeError):
+        out.sum().backward()
+
+
+def check_routing_views(device):
+    """Gradients that are broadcast, tokens that are, no weights, a plan used again, rows of another layout."""
+    from mneslam_amd.routing import expert_combine, expert_dispatch, expert_sort
+    ids = torch.tensor([[2, 2], [0, -1], [1, 2], [-1, -1]], device=device)
+    plan = expert_sort(ids.t().contiguous().t(), 3)
+    one = torch.arange(1.0, 4.0, device=device, requires_grad=True)
+    x = one.expand(4, 3)
+    rows = expert_dispatch(x, plan)
+    live = int(plan.live)
+    assert live == 5 and torch.equal(rows[:live], one.detach().expand(5, 3)) and not rows[live:].any()
+    rows.sum().backward()                                   # the gradient of a sum is one number broadcast over all rows
+    assert torch.equal(one.grad, torch.full((3,), 5.0, device=device))
+    y = torch.arange(8.0 * 3, device=device).view(3, 8).t().requires_grad_(True)          # columns next to each other
+    out = expert_combine(y, plan)
+    out.sum().backward()
+    want = torch.zeros(4, 3, device=device)
+    for t in range(4):
+        for j in range(2):
+            if ids[t, j] >= 0:
+                want[t] += y.detach()[int(plan.position[t, j])]
+    assert torch.equal(out, want)
+    assert torch.equal(y.grad, (torch.arange(8, device=device) < live).float()[:, None].expand(8, 3))
+    # a value of its own for each token and choice, against differences (the outputs are linear in each: any step is exact up to rounding)
+    w = torch.rand(4, 2, device=device, requires_grad=True)
+    yd = torch.rand(8, 3, device=device)
+    probe = torch.rand(4, 3, device=device)
+    (expert_combine(yd, plan, w) * probe).sum().backward()
+    for t in range(4):
+        for j in range(2):
+            up = w.detach().clone()
+            up[t, j] += 1.0
+            diff = ((expert_combine(yd, plan, up) - expert_combine(yd, plan, w.detach())).double() * probe.double()).sum()
+            assert abs(float(diff) - float(w.grad[t, j])) <= 64 * EPS32
+    empty = expert_sort(torch.zeros(0, 2, dtype=torch.int64, device=device), 3)
+    assert empty.offsets.tolist() == [0, 0, 0, 0] and expert_dispatch(torch.zeros(0, 5, device=device), empty).shape == (0, 5)
+    assert expert_combine(torch.zeros(0, 5, device=device), empty).shape == (0, 5)

@@ -71,3 +71,52 @@ def test_expert_rows_needed_gradients(dtype, wtype, need):
 @pytest.mark.parametrize("kind", ["hot", "none", "outside"])
 def test_expert_rows_batches(kind):
     oc.check_expert_rows(DEV, "bf16", 130, 2, 7, 40, 24, kind, odd=False)
+
+
+def test_agent_maps(tmp_path):
+    oc.check_agent_maps(DEV, tmp_path)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("ptype", ["f32", "bf16"])
+def test_mixture_step(bits, ptype):
+    oc.check_mixture_step(DEV, bits, ptype)
+
+
+def test_adamw_refusals():
+    oc.check_adamw_refusals(DEV)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_adamw_nonfinite(bits):
+    oc.check_adamw_nonfinite(DEV, bits)
+
+
+def test_adamw_8_small_and_zero():
+    oc.check_adamw8_small_and_zero(DEV)
+
+
+def test_adamw_8_dither():
+    oc.check_adamw8_dither(DEV)
+
+
+def test_fused_adamw():
+    oc.check_fused_adamw(DEV)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_adamw_many_tensors(bits):
+    oc.check_adamw_many(DEV, 170, bits)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_adamw_clock(bits):
+    oc.check_adamw_clock(DEV, bits)
+
+
+def test_routing_refusals():
+    oc.check_routing_refusals(DEV)
+
+
+def test_routing_views():
+    oc.check_routing_views(DEV)
