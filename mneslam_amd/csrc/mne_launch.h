@@ -358,7 +358,7 @@ struct ExpertRowArgs {
     const float* weights;          // [n][k] or NULL
     float* dw;                     // [n][k] or NULL
     long long a_stride, b_stride;  // bytes between rows
-    int n, k, width, cols, tiles;  // cols: 16-byte pieces and single elements of a row
+    int n, k, width, cols, tiles;  // cols: pieces of a row that a lane takes
 };
 long long mne_expert_workspace_ints(long long m, int experts);
 int mne_launch_expert_sort(ExpertSortArgs a, void* workspace, hipStream_t st);

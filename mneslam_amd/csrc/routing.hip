@@ -195,65 +195,71 @@ int mne_launch_expert_sort(ExpertSortArgs a, void* workspace, hipStream_t st) {
 }
 
 // ---- rows ------------------------------------------------------------------------------------------------------------
-// A row is cut into 16-byte pieces and, behind them, single elements; column c of a row is piece c or element c - pieces.  The pieces
-// are loaded and stored whole whatever the row's alignment is (element by element, odd widths would take eight times the instructions).
-typedef unsigned ex_words __attribute__((ext_vector_type(4)));
-typedef unsigned ex_words_in_memory __attribute__((ext_vector_type(4), aligned(2)));
-template <int T, int PAST> struct ExCol {
-    typedef typename MneElem<T>::mem mem;
-    static constexpr int N = 16 / (int)sizeof(mem);
-    ex_words v;
-    __device__ __forceinline__ void clear() { v = (ex_words)(0u); }
-    __device__ __forceinline__ void load(const void* row, int c, int width) {
-        const int pieces = width / N;
-        if (c < pieces) {
-            if (PAST == 2) v = __builtin_nontemporal_load(&((const ex_words_in_memory*)row)[c]);
-            else v = ((const ex_words_in_memory*)row)[c];
-        }
-        else {
-            const mem* q = (const mem*)row + pieces * N + (c - pieces);
-            clear();
-            v.x = sizeof(mem) == 2 ? (unsigned)*(const unsigned short*)q : *(const unsigned*)q;
-        }
+// A row is cut into columns of P bytes: 16, or where it has fewer the largest power of two it has.  The last column ends where the row
+// ends, over a part of the one before it if it must: what two lanes read and write there is the same.  Columns are loaded and stored
+// whole whatever their alignment (global memory takes them in one piece; element by element, odd widths would take eight times the
+// instructions).  PAST: see ex_past.
+typedef unsigned ex_words4 __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned ex_words2 __attribute__((ext_vector_type(2), aligned(2)));
+typedef unsigned ex_words1 __attribute__((aligned(2)));
+template <int P> struct ExWords;
+template <> struct ExWords<16> { typedef ex_words4 mem; typedef unsigned reg __attribute__((ext_vector_type(4))); };
+template <> struct ExWords<8> { typedef ex_words2 mem; typedef unsigned reg __attribute__((ext_vector_type(2))); };
+template <> struct ExWords<4> { typedef ex_words1 mem; typedef unsigned reg; };
+template <> struct ExWords<2> { typedef unsigned short mem; typedef unsigned short reg; };
+
+template <int T, int P, int PAST> struct ExCol {
+    typedef typename MneElem<T>::mem elem;
+    typedef typename MneWord<sizeof(elem)>::type word;
+    typedef typename ExWords<P>::mem mem;
+    static constexpr int N = P / (int)sizeof(elem);
+    typename ExWords<P>::reg v;
+    static __device__ __forceinline__ int start(int c, int width) { return c * N < width - N ? c * N : width - N; }
+    __device__ __forceinline__ void clear() { v = (typename ExWords<P>::reg)(0u); }
+    __device__ __forceinline__ void load(const char* row, int c, int width) {
+        const mem* p = (const mem*)((const elem*)row + start(c, width));
+        if (PAST == 2) v = __builtin_nontemporal_load(p);
+        else v = *p;
     }
-    __device__ __forceinline__ void store(void* row, int c, int width) const {
-        const int pieces = width / N;
-        if (c < pieces) {
-            if (PAST) __builtin_nontemporal_store(v, &((ex_words_in_memory*)row)[c]);
-            else ((ex_words_in_memory*)row)[c] = v;
-        }
-        else {
-            mem* q = (mem*)row + pieces * N + (c - pieces);
-            if (sizeof(mem) == 2) *(unsigned short*)q = (unsigned short)v.x;
-            else *(unsigned*)q = v.x;
-        }
+    __device__ __forceinline__ void store(char* row, int c, int width) const {
+        mem* p = (mem*)((elem*)row + start(c, width));
+        if (PAST) __builtin_nontemporal_store(v, p);
+        else *p = v;
+    }
+    __device__ __forceinline__ unsigned at(int i) const {            // 32 bits of it
+        if constexpr (P >= 8) return v[i];
+        else return v;
     }
     __device__ __forceinline__ float get(int j) const {
-        if (sizeof(mem) == 4) return __uint_as_float(v[j]);
-        return MneElem<T>::get(__builtin_bit_cast(mem, (typename MneWord<sizeof(mem)>::type)(v[j >> 1] >> (j & 1 ? 16 : 0))));
+        if constexpr (sizeof(elem) == 4) return __uint_as_float(at(j));
+        else return MneElem<T>::get(__builtin_bit_cast(elem, (word)(at(j >> 1) >> (j & 1 ? 16 : 0))));
     }
     __device__ __forceinline__ void put(const float* x) {
+        if constexpr (P == 2) v = __builtin_bit_cast(word, MneElem<T>::put(x[0]));
+        else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (sizeof(mem) == 4) v[j] = __float_as_uint(x[j]);
-            else {
-                typedef typename MneWord<sizeof(mem)>::type word;
-                v[j] = (unsigned)__builtin_bit_cast(word, MneElem<T>::put(x[N / 4 * j])) | (unsigned)__builtin_bit_cast(word, MneElem<T>::put(x[N / 4 * j + N / 4 - 1])) << 16;
+            for (int i = 0; i < P / 4; ++i) {
+                unsigned u;
+                if constexpr (sizeof(elem) == 4) u = __float_as_uint(x[i]);
+                else u = (unsigned)__builtin_bit_cast(word, MneElem<T>::put(x[2 * i])) | (unsigned)__builtin_bit_cast(word, MneElem<T>::put(x[2 * i + 1])) << 16;
+                if constexpr (P >= 8) v[i] = u;
+                else v = u;
             }
         }
     }
 };
 
 // GROUP lanes have a token and a tile of GROUP * U columns.
-template <int T, int U, int PAST>
+template <int T, int P, int U, int PAST>
 __global__ __launch_bounds__(EX_THREADS) void expert_dispatch_kernel(ExpertRowArgs a, int group) {
+    typedef ExCol<T, P, PAST> Col;
     const long long unit = ((long long)blockIdx.x * EX_THREADS + threadIdx.x) / group;
     const int l = threadIdx.x & (group - 1);
     if (unit >= (long long)a.n * a.tiles) return;
     const int n = (int)(unit / a.tiles), c0 = (int)(unit % a.tiles) * group * U + l;
-    const long long size = (long long)a.width * sizeof(typename MneElem<T>::mem), slot = (long long)n * a.k;
+    const long long size = (long long)a.width * sizeof(typename Col::elem), slot = (long long)n * a.k;
     const int total = *a.total;
-    ExCol<T, PAST> x[U];
+    Col x[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
         if (c0 + u * group < a.cols) x[u].load((const char*)a.a + n * a.a_stride, c0 + u * group, a.width);
@@ -265,7 +271,7 @@ __global__ __launch_bounds__(EX_THREADS) void expert_dispatch_kernel(ExpertRowAr
                 if (c0 + u * group < a.cols) x[u].store((char*)a.out + row * size, c0 + u * group, a.width);
         }
         if (slot + k >= total) {                    // a row behind the live ones: zero
-            ExCol<T, PAST> zero;
+            Col zero;
             zero.clear();
 #pragma unroll
             for (int u = 0; u < U; ++u)
@@ -274,14 +280,14 @@ __global__ __launch_bounds__(EX_THREADS) void expert_dispatch_kernel(ExpertRowAr
     }
 }
 
-template <int T, int U, int PAST>
+template <int T, int P, int U, int PAST>
 __global__ __launch_bounds__(EX_THREADS) void expert_combine_kernel(ExpertRowArgs a, int group) {
-    typedef ExCol<T, PAST> Col;
+    typedef ExCol<T, P, PAST> Col;
     const long long unit = ((long long)blockIdx.x * EX_THREADS + threadIdx.x) / group;
     const int l = threadIdx.x & (group - 1);
     if (unit >= (long long)a.n * a.tiles) return;
     const int n = (int)(unit / a.tiles), c0 = (int)(unit % a.tiles) * group * U + l;
-    const long long size = (long long)a.width * sizeof(typename Col::mem), slot = (long long)n * a.k;
+    const long long size = (long long)a.width * sizeof(typename Col::elem), slot = (long long)n * a.k;
     float acc[U][Col::N] = {};
     for (int k = 0; k < a.k; k += 2) {              // two rows in flight
         int row[2];
@@ -319,13 +325,13 @@ __global__ __launch_bounds__(EX_THREADS) void expert_combine_kernel(ExpertRowArg
 }
 
 // GROUP lanes have a token: its row of dout against its rows of y, K slots and U columns of a lane at a time.
-template <int T, int K, int U, int PAST>
+template <int T, int P, int K, int U, int PAST>
 __global__ __launch_bounds__(EX_THREADS) void expert_combine_backward_kernel(ExpertRowArgs a, int group) {
-    typedef ExCol<T, PAST> Col;
+    typedef ExCol<T, P, PAST> Col;
     const long long n = ((long long)blockIdx.x * EX_THREADS + threadIdx.x) / group;
     const int l = threadIdx.x & (group - 1);
     const bool there = n < a.n;                     // (all lanes stay: they add up the dot products together)
-    const long long size = (long long)a.width * sizeof(typename Col::mem), slot = n * a.k;
+    const long long size = (long long)a.width * sizeof(typename Col::elem), slot = n * a.k;
     const int total = *a.total;
     for (int k0 = 0; k0 < a.k; k0 += K) {
         int row[K];
@@ -354,14 +360,15 @@ __global__ __launch_bounds__(EX_THREADS) void expert_combine_backward_kernel(Exp
                             if (row[i] >= 0 && c0 + u * group < a.cols) y[i][u].load((const char*)a.b + row[i] * a.b_stride, c0 + u * group, a.width);
                         }
 #pragma unroll
-                    for (int i = 0; i < K; ++i)
+                    for (int u = 0; u < U; ++u) {
+                        const int c = c0 + u * group, twice = c * Col::N - Col::start(c, a.width);     // elements that the column before has
 #pragma unroll
-                        for (int u = 0; u < U; ++u) {
-                            const int live = c0 + u * group < a.width / Col::N ? Col::N : 1;     // (what is not there is zero on both sides)
+                        for (int j = 0; j < Col::N; ++j) {
+                            const float x = j >= twice ? d[u].get(j) : 0.0f;
 #pragma unroll
-                            for (int j = 0; j < Col::N; ++j)
-                                if (j < live) dot[i] = fmaf(d[u].get(j), y[i][u].get(j), dot[i]);
+                            for (int i = 0; i < K; ++i) dot[i] = fmaf(x, y[i][u].get(j), dot[i]);
                         }
+                    }
                 }
                 if (a.out) {
 #pragma unroll
@@ -395,18 +402,26 @@ __global__ __launch_bounds__(EX_THREADS) void expert_combine_backward_kernel(Exp
     }
 }
 
-// Lanes of a token (a power of two, at most a wave) and columns of a lane, 1 to `most`: of the forms that leave the fewest lanes without
-// a column the one with most columns a lane (more loads in flight).  Where that leaves the machine without waves, one column a lane.
+static long long ex_row_bytes(const ExpertRowArgs& a, int type) { return (long long)a.width * (type == MNE_T_F32 ? 4 : 2); }
+static int ex_piece(const ExpertRowArgs& a, int type) {
+    const long long size = ex_row_bytes(a, type);
+    return size >= 16 ? 16 : size >= 8 ? 8 : size >= 4 ? 4 : 2;
+}
+
+// Lanes of a token (a power of two, at most a wave, no fewer than make a 128-byte line where there are as many columns) and columns of
+// a lane (1 to `most`): of the forms that leave the fewest lanes without a column the one with most columns a lane, whose loads are in
+// flight together.  Where that leaves the machine without waves, one column a lane.
 struct ExForm { int group, u; };
 static ExForm ex_form(ExpertRowArgs& a, int type, int most) {
-    const int per = type == MNE_T_F32 ? 4 : 8;
-    a.cols = a.width / per + a.width % per;
-    ExForm best = {1, 1};
+    const int piece = ex_piece(a, type);
+    a.cols = (int)((ex_row_bytes(a, type) + piece - 1) / piece);
+    if ((long long)a.n * a.cols < 1 << 17 || piece < 16) most = 1;
+    ExForm best = {64, most};
     long long least = 1ll << 62;
-    if ((long long)a.n * a.cols < 1 << 17) most = 1;
     for (int u = 1; u <= most; ++u) {
         int group = 1;
         while (group < 64 && group * u < a.cols) group <<= 1;
+        if (group < 8 && u > 1) continue;
         const long long used = ((long long)a.cols + group * u - 1) / (group * u) * (group * u);
         if (used <= least) { least = used; best = {group, u}; }
     }
@@ -419,61 +434,87 @@ static unsigned ex_grid(long long units, int group) {
     return blocks * EX_THREADS <= 0xFFFFFFFFll ? (unsigned)blocks : 0u;
 }
 
-template <int T, int PAST> static int ex_dispatch(ExpertRowArgs a, hipStream_t st) {
-    const ExForm f = ex_form(a, T, 4);
-    const unsigned grid = ex_grid((long long)a.n * a.tiles, f.group);
-    if (!grid) return -1;
-    if (f.u == 4) MNE_LAUNCH((expert_dispatch_kernel<T, 4, PAST>), grid, EX_THREADS, 0, st, a, f.group);
-    else if (f.u == 3) MNE_LAUNCH((expert_dispatch_kernel<T, 3, PAST>), grid, EX_THREADS, 0, st, a, f.group);
-    else if (f.u == 2) MNE_LAUNCH((expert_dispatch_kernel<T, 2, PAST>), grid, EX_THREADS, 0, st, a, f.group);
-    else MNE_LAUNCH((expert_dispatch_kernel<T, 1, PAST>), grid, EX_THREADS, 0, st, a, f.group);
-    return 0;
-}
-template <int T, int PAST> static int ex_combine(ExpertRowArgs a, hipStream_t st) {
-    const ExForm f = ex_form(a, T, 4);
-    const unsigned grid = ex_grid((long long)a.n * a.tiles, f.group);
-    if (!grid) return -1;
-    if (f.u == 4) MNE_LAUNCH((expert_combine_kernel<T, 4, PAST>), grid, EX_THREADS, 0, st, a, f.group);
-    else if (f.u == 3) MNE_LAUNCH((expert_combine_kernel<T, 3, PAST>), grid, EX_THREADS, 0, st, a, f.group);
-    else if (f.u == 2) MNE_LAUNCH((expert_combine_kernel<T, 2, PAST>), grid, EX_THREADS, 0, st, a, f.group);
-    else MNE_LAUNCH((expert_combine_kernel<T, 1, PAST>), grid, EX_THREADS, 0, st, a, f.group);
-    return 0;
-}
-template <int T, int PAST> static int ex_backward(ExpertRowArgs a, hipStream_t st) {
-    const ExForm f = ex_form(a, T, 4);
-    const unsigned grid = ex_grid(a.n, f.group);
-    if (!grid) return -1;
-    if (a.k == 1) MNE_LAUNCH((expert_combine_backward_kernel<T, 1, 4, PAST>), grid, EX_THREADS, 0, st, a, f.group);
-    else if (a.k == 2) MNE_LAUNCH((expert_combine_backward_kernel<T, 2, 2, PAST>), grid, EX_THREADS, 0, st, a, f.group);
-    else MNE_LAUNCH((expert_combine_backward_kernel<T, 4, 1, PAST>), grid, EX_THREADS, 0, st, a, f.group);
-    return 0;
-}
-
 // What goes past the caches (PAST): 0 nothing, 1 what is written, 2 what is read as well.
 // Written: rows of whole 128-byte lines only -- 32768 rows of 2 KB combined 16 us instead of 30, dealt out 17 instead of 22; with rows of
 // 260 bytes, whose lines are written by two, 61 us instead of 36.  Dealt-out rows up to 1 GB (2.1 GB: 500 us instead of 475).
+// (Combined rows lie one after the other, and still: rows of 64 bytes 69 us and 67 without, of 32 bytes 98 and 78.)
 // Read: combined rows of 128 MB and more in all, half of what the last cache holds: 128 MB 31 us instead of 33, 2.1 GB 429 instead of 464;
 // with 64 MB 17 us instead of 15.  (Its backward pass: 0 to 3 % either way, left alone.)
-static bool ex_whole_lines(const ExpertRowArgs& a, int type) {
-    return (long long)a.width * (type == MNE_T_F32 ? 4 : 2) % 128 == 0 && (uintptr_t)a.out % 128 == 0;
+static bool ex_whole_lines(const ExpertRowArgs& a, int type) { return ex_row_bytes(a, type) % 128 == 0 && (uintptr_t)a.out % 128 == 0; }
+static long long ex_bytes(const ExpertRowArgs& a, int type) { return (long long)a.n * a.k * ex_row_bytes(a, type); }
+
+template <int T, int P, int PAST> static int ex_dispatch(ExpertRowArgs a, hipStream_t st) {
+    const ExForm f = ex_form(a, T, 4);
+    const unsigned grid = ex_grid((long long)a.n * a.tiles, f.group);
+    if (!grid) return -1;
+    if constexpr (P == 16) {
+        if (f.u == 4) { MNE_LAUNCH((expert_dispatch_kernel<T, P, 4, PAST>), grid, EX_THREADS, 0, st, a, f.group); return 0; }
+        if (f.u == 3) { MNE_LAUNCH((expert_dispatch_kernel<T, P, 3, PAST>), grid, EX_THREADS, 0, st, a, f.group); return 0; }
+        if (f.u == 2) { MNE_LAUNCH((expert_dispatch_kernel<T, P, 2, PAST>), grid, EX_THREADS, 0, st, a, f.group); return 0; }
+    }
+    MNE_LAUNCH((expert_dispatch_kernel<T, P, 1, PAST>), grid, EX_THREADS, 0, st, a, f.group);
+    return 0;
 }
-static long long ex_bytes(const ExpertRowArgs& a, int type) { return (long long)a.n * a.k * a.width * (type == MNE_T_F32 ? 4 : 2); }
+template <int T, int P, int PAST> static int ex_combine(ExpertRowArgs a, hipStream_t st) {
+    const ExForm f = ex_form(a, T, 4);
+    const unsigned grid = ex_grid((long long)a.n * a.tiles, f.group);
+    if (!grid) return -1;
+    if constexpr (P == 16) {
+        if (f.u == 4) { MNE_LAUNCH((expert_combine_kernel<T, P, 4, PAST>), grid, EX_THREADS, 0, st, a, f.group); return 0; }
+        if (f.u == 3) { MNE_LAUNCH((expert_combine_kernel<T, P, 3, PAST>), grid, EX_THREADS, 0, st, a, f.group); return 0; }
+        if (f.u == 2) { MNE_LAUNCH((expert_combine_kernel<T, P, 2, PAST>), grid, EX_THREADS, 0, st, a, f.group); return 0; }
+    }
+    MNE_LAUNCH((expert_combine_kernel<T, P, 1, PAST>), grid, EX_THREADS, 0, st, a, f.group);
+    return 0;
+}
+// (four rows at a time from three choices on)
+template <int T, int P, int PAST, int K, int MOST> static int ex_backward(ExpertRowArgs a, hipStream_t st) {
+    const ExForm f = ex_form(a, T, MOST);
+    const unsigned grid = ex_grid(a.n, f.group);
+    if (!grid) return -1;
+    if constexpr (P == 16) {
+        if constexpr (MOST >= 4) if (f.u == 4) { MNE_LAUNCH((expert_combine_backward_kernel<T, P, K, 4, PAST>), grid, EX_THREADS, 0, st, a, f.group); return 0; }
+        if constexpr (MOST >= 3) if (f.u == 3) { MNE_LAUNCH((expert_combine_backward_kernel<T, P, K, 3, PAST>), grid, EX_THREADS, 0, st, a, f.group); return 0; }
+        if (f.u == 2) { MNE_LAUNCH((expert_combine_backward_kernel<T, P, K, 2, PAST>), grid, EX_THREADS, 0, st, a, f.group); return 0; }
+    }
+    MNE_LAUNCH((expert_combine_backward_kernel<T, P, K, 1, PAST>), grid, EX_THREADS, 0, st, a, f.group);
+    return 0;
+}
+template <int T, int P, int PAST> static int ex_backward_by_k(const ExpertRowArgs& a, hipStream_t st) {
+    return a.k == 1 ? ex_backward<T, P, PAST, 1, 4>(a, st) : a.k == 2 ? ex_backward<T, P, PAST, 2, 3>(a, st) : ex_backward<T, P, PAST, 4, 2>(a, st);
+}
+
+// F<T, P, PAST>::go by the row's piece; rows shorter than 16 bytes never go past the caches
+template <template <int, int, int> class F, int T> static int ex_by_piece(const ExpertRowArgs& a, int past, hipStream_t st) {
+    switch (ex_piece(a, T)) {
+        case 16: return past == 2 ? F<T, 16, 2>::go(a, st) : past == 1 ? F<T, 16, 1>::go(a, st) : F<T, 16, 0>::go(a, st);
+        case 8: return F<T, 8, 0>::go(a, st);
+        case 4: return F<T, 4, 0>::go(a, st);
+        default:
+            if constexpr (T != MNE_T_F32) return F<T, 2, 0>::go(a, st);
+            else return -1;
+    }
+}
+template <int T, int P, int PAST> struct ExDispatch {
+    static int go(const ExpertRowArgs& a, hipStream_t st) { return ex_dispatch<T, P, PAST == 2 ? 1 : PAST>(a, st); }
+};
+template <int T, int P, int PAST> struct ExCombine {
+    static int go(const ExpertRowArgs& a, hipStream_t st) { return ex_combine<T, P, PAST>(a, st); }
+};
+template <int T, int P, int PAST> struct ExBackward {
+    static int go(const ExpertRowArgs& a, hipStream_t st) { return ex_backward_by_k<T, P, PAST == 2 ? 1 : PAST>(a, st); }
+};
+template <template <int, int, int> class F> static int ex_by_type(const ExpertRowArgs& a, int type, int past, hipStream_t st) {
+    return type == MNE_T_F32 ? ex_by_piece<F, MNE_T_F32>(a, past, st) : type == MNE_T_BF16 ? ex_by_piece<F, MNE_T_BF16>(a, past, st) : ex_by_piece<F, MNE_T_F16>(a, past, st);
+}
 
 int mne_launch_expert_dispatch(ExpertRowArgs a, int type, hipStream_t st) {
-    const bool past = ex_whole_lines(a, type) && ex_bytes(a, type) <= 1ll << 30;
-    if (type == MNE_T_F32) return past ? ex_dispatch<MNE_T_F32, 1>(a, st) : ex_dispatch<MNE_T_F32, 0>(a, st);
-    return past ? ex_dispatch<MNE_T_F16, 1>(a, st) : ex_dispatch<MNE_T_F16, 0>(a, st);       // (rows are copied: any 16-bit type)
-}
-template <int T> static int ex_combine_by(const ExpertRowArgs& a, hipStream_t st) {
-    if (!ex_whole_lines(a, T)) return ex_combine<T, 0>(a, st);
-    return ex_bytes(a, T) < 1ll << 27 ? ex_combine<T, 1>(a, st) : ex_combine<T, 2>(a, st);
+    const int past = ex_whole_lines(a, type) && ex_bytes(a, type) <= 1ll << 30;
+    return type == MNE_T_F32 ? ex_by_piece<ExDispatch, MNE_T_F32>(a, past, st) : ex_by_piece<ExDispatch, MNE_T_F16>(a, past, st);   // (rows are copied: any 16-bit type)
 }
 int mne_launch_expert_combine(ExpertRowArgs a, int type, hipStream_t st) {
-    return type == MNE_T_F32 ? ex_combine_by<MNE_T_F32>(a, st) : type == MNE_T_BF16 ? ex_combine_by<MNE_T_BF16>(a, st) : ex_combine_by<MNE_T_F16>(a, st);
-}
-template <int T> static int ex_backward_by(const ExpertRowArgs& a, hipStream_t st) {
-    return ex_whole_lines(a, T) ? ex_backward<T, 1>(a, st) : ex_backward<T, 0>(a, st);
+    return ex_by_type<ExCombine>(a, type, !ex_whole_lines(a, type) ? 0 : ex_bytes(a, type) < 1ll << 27 ? 1 : 2, st);
 }
 int mne_launch_expert_combine_backward(ExpertRowArgs a, int type, hipStream_t st) {
-    return type == MNE_T_F32 ? ex_backward_by<MNE_T_F32>(a, st) : type == MNE_T_BF16 ? ex_backward_by<MNE_T_BF16>(a, st) : ex_backward_by<MNE_T_F16>(a, st);
+    return ex_by_type<ExBackward>(a, type, ex_whole_lines(a, type), st);
 }
