@@ -14,11 +14,18 @@
 #define EX_THREADS 256
 #define EX_WAVES (EX_THREADS / 64)
 #define EX_CHUNKS 512                               // workgroups of the long form at most
-#define EX_SHORT 16384                              // slots up to which one workgroup of 1024 does it all
+#define EX_SHORT 4096                               // slots up to which one workgroup of 1024 does it all
 #define EX_SHORT_EXPERTS 2000                       // its counters of 16 waves fit the LDS
+#define EX_SUMS_MOST 16384                          // counters that every workgroup may add up itself
 #define EX_AHEAD 8                                  // ids that a lane loads before it looks at the first
 
 // ---- sort ------------------------------------------------------------------------------------------------------------
+// Bound by launches and round trips to memory, not by bytes.  Three forms (us, 8 / 129 / 1000 experts, one choice each):
+//   slots                                     512                4096               32768              524288
+//   one workgroup                             4.0 / 4.4 / 5.7    6.8 / 7.7 / 9.4    (16384: 16.9 / 20.5 / 23.5)
+//   count, place with the sums in it          6.8 / 7.2 / -      6.9 / 8.1 / -      7.2 / 15.6* / -    12.3 / - / -
+//   count, scan, place                        10.6 / 11.1 / 13.5 10.8 / 11.5 / 14.2 11.1 / 12.0 / 14.4 15.1 / 17.1 / 22.2
+// so: one workgroup up to 4096 slots, else sums in place up to 16384 counters (* : beyond them), else a scan of its own.
 __device__ __forceinline__ int ex_id(const ExpertSortArgs& a, int slot) {        // what names no expert sorts behind all of them
     const long long e = a.wide ? ((const long long*)a.ids)[slot] : ((const int*)a.ids)[slot];
     return e >= 0 && e < a.experts ? (int)e : a.experts;
@@ -82,12 +89,16 @@ __global__ __launch_bounds__(1024) void expert_scan_kernel(ExpertSortArgs a) {
     if (e <= a.experts && w == 0) a.total[e] = all;
 }
 
-// Rows of a workgroup's slots: WAVES waves of a.per_wave consecutive slots.  ALONE: one workgroup has all slots.
-template <int WAVES, bool ALONE>
+// Rows of a workgroup's slots: WAVES waves of a.per_wave consecutive slots.  How many slots of an expert there are in all, and in the
+// workgroups before: EX_ALONE, there is one workgroup; EX_SCANNED, expert_scan_kernel has added them up; EX_SUMS, every workgroup adds
+// all counters up itself, which is less than another launch as long as they are few.
+enum { EX_ALONE, EX_SCANNED, EX_SUMS };
+template <int WAVES, int HOW>
 __global__ __launch_bounds__(WAVES * 64) void expert_place_kernel(ExpertSortArgs a) {
+    constexpr bool ALONE = HOW == EX_ALONE;
     MNE_DYN_LDS(lds);
     int* cnt = (int*)lds;                           // [WAVES][experts + 1]: counters, then next rows
-    __shared__ int part[WAVES];
+    __shared__ int part[WAVES], sums[HOW == EX_SUMS ? 2 * EX_THREADS : 1];
     const int bins = a.experts + 1, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     int* mine = cnt + w * bins;
     for (int e = threadIdx.x; e < WAVES * bins; e += WAVES * 64) cnt[e] = 0;
@@ -95,6 +106,34 @@ __global__ __launch_bounds__(WAVES * 64) void expert_place_kernel(ExpertSortArgs
     const long long first = ((long long)blockIdx.x * WAVES + w) * a.per_wave;
     const long long last = first + a.per_wave < a.m ? first + a.per_wave : a.m;
     ex_count(a, first, last, mine);
+    if (HOW == EX_SUMS) {                           // `lane` e of every `span` has expert e, the spans share the chunks
+        int span = 1;
+        while (span < bins) span <<= 1;
+        const int e = threadIdx.x & (span - 1), at = threadIdx.x / span, step = EX_THREADS / span;
+        int before = 0, all = 0;
+        if (e < bins)
+            for (int c0 = at; c0 < a.chunks; c0 += 8 * step) {
+                int x[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = c0 + i * step < a.chunks ? a.count[(long long)(c0 + i * step) * bins + e] : 0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    all += x[i];
+                    before += c0 + i * step < (int)blockIdx.x ? x[i] : 0;
+                }
+            }
+        sums[2 * threadIdx.x] = before;
+        sums[2 * threadIdx.x + 1] = all;
+        __syncthreads();
+        before = all = 0;
+        if ((int)threadIdx.x < bins)
+            for (int i = 0; i < step; ++i) {
+                before += sums[2 * (i * span + threadIdx.x)];
+                all += sums[2 * (i * span + threadIdx.x) + 1];
+            }
+        __syncthreads();
+        if ((int)threadIdx.x < bins) { sums[2 * threadIdx.x] = before; sums[2 * threadIdx.x + 1] = all; }
+    }
     __syncthreads();
     // first row of every expert: a thread has a run of them, the threads' sums are scanned
     const int each = (bins + WAVES * 64 - 1) / (WAVES * 64), lo = threadIdx.x * each, hi = lo + each < bins ? lo + each : bins;
@@ -102,7 +141,7 @@ __global__ __launch_bounds__(WAVES * 64) void expert_place_kernel(ExpertSortArgs
     for (int e = lo; e < hi; ++e) {
         int t = 0;
         if (ALONE) for (int i = 0; i < WAVES; ++i) t += cnt[i * bins + e];
-        else t = a.total[e];
+        else t = HOW == EX_SUMS ? sums[2 * e + 1] : a.total[e];
         sum += t;
     }
     int scan = sum;
@@ -116,14 +155,14 @@ __global__ __launch_bounds__(WAVES * 64) void expert_place_kernel(ExpertSortArgs
     for (int i = 0; i < w; ++i) row += part[i];
     for (int e = lo; e < hi; ++e) {
         if (blockIdx.x == 0) a.offsets[e] = row;    // (the entry behind the last expert: the number of live rows)
-        int t = 0, next = ALONE ? row : row + a.count[(long long)blockIdx.x * bins + e];
+        int t = 0, next = ALONE ? row : row + (HOW == EX_SUMS ? sums[2 * e] : a.count[(long long)blockIdx.x * bins + e]);
         for (int i = 0; i < WAVES; ++i) {
             const int c = cnt[i * bins + e];
             cnt[i * bins + e] = next;
             next += c;
             t += c;
         }
-        row += ALONE ? t : a.total[e];
+        row += ALONE ? t : HOW == EX_SUMS ? sums[2 * e + 1] : a.total[e];
     }
     __syncthreads();
     int bits = 0;
@@ -167,6 +206,11 @@ static int ex_chunks(long long m, int experts) {
     const long long chunk = (long long)EX_WAVES * ex_per_wave(m, experts);
     return (int)((m + chunk - 1) / chunk);
 }
+static bool ex_sums(long long m, int experts) {
+    int span = 1;
+    while (span < experts + 1) span <<= 1;
+    return span <= EX_THREADS && (long long)ex_chunks(m, experts) * span <= EX_SUMS_MOST;
+}
 static bool ex_short(long long m, int experts) { return m <= EX_SHORT && experts <= EX_SHORT_EXPERTS; }
 
 long long mne_expert_workspace_ints(long long m, int experts) {
@@ -178,8 +222,8 @@ int mne_launch_expert_sort(ExpertSortArgs a, void* workspace, hipStream_t st) {
     if (ex_short(a.m, a.experts)) {
         a.per_wave = (int)(((a.m + 15) / 16 + 63) / 64 * 64);
         const size_t lds = (size_t)16 * bins * sizeof(int);
-        MNE_SET_MAX_LDS((expert_place_kernel<16, true>), lds);
-        MNE_LAUNCH((expert_place_kernel<16, true>), 1, 1024, lds, st, a);
+        MNE_SET_MAX_LDS((expert_place_kernel<16, EX_ALONE>), lds);
+        MNE_LAUNCH((expert_place_kernel<16, EX_ALONE>), 1, 1024, lds, st, a);
         return 0;
     }
     a.chunks = ex_chunks(a.m, a.experts);
@@ -187,10 +231,14 @@ int mne_launch_expert_sort(ExpertSortArgs a, void* workspace, hipStream_t st) {
     a.count = (int*)workspace;
     a.total = a.count + (long long)a.chunks * bins;
     MNE_LAUNCH(expert_count_kernel, a.chunks, EX_THREADS, bins * sizeof(int), st, a);
-    MNE_LAUNCH(expert_scan_kernel, (bins + 63) / 64, 1024, 0, st, a);
     const size_t lds = (size_t)EX_WAVES * bins * sizeof(int);
-    MNE_SET_MAX_LDS((expert_place_kernel<EX_WAVES, false>), lds);
-    MNE_LAUNCH((expert_place_kernel<EX_WAVES, false>), a.chunks, EX_THREADS, lds, st, a);
+    if (ex_sums(a.m, a.experts)) {
+        MNE_LAUNCH((expert_place_kernel<EX_WAVES, EX_SUMS>), a.chunks, EX_THREADS, lds, st, a);
+        return 0;
+    }
+    MNE_LAUNCH(expert_scan_kernel, (bins + 63) / 64, 1024, 0, st, a);
+    MNE_SET_MAX_LDS((expert_place_kernel<EX_WAVES, EX_SCANNED>), lds);
+    MNE_LAUNCH((expert_place_kernel<EX_WAVES, EX_SCANNED>), a.chunks, EX_THREADS, lds, st, a);
     return 0;
 }
 
