@@ -129,11 +129,11 @@ __global__ __launch_bounds__(AW_THREADS) void adamw32_kernel(Adamw32Args a) {
 
 // Code of x in 0..most^2 with the dither k / 65536: floor of the root, or one more if k / 65536 (2 c + 1) < x - c^2.  The floor is exact
 // with a root that is 1 ulp off: it is the floor of the root of floor(x) + 1/2, which is no nearer than 1 / (4 most) to a whole number.
-// The difference is exact too (a multiple of x's last place, no larger than x).
+// The difference is exact too (c^2 is, and it is a multiple of x's last place, no larger than x).
 __device__ __forceinline__ int aw_code(float x, unsigned k) {
     const int c = (int)mne_sqrt_fast(floorf(x) + 0.5f);
     const float f = (float)c;
-    return (float)k * fmaf(f, 2.0f / 65536.0f, 1.0f / 65536.0f) < x - f * f ? c + 1 : c;
+    return (float)k * fmaf(f, 2.0f / 65536.0f, 1.0f / 65536.0f) < fmaf(-f, f, x) ? c + 1 : c;
 }
 
 __device__ __forceinline__ unsigned aw_max(unsigned x) {        // over the lanes of a block
@@ -204,7 +204,7 @@ __device__ __forceinline__ void adamw8_body(const Adamw8Args& a, const AdamwHype
 #pragma unroll
             for (int j = 0; j < N; ++j) {
                 // (a reciprocal is enough here: nothing of the parameter enters the codes)
-                p[k][j] = p[k][j] * h.decay - h.step_size * (m[k][j] * mne_rcp_fast(fmaf(r[k][j], inv, h.eps)));
+                p[k][j] = fmaf(-h.step_size, m[k][j] * mne_rcp_fast(fmaf(r[k][j], inv, h.eps)), p[k][j] * h.decay);
                 g[k][j] = 0.0f;
             }
             aw_store<PT, N, FULL>(p[k], a.p[s], i, n);
