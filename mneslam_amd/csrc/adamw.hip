@@ -130,10 +130,11 @@ __global__ __launch_bounds__(AW_THREADS) void adamw32_kernel(Adamw32Args a) {
 // Code of x in 0..most^2 with the dither k / 65536: floor of the root, or one more if k / 65536 (2 c + 1) < x - c^2.  The floor is exact
 // with a root that is 1 ulp off: it is the floor of the root of floor(x) + 1/2, which is no nearer than 1 / (4 most) to a whole number.
 // The difference is exact too (c^2 is, and it is a multiple of x's last place, no larger than x).
-__device__ __forceinline__ int aw_code(float x, unsigned k) {
+// SOME: what is not zero gets at least 1 (below 1 the step to it is taken whatever the dither is: its weight, 2 c + 1, is held to c).
+template <bool SOME> __device__ __forceinline__ int aw_code(float x, unsigned short k) {
     const int c = (int)mne_sqrt_fast(floorf(x) + 0.5f);
-    const float f = (float)c;
-    return (float)k * fmaf(f, 2.0f / 65536.0f, 1.0f / 65536.0f) < fmaf(-f, f, x) ? c + 1 : c;
+    const float f = (float)c, w = fmaf(f, 2.0f / 65536.0f, 1.0f / 65536.0f);
+    return (float)k * (SOME ? fminf(w, f) : w) < fmaf(-f, f, x) ? c + 1 : c;
 }
 
 __device__ __forceinline__ unsigned aw_max(unsigned x) {        // over the lanes of a block
@@ -264,26 +265,31 @@ __device__ __forceinline__ void adamw8_body(const Adamw8Args& a, const AdamwHype
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         const long long i = i0 + k * (LANES * N);
-        union { MneBytes<N> v; unsigned char c[N]; } mc, rc;
+        unsigned cm[N], cr[N];
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             unsigned u = kb + (unsigned)(k * LANES * N + j) * AW_GOLD;
             u = (u ^ (u >> 16)) * 0x7FEB352Du;
             u ^= u >> 15;
-            int cm = aw_code(fabsf(m[k][j]) * im, u & 0xFFFFu), cr = aw_code(r[k][j] * ir, u >> 16);
-            cm = cm < 127 ? cm : 127;
-            const int least = r[k][j] > 0.0f ? 1 : 0;
-            cr = cr < least ? least : cr < 255 ? cr : 255;
-            mc.c[j] = (unsigned char)(m[k][j] < 0.0f ? -cm : cm);
-            rc.c[j] = (unsigned char)cr;
+            int x = aw_code<false>(fabsf(m[k][j]) * im, (unsigned short)u);
+            x = x < 127 ? x : 127;
+            cm[j] = (unsigned)(m[k][j] < 0.0f ? -x : x);
+            x = aw_code<true>(r[k][j] * ir, (unsigned short)(u >> 16));
+            cr[j] = (unsigned)(x < 255 ? x : 255);
         }
         if (FULL) {
+            union { MneBytes<N> v; unsigned w[N / 4]; } mc, rc;
+#pragma unroll
+            for (int j = 0; j < N / 4; ++j) {
+                mc.w[j] = mne_pack4(cm[4 * j], cm[4 * j + 1], cm[4 * j + 2], cm[4 * j + 3]);
+                rc.w[j] = mne_pack4(cr[4 * j], cr[4 * j + 1], cr[4 * j + 2], cr[4 * j + 3]);
+            }
             *(MneBytes<N>*)((signed char*)a.m[s] + i) = mc.v;
             *(MneBytes<N>*)((unsigned char*)a.v[s] + i) = rc.v;
         } else {
 #pragma unroll
             for (int j = 0; j < N; ++j)
-                if (i + j < n) { ((unsigned char*)a.m[s])[i + j] = mc.c[j]; ((unsigned char*)a.v[s])[i + j] = rc.c[j]; }
+                if (i + j < n) { ((unsigned char*)a.m[s])[i + j] = (unsigned char)cm[j]; ((unsigned char*)a.v[s])[i + j] = (unsigned char)cr[j]; }
         }
     }
     if (l == 0 && there) {

@@ -774,6 +774,7 @@ int mne_adamw_moments(const int8_t* m, const uint8_t* v, const float* scales, in
     if (n < 0 || n > (1ll << 34) - 4096) return fail(-1, "mne_adamw_moments: bad number of elements");
     if (n == 0) return 0;
     if (!m || !v || !scales || !exp_avg || !exp_avg_sq) return fail(-1, "mne_adamw_moments: NULL argument");
+    if ((uintptr_t)scales % 8 || (uintptr_t)exp_avg % 4 || (uintptr_t)exp_avg_sq % 4) return fail(-1, "mne_adamw_moments: misaligned address");
     mne_launch_adamw_moments(m, v, scales, n, exp_avg, exp_avg_sq, (hipStream_t)stream);
     return check_launch("adamw_moments");
 }

@@ -263,8 +263,15 @@ struct CombineNode : torch::autograd::Function<CombineNode> {
     }
 };
 
+void check_plan(const char* what, const at::Tensor& position, const at::Tensor& offsets) {
+    if (position.scalar_type() != at::kInt || offsets.scalar_type() != at::kInt) throw py::type_error(std::string(what) + ": a plan's tensors are int32");
+    if (position.dim() != 2 || position.size(1) < 1 || offsets.dim() != 1 || offsets.size(0) < 2 || !position.is_contiguous() || !offsets.is_contiguous())
+        throw py::value_error(std::string(what) + ": not a plan of expert_sort");
+}
+
 at::Tensor expert_dispatch(const at::Tensor& x, const at::Tensor& position, const at::Tensor& offsets) {
     one_device("expert_dispatch", {&x, &position, &offsets});
+    check_plan("expert_dispatch", position, offsets);
     if (x.dim() != 2 || x.size(0) != position.size(0))
         throw py::value_error("expert_dispatch: x must be [" + std::to_string(position.size(0)) + " tokens, width]");
     rows(x, "expert_dispatch");
@@ -274,6 +281,7 @@ at::Tensor expert_dispatch(const at::Tensor& x, const at::Tensor& position, cons
 at::Tensor expert_combine(const at::Tensor& y, const at::Tensor& position, const at::Tensor& offsets, const c10::optional<at::Tensor>& weights) {
     const at::Tensor w = weights ? *weights : at::Tensor();
     one_device("expert_combine", {&y, &position, &offsets, &w});
+    check_plan("expert_combine", position, offsets);
     if (y.dim() != 2 || y.size(0) != position.numel())
         throw py::value_error("expert_combine: y must be [" + std::to_string(position.numel()) + " rows, width]");
     if (w.defined()) {

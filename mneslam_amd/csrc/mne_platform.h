@@ -12,6 +12,7 @@ static inline unsigned mne_max16(unsigned v) {                    // largest val
     return v;
 }
 static inline float mne_quad(float v, int k) { return __shfl(v, (int)(threadIdx.x & 60u) | k); }      // lane k's of every four lanes
+static inline unsigned mne_pack4(unsigned a, unsigned b, unsigned c, unsigned d) { return (a & 255u) | (b & 255u) << 8 | (c & 255u) << 16 | d << 24; }
 static inline int mne_first_lane(int v) { return __shfl(v, 0); }
 // bf16 <-> fp32, rounded to nearest even
 static inline float mne_bf16_to_float(unsigned short x) { return __uint_as_float((unsigned)x << 16); }
@@ -77,6 +78,10 @@ static __device__ __forceinline__ float mne_quad(float v, int k) {
         case 2: return __int_as_float(__builtin_amdgcn_update_dpp(0, x, 0xAA, 0xF, 0xF, true));
         default: return __int_as_float(__builtin_amdgcn_update_dpp(0, x, 0xFF, 0xF, 0xF, true));
     }
+}
+// the lowest bytes of four words
+static __device__ __forceinline__ unsigned mne_pack4(unsigned a, unsigned b, unsigned c, unsigned d) {
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x0C0C0400u), __builtin_amdgcn_perm(b, a, 0x0C0C0400u), 0x05040100u);
 }
 static __device__ __forceinline__ int mne_first_lane(int v) { return __builtin_amdgcn_readfirstlane(v); }
 static __device__ __forceinline__ unsigned mne_max16(unsigned v) {

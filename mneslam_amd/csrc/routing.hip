@@ -297,6 +297,12 @@ template <int T, int P, int PAST> struct ExCol {
     }
 };
 
+// a slot's row, -1 where it has none (or the plan's entry is none of a plan's)
+__device__ __forceinline__ int ex_row(const ExpertRowArgs& a, long long slot) {
+    const int row = a.position[slot];
+    return (long long)row < (long long)a.n * a.k ? row : -1;
+}
+
 // GROUP lanes have a token and a tile of GROUP * U columns.
 template <int T, int P, int U, int PAST>
 __global__ __launch_bounds__(EX_THREADS) void expert_dispatch_kernel(ExpertRowArgs a, int group) {
@@ -312,7 +318,7 @@ __global__ __launch_bounds__(EX_THREADS) void expert_dispatch_kernel(ExpertRowAr
     for (int u = 0; u < U; ++u)
         if (c0 + u * group < a.cols) x[u].load((const char*)a.a + n * a.a_stride, c0 + u * group, a.width);
     for (int k = 0; k < a.k; ++k) {
-        const int row = a.position[slot + k];
+        const int row = ex_row(a, slot + k);
         if (row >= 0) {
 #pragma unroll
             for (int u = 0; u < U; ++u)
@@ -344,7 +350,7 @@ __global__ __launch_bounds__(EX_THREADS) void expert_combine_kernel(ExpertRowArg
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const bool on = k + i < a.k;
-            row[i] = on ? a.position[slot + k + i] : -1;
+            row[i] = on ? ex_row(a, slot + k + i) : -1;
             w[i] = on && a.weights ? a.weights[slot + k + i] : 1.0f;
         }
 #pragma unroll
@@ -387,7 +393,7 @@ __global__ __launch_bounds__(EX_THREADS) void expert_combine_backward_kernel(Exp
 #pragma unroll
         for (int i = 0; i < K; ++i) {
             const bool on = there && k0 + i < a.k;
-            row[i] = on ? a.position[slot + k0 + i] : -1;
+            row[i] = on ? ex_row(a, slot + k0 + i) : -1;
             w[i] = on && a.weights ? a.weights[slot + k0 + i] : 1.0f;
             dot[i] = 0.0f;
         }

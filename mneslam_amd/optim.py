@@ -258,6 +258,8 @@ class FusedAdamW(torch.optim.Optimizer):
                     self.state[p][key] = int(value)
                 elif key in ("exp_avg", "exp_avg_sq", "scales"):
                     like = value if key == "scales" else p
+                    if not value.is_floating_point() and any(n > 1 and a != b for n, a, b in zip(p.shape, p.stride(), value.stride())):
+                        raise ValueError("8-bit moments of a parameter that was laid out otherwise: its blocks are others")
                     dtype = torch.float32 if value.is_floating_point() else value.dtype
                     self.state[p][key] = torch.empty_like(like, dtype=dtype, device=p.device, requires_grad=False).copy_(value)
 

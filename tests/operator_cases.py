@@ -606,6 +606,11 @@ def check_fused_adamw(device):
     opt_b.step()
     for p, q in zip(ps, other):
         assert torch.equal(p, q) and all(torch.equal(a, b) for a, b in zip(opt.moments(p), opt_b.moments(q)))
+    # ... but not into a parameter whose memory has another order: its blocks would be others
+    other = [torch.nn.Parameter(p.detach().clone().contiguous()) for p in ps]
+    opt_b = optim.FusedAdamW([{"params": other[:1]}, {"params": other[1:]}])
+    with pytest.raises(ValueError):
+        opt_b.load_state_dict(saved)
     for kw in (dict(lr=-1), dict(betas=(0.9, 1.0)), dict(eps=-1), dict(weight_decay=-1), dict(state_bits=4), dict(seed=-1)):
         with pytest.raises(ValueError):
             optim.FusedAdamW(ps, **kw)
@@ -687,6 +692,18 @@ def check_routing_refusals(device):
         for f in (lambda: expert_sort(ids.cpu(), 4), lambda: expert_dispatch(x.cpu(), plan), lambda: expert_combine(y, plan, w.cpu())):
             with pytest.raises(ValueError):
                 f()
+    from mneslam_amd.routing import ExpertPlan
+    wrong = ExpertPlan(plan.order.long(), plan.position.long(), plan.offsets)
+    for f in (lambda: expert_dispatch(x, wrong), lambda: expert_combine(y, wrong)):
+        with pytest.raises(TypeError):
+            f()
+    with pytest.raises(ValueError):
+        expert_dispatch(x, ExpertPlan(plan.order, plan.position.t().contiguous().t(), plan.offsets))
+    # a plan's entry that is no row is none (nothing is read or written outside)
+    broken = ExpertPlan(plan.order, plan.position.clone(), plan.offsets)
+    broken.position[2, 1], broken.position[3, 0] = 12, 2 ** 31 - 1
+    got = expert_combine(y, broken, w)
+    assert torch.equal(got[2:4], torch.ones(2, 5, device=device)) and expert_dispatch(x, broken).shape == (12, 5)
     # differentiable once
     a = x.clone().requires_grad_(True)
     out = expert_dispatch(a, plan)
