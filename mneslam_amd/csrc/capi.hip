@@ -721,12 +721,14 @@ int mne_adamw_step(const int64_t* table, int64_t n_tensors, const mne_adamw_cfg_
     const bool small = cfg->state_bits == 8;
     const int per_wg = mne_adamw_per_wg(cfg->state_bits);
     const int64_t most = 0xFFFFFFFFll / 256;                // workgroups of a launch: its threads are counted in 32 bits
+    long long all = 0;
     const int64_t psize = cfg->p_type == MNE_T_F32 ? 4 : 2, gsize = cfg->g_type == MNE_T_F32 ? 4 : 2;
     for (int64_t i = 0; i < n_tensors; ++i) {               // nothing is launched unless every row is sound
         const int64_t* t = table + 7 * i;
         if (t[5] < 0 || t[5] > most * per_wg) return fail(-1, "mne_adamw_step: bad number of elements");
         if (t[5] && (!t[0] || !t[1] || !t[2] || !t[3] || (small && !t[4]))) return fail(-1, "mne_adamw_step: NULL address");
         if (t[0] % psize || t[1] % gsize || (small ? t[4] % 8 : t[2] % 4 || t[3] % 4)) return fail(-1, "mne_adamw_step: misaligned address");
+        all += t[5];
     }
     AdamwHyper h = {};
     const double bc1 = 1.0 - std::pow(cfg->beta1, (double)cfg->step), bc2 = 1.0 - std::pow(cfg->beta2, (double)cfg->step);
@@ -739,6 +741,7 @@ int mne_adamw_step(const int64_t* table, int64_t n_tensors, const mne_adamw_cfg_
     Clock clk = {};
     if (clock && fill_clock(clock, clk, cfg->beta1, cfg->beta2, true))
         return fail(-1, "mne_adamw_step: clock incomplete or made for other betas");
+    const bool past = mne_adamw_past(all, cfg->p_type, cfg->g_type, cfg->state_bits);
     Adamw32Args a32;
     Adamw8Args a8;
     a32.h = a8.h = h; a32.clk = a8.clk = clk; a32.zero_grad = a8.zero_grad = cfg->zero_grad;
@@ -749,8 +752,8 @@ int mne_adamw_step(const int64_t* table, int64_t n_tensors, const mne_adamw_cfg_
         const long long more = i < n_tensors ? (t[5] + per_wg - 1) / per_wg : 0;
         if (n_seg && (i == n_tensors || n_seg == (small ? MNE_ADAMW8_SEGS : MNE_ADAMW32_SEGS) || blocks + more > most)) {
             a32.n_seg = a8.n_seg = n_seg;
-            if (small) mne_launch_adamw8(a8, cfg->p_type, cfg->g_type, (unsigned)blocks, (hipStream_t)stream);
-            else mne_launch_adamw32(a32, cfg->p_type, cfg->g_type, (unsigned)blocks, (hipStream_t)stream);
+            if (small) mne_launch_adamw8(a8, cfg->p_type, cfg->g_type, (unsigned)blocks, past, (hipStream_t)stream);
+            else mne_launch_adamw32(a32, cfg->p_type, cfg->g_type, (unsigned)blocks, past, (hipStream_t)stream);
             if (check_launch("adamw_step")) return -10;
             n_seg = 0; blocks = 0;
         }

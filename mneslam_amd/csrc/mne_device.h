@@ -121,8 +121,8 @@ __device__ __forceinline__ float quartic_cdf(float t) {
 }
 
 // Two cumulative values at once (bins b, b + 1): the same fp32 operations on the same inputs as quartic_cdf, element by element
-// (-ffp-contract=off: no fused multiply-add either way), written on float2 so that the multiplies and adds issue as
-// v_pk_mul_f32 / v_pk_add_f32 -- two values per VALU instruction.  Round 6: the OneBlob was ~400 scalar VALU instructions per lane
+// (-ffp-contract=off: no fused multiply-add either way), written on float2 (packed multiplies and adds where the build allows them;
+// it does not, see the compiler flags).  Round 6: the OneBlob was ~400 scalar VALU instructions per lane
 // and 32-sample tile (25 cumulative values x 15 operations), a fifth of what a decode wave issues.
 typedef float mne_f2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ mne_f2 quartic_cdf2(mne_f2 t) {

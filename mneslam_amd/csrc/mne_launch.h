@@ -338,9 +338,10 @@ struct Adamw8Args {
 };
 static_assert(sizeof(Adamw32Args) <= 4096 && sizeof(Adamw8Args) <= 4096, "kernel arguments are limited to 4 KB");
 
-int mne_launch_adamw32(const Adamw32Args& a, int p_type, int g_type, unsigned blocks, hipStream_t st);
-int mne_launch_adamw8(const Adamw8Args& a, int p_type, int g_type, unsigned blocks, hipStream_t st);
+int mne_launch_adamw32(const Adamw32Args& a, int p_type, int g_type, unsigned blocks, bool past, hipStream_t st);
+int mne_launch_adamw8(const Adamw8Args& a, int p_type, int g_type, unsigned blocks, bool past, hipStream_t st);
 int mne_launch_adamw_moments(const signed char* mc, const unsigned char* rc, const float* scales, long long n, float* m, float* v, hipStream_t st);
+bool mne_adamw_past(long long elements, int p_type, int g_type, int state_bits);      // whether the call goes past the caches
 int mne_adamw_per_wg(int state_bits);       // elements of a workgroup
 unsigned mne_adamw_key(unsigned seed, unsigned ordinal);
 
