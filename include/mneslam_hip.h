@@ -516,8 +516,8 @@ int mne_adam_step(const mne_adam_seg_t* segs, int n_seg, int zero_grad, const mn
  * p -= lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)      -- torch.optim.AdamW (amsgrad = False, maximize = False),
  * in fp32 whatever p and g are held in; a 16-bit parameter is rounded to nearest even.
  * `table` is a HOST array of n_tensors rows of 7: address of p, of g, of m, of v, of the scales, number of elements, ordinal.
- * Every tensor is one run of n elements in memory; addresses are multiples of the element's size (of 16 bytes: faster), and no
- * two tensors overlap.
+ * Every tensor is one run of n elements in memory; addresses are multiples of the element's size, and no two
+ * tensors overlap.
  * state_bits 32: m, v fp32 [n] (scales and ordinal unused).
  * state_bits 8:  m int8 [n], v uint8 [n], scales fp32 [ceil(n / 256)][2].  Block b = elements 256 b .. 256 b + 255:
  *   m = sign(c) c^2 scales[b][0],  sqrt(v) = c^2 scales[b][1]   (mne_adamw_moments gives both as numbers).

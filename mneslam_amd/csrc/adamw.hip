@@ -130,7 +130,7 @@ __global__ __launch_bounds__(AW_THREADS) void adamw32_kernel(Adamw32Args a) {
     AdamwHyper h = a.h;
     if (a.clk.bias_table) clock_bias(a.clk, h.lr, h.step, h.step_size, h.root_bc2);
     const long long base = (long long)((int)blockIdx.x - a.first[s]) * AW_WG32;
-    if (a.aligned[s] && base + AW_WG32 <= a.n[s]) adamw32_body<PT, GT, PAST, true>(a, h, s, base);
+    if (base + AW_WG32 <= a.n[s]) adamw32_body<PT, GT, PAST, true>(a, h, s, base);
     else adamw32_body<PT, GT, PAST, false>(a, h, s, base);
 }
 
@@ -316,19 +316,19 @@ __global__ __launch_bounds__(AW_THREADS) void adamw8_kernel(Adamw8Args a) {
     }
     constexpr int BLOCKS = AW_THREADS / AW_LANES8;
     const long long wg = (int)blockIdx.x - a.first[s], b = wg * BLOCKS + threadIdx.x / AW_LANES8;
-    if (a.aligned[s] && (wg + 1) * AW_WG8 <= a.n[s]) adamw8_body<PT, GT, PAST, true>(a, h, step, s, b);
+    if ((wg + 1) * AW_WG8 <= a.n[s]) adamw8_body<PT, GT, PAST, true>(a, h, step, s, b);
     else adamw8_body<PT, GT, PAST, false>(a, h, step, s, b);
 }
 
 // what 8-bit moments stand for, in 32 bits: exp_avg and exp_avg_sq, four elements a thread
 __global__ __launch_bounds__(AW_THREADS) void adamw_moments_kernel(const signed char* mc, const unsigned char* rc, const float* scales,
-                                                                   long long n, float* m, float* v, int aligned) {
+                                                                   long long n, float* m, float* v) {
     const long long i = 4 * ((long long)blockIdx.x * AW_THREADS + threadIdx.x);
     if (i >= n) return;
     const float2 scale = ((const float2*)scales)[i / AW_BLOCK];
     union { MneBytes<4> v; signed char c[4]; } a;
     union { MneBytes<4> v; unsigned char c[4]; } b;
-    const bool full = aligned && i + 4 <= n;
+    const bool full = i + 4 <= n;
     if (full) {
         a.v = *(const MneBytes<4>*)(mc + i);
         b.v = *(const MneBytes<4>*)(rc + i);
@@ -386,8 +386,7 @@ int mne_launch_adamw8(const Adamw8Args& a, int p_type, int g_type, unsigned bloc
     return aw_by_type<Adamw8Args, Launch8>(a, p_type, g_type, blocks, past, st);
 }
 int mne_launch_adamw_moments(const signed char* mc, const unsigned char* rc, const float* scales, long long n, float* m, float* v, hipStream_t st) {
-    const int aligned = ((uintptr_t)mc % 4 | (uintptr_t)rc % 4 | (uintptr_t)m % 16 | (uintptr_t)v % 16) == 0;
-    MNE_LAUNCH(adamw_moments_kernel, (unsigned)((n + 4 * AW_THREADS - 1) / (4 * AW_THREADS)), AW_THREADS, 0, st, mc, rc, scales, n, m, v, aligned);
+    MNE_LAUNCH(adamw_moments_kernel, (unsigned)((n + 4 * AW_THREADS - 1) / (4 * AW_THREADS)), AW_THREADS, 0, st, mc, rc, scales, n, m, v);
     return 0;
 }
 // Calls that touch more than twice what the last cache holds leave it to others: 33.6 M fp32 values (940 MB) 163 us instead of 181; of less,

@@ -762,11 +762,9 @@ int mne_adamw_step(const int64_t* table, int64_t n_tensors, const mne_adamw_cfg_
             a8.p[n_seg] = (void*)t[0]; a8.g[n_seg] = (void*)t[1]; a8.m[n_seg] = (void*)t[2]; a8.v[n_seg] = (void*)t[3];
             a8.scales[n_seg] = (float*)t[4]; a8.n[n_seg] = t[5]; a8.key[n_seg] = mne_adamw_key(cfg->seed, (unsigned)t[6]);
             a8.first[n_seg] = (int)blocks;
-            a8.aligned[n_seg] = t[0] % 16 == 0 && t[1] % 16 == 0 && t[2] % 8 == 0 && t[3] % 8 == 0;
         } else {
             a32.p[n_seg] = (void*)t[0]; a32.g[n_seg] = (void*)t[1]; a32.m[n_seg] = (void*)t[2]; a32.v[n_seg] = (void*)t[3];
             a32.n[n_seg] = t[5]; a32.first[n_seg] = (int)blocks;
-            a32.aligned[n_seg] = ((t[0] | t[1] | t[2] | t[3]) & 15) == 0;
         }
         ++n_seg; blocks += more;
     }

@@ -323,7 +323,6 @@ struct Adamw32Args {
     void *p[MNE_ADAMW32_SEGS], *g[MNE_ADAMW32_SEGS], *m[MNE_ADAMW32_SEGS], *v[MNE_ADAMW32_SEGS];
     long long n[MNE_ADAMW32_SEGS];
     int first[MNE_ADAMW32_SEGS];
-    unsigned char aligned[MNE_ADAMW32_SEGS];      // every address a multiple of 16 bytes
 };
 struct Adamw8Args {
     AdamwHyper h;
@@ -334,7 +333,6 @@ struct Adamw8Args {
     long long n[MNE_ADAMW8_SEGS];
     unsigned key[MNE_ADAMW8_SEGS];
     int first[MNE_ADAMW8_SEGS];
-    unsigned char aligned[MNE_ADAMW8_SEGS];       // parameter and gradient at multiples of 16 bytes, codes of 8
 };
 static_assert(sizeof(Adamw32Args) <= 4096 && sizeof(Adamw8Args) <= 4096, "kernel arguments are limited to 4 KB");
 

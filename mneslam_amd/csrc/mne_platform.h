@@ -109,9 +109,11 @@ static __device__ __forceinline__ int mne_xcc_id() {
     } while (0)
 #endif
 
-// B bytes of memory that are loaded and stored as one
-template <int B> struct MneBytes { typedef unsigned words __attribute__((ext_vector_type(B / 4))); words v; };
-template <> struct MneBytes<4> { typedef unsigned words; words v; };
+// B bytes of memory, at any address, that are loaded and stored as one (global memory takes them so whatever their alignment)
+template <int B> struct MneBytes;
+template <> struct MneBytes<16> { typedef unsigned words __attribute__((ext_vector_type(4), aligned(1))); words v; };
+template <> struct MneBytes<8> { typedef unsigned words __attribute__((ext_vector_type(2), aligned(1))); words v; };
+template <> struct MneBytes<4> { typedef unsigned words __attribute__((aligned(1))); words v; };
 // of data that nothing reads again soon: it leaves the caches to others
 template <int B> static __device__ __forceinline__ MneBytes<B> mne_load_once(const MneBytes<B>* p) {
     MneBytes<B> x;

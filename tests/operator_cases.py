@@ -641,6 +641,38 @@ def check_adamw_many(device, count, bits):
         assert torch.equal(p, ps[k]) and all(torch.equal(a, b) for a, b in zip(st[0][0], state[k][0])), k
 
 
+def check_adamw_flat(device, bits, ptype):
+    """Tensors cut from flat buffers at odd places, moments and codes too: the same bits as for tensors of their own, and what lies
+    between them is left as it was."""
+    gen = torch.Generator().manual_seed(14)
+    dt, sizes = NAMES[ptype], [5000, 2048, 3, 4099, 1]
+    starts = [1 + sum(sizes[:k]) + 3 * k for k in range(len(sizes))]
+    total = starts[-1] + sizes[-1] + 7
+    flat = lambda t: torch.full((total,), 77, dtype=t, device=device)          # noqa: E731
+    p, g, m, v = flat(dt), flat(dt), flat(torch.int8 if bits == 8 else torch.float32), flat(torch.uint8 if bits == 8 else torch.float32)
+    cut = lambda t: [t[a:a + n] for a, n in zip(starts, sizes)]                # noqa: E731
+    for q, h in zip(cut(p), cut(g)):
+        q.copy_(torch.randn(len(q), generator=gen))
+        h.copy_(torch.randn(len(h), generator=gen))
+    for t in cut(m) + cut(v):
+        t.zero_()
+    own = [[t.clone() for t in cut(x)] for x in (p, g, m, v)]
+    scales = [[torch.zeros(-(-n // 256), 2, device=device) for n in sizes] if bits == 8 else None for _ in range(2)]
+    for step in (1, 2):
+        for lists, s in (([cut(x) for x in (p, g, m, v)], scales[0]), (own, scales[1])):
+            optim.adamw_step(*lists, s, step=step, lr=0.01, seed=3)
+    for x, y in zip((p, m, v), (own[0], own[2], own[3])):
+        assert all(torch.equal(a, b) for a, b in zip(cut(x), y))
+        between = torch.ones(total, dtype=torch.bool, device=device)
+        for a, n in zip(starts, sizes):
+            between[a:a + n] = False
+        assert (x[between] == 77).all()
+    if bits == 8:
+        for a, n, s in zip(starts, sizes, scales[0]):
+            got, want = optim.adamw_moments(m[a:a + n], v[a:a + n], s), optim.adamw_moments(m[a:a + n].clone(), v[a:a + n].clone(), s)
+            assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
 def check_adamw_clock(device, bits):
     """Steps that read their number from device memory equal those that are given it."""
     import ctypes as C

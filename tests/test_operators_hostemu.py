@@ -110,6 +110,12 @@ def test_adamw_many_tensors(bits):
 
 
 @pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("ptype", ["f32", "bf16"])
+def test_adamw_flat_buffers(bits, ptype):
+    oc.check_adamw_flat(DEV, bits, ptype)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
 def test_adamw_clock(bits):
     oc.check_adamw_clock(DEV, bits)
 
