@@ -41,23 +41,30 @@ __device__ __forceinline__ void ex_ids(const ExpertSortArgs& a, long long first,
     }
 }
 
-__device__ __forceinline__ void ex_count(const ExpertSortArgs& a, long long first, long long last, int* cnt) {
-    for (long long j0 = first; j0 < last; j0 += 64 * EX_AHEAD) {
-        int e[EX_AHEAD];
-        ex_ids(a, j0, last, e);
+// e: the ids of the first EX_AHEAD x 64 slots, loaded before
+__device__ __forceinline__ void ex_count(const ExpertSortArgs& a, long long first, long long last, const int* e, int* cnt) {
+#pragma unroll
+    for (int j = 0; j < EX_AHEAD; ++j)
+        if (e[j] >= 0) atomicAdd(&cnt[e[j]], 1);
+    for (long long j0 = first + 64 * EX_AHEAD; j0 < last; j0 += 64 * EX_AHEAD) {
+        int more[EX_AHEAD];
+        ex_ids(a, j0, last, more);
 #pragma unroll
         for (int j = 0; j < EX_AHEAD; ++j)
-            if (e[j] >= 0) atomicAdd(&cnt[e[j]], 1);
+            if (more[j] >= 0) atomicAdd(&cnt[more[j]], 1);
     }
 }
 
 __global__ __launch_bounds__(EX_THREADS) void expert_count_kernel(ExpertSortArgs a) {
     MNE_DYN_LDS(lds);
     int* cnt = (int*)lds;
+    const long long first = ((long long)blockIdx.x * EX_WAVES + (threadIdx.x >> 6)) * a.per_wave;
+    const long long last = first + a.per_wave < a.m ? first + a.per_wave : a.m;
+    int ids[EX_AHEAD];
+    ex_ids(a, first, last, ids);
     for (int e = threadIdx.x; e <= a.experts; e += EX_THREADS) cnt[e] = 0;
     __syncthreads();
-    const long long first = ((long long)blockIdx.x * EX_WAVES + (threadIdx.x >> 6)) * a.per_wave;
-    ex_count(a, first, first + a.per_wave < a.m ? first + a.per_wave : a.m, cnt);
+    ex_count(a, first, last, ids, cnt);
     __syncthreads();
     for (int e = threadIdx.x; e <= a.experts; e += EX_THREADS) a.count[(long long)blockIdx.x * (a.experts + 1) + e] = cnt[e];
 }
@@ -101,12 +108,12 @@ __global__ __launch_bounds__(WAVES * 64) void expert_place_kernel(ExpertSortArgs
     __shared__ int part[WAVES], sums[HOW == EX_SUMS ? 2 * EX_THREADS : 1];
     const int bins = a.experts + 1, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     int* mine = cnt + w * bins;
-    for (int e = threadIdx.x; e < WAVES * bins; e += WAVES * 64) cnt[e] = 0;
-    __syncthreads();
     const long long first = ((long long)blockIdx.x * WAVES + w) * a.per_wave;
     const long long last = first + a.per_wave < a.m ? first + a.per_wave : a.m;
-    ex_count(a, first, last, mine);
-    if (HOW == EX_SUMS) {                           // `lane` e of every `span` has expert e, the spans share the chunks
+    int ids[EX_AHEAD];                              // on their way while the counters are cleared and added up
+    ex_ids(a, first, last, ids);
+    for (int e = threadIdx.x; e < WAVES * bins; e += WAVES * 64) cnt[e] = 0;
+    if (HOW == EX_SUMS) {                           // lane e of every `span` has expert e, the spans share the chunks
         int span = 1;
         while (span < bins) span <<= 1;
         const int e = threadIdx.x & (span - 1), at = threadIdx.x / span, step = EX_THREADS / span;
@@ -134,6 +141,8 @@ __global__ __launch_bounds__(WAVES * 64) void expert_place_kernel(ExpertSortArgs
         __syncthreads();
         if ((int)threadIdx.x < bins) { sums[2 * threadIdx.x] = before; sums[2 * threadIdx.x + 1] = all; }
     }
+    __syncthreads();
+    ex_count(a, first, last, ids, mine);
     __syncthreads();
     // first row of every expert: a thread has a run of them, the threads' sums are scanned
     const int each = (bins + WAVES * 64 - 1) / (WAVES * 64), lo = threadIdx.x * each, hi = lo + each < bins ? lo + each : bins;
@@ -168,8 +177,7 @@ __global__ __launch_bounds__(WAVES * 64) void expert_place_kernel(ExpertSortArgs
     int bits = 0;
     while ((1 << bits) < bins) ++bits;
     for (long long j0 = first; j0 < last; j0 += 64 * EX_AHEAD) {
-        int ids[EX_AHEAD];
-        ex_ids(a, j0, last, ids);
+        if (j0 > first || last - first > 64 * EX_AHEAD) ex_ids(a, j0, last, ids);
         for (int j = 0; j < EX_AHEAD && j0 + 64 * j < last; ++j) {        // 64 slots at a time, in order
             int e = -1;
 #pragma unroll
