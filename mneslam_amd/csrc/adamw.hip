@@ -20,7 +20,7 @@
 //
 // With 32-bit moments the step is bound by memory: 38.4 M fp32 values 180 us (28 bytes each, 6.0 TB/s), 67 M bf16 values in 256 tensors 250 us
 // (22 bytes, 5.9 TB/s).  With 8-bit ones it is where the parameters are fp32 (38.4 M: 95 us, 16 bytes, 6.5 TB/s); with bf16 parameters (10
-// bytes) it is bound by its 83 vector instructions an element, four of them roots and reciprocals: 67 M values 187 us.
+// bytes) it is bound by its 83 vector instructions an element, four of them roots and reciprocals: 67 M values 176 us (3.8 TB/s).
 #include "mne_device.h"
 #include "mne_elem.h"
 #include "mne_launch.h"
@@ -29,7 +29,8 @@
 #define AW_BLOCK 256                                 // elements that share two scales
 // Elements a workgroup takes: 4 a thread with 32-bit moments, and 8 a thread (32 lanes a block) with 8-bit ones.  Measured: 32-bit
 // moments, 67 M bf16 values in 256 tensors: 250 us with 4 a thread, 291 with 8, 331 with 16 (38.4 M fp32 values: 180, 186, 183); 8-bit
-// moments: 187 us with 32 lanes a block, 204 with 16, 216 with 64, which are 0.5 us faster than 32 in the smallest calls (5.7 us).
+// moments: 187 us with 32 lanes a block, 204 with 16, 216 with 64, which are 0.5 us faster than 32 in the smallest calls (5.7 us).  (All
+// of these before the last 5 %, which came to each of them.)
 #define AW_PAST (1ll << 29)                          // bytes of a call from which on it goes past the caches
 #define AW_EACH32 4
 #define AW_LANES8 32

@@ -5,6 +5,10 @@
 //   dispatch  out[position[n][k]] = x[n]                                  dx[n] = sum_k dout[position[n][k]]      (combine, no weights)
 //   combine   out[n] = sum_k w[n][k] y[position[n][k]]                    dy[position[n][k]] = w[n][k] dout[n],  dw[n][k] = <dout[n], y[position[n][k]]>
 //
+// The row movements are bound by memory: 131071 tokens x 4 rows of 2048 bf16 are dealt out in 500 us (2.7 GB, 5.4 TB/s) and combined in 435
+// (6.1 TB/s), 16384 x 2 rows of 1024 bf16 in 17 and 16 us, their gradients in 16 and 28 us (166 MB, 5.9 TB/s); rows whose length is no
+// multiple of a line at 4 to 5 TB/s (275200 rows of 65 fp32: 37, 36, 36 and 48 us).
+//
 // A row of the sorted side belongs to one slot, so nothing is added up across workgroups: no atomics on results, and the same bits
 // every time.  Sums are fp32 over k = 0, 1, ... (and over a row in a fixed order); a 16-bit result is rounded to nearest even once.
 #include "mne_device.h"
@@ -22,9 +26,9 @@
 // ---- sort ------------------------------------------------------------------------------------------------------------
 // Bound by launches and round trips to memory, not by bytes.  Three forms (us, 8 / 129 / 1000 experts, one choice each):
 //   slots                                     512                4096               32768              524288
-//   one workgroup                             4.0 / 4.4 / 5.7    6.8 / 7.7 / 9.4    (16384: 16.9 / 20.5 / 23.5)
-//   count, place with the sums in it          6.8 / 7.2 / -      6.9 / 8.1 / -      7.2 / 15.6* / -    12.3 / - / -
-//   count, scan, place                        10.6 / 11.1 / 13.5 10.8 / 11.5 / 14.2 11.1 / 12.0 / 14.4 15.1 / 17.1 / 22.2
+//   one workgroup                             3.6 / 4.0 / 5.2    6.1 / 7.0 / 8.6    (16384: 16 / 20 / 23)
+//   count, place with the sums in it          6.4 / 6.8 / -      6.5 / 7.7 / -      6.9 / 15.2* / -    11.7 / - / -
+//   count, scan, place                        10.2 / 10.7 / 13.1 10.4 / 11.1 / 13.8 10.7 / 11.7 / 13.9 14.5 / 16.4 / 21.5
 // so: one workgroup up to 4096 slots, else sums in place up to 16384 counters (* : beyond them), else a scan of its own.
 __device__ __forceinline__ int ex_id(const ExpertSortArgs& a, int slot) {        // what names no expert sorts behind all of them
     const long long e = a.wide ? ((const long long*)a.ids)[slot] : ((const int*)a.ids)[slot];
@@ -498,7 +502,7 @@ static unsigned ex_grid(long long units, int group) {
 
 // What goes past the caches (PAST): 0 nothing, 1 what is written, 2 what is read as well.
 // Written: rows of whole 128-byte lines only -- 32768 rows of 2 KB combined 16 us instead of 30, dealt out 17 instead of 22; with rows of
-// 260 bytes, whose lines are written by two, 61 us instead of 36.  Dealt-out rows up to 1 GB (2.1 GB: 500 us instead of 475).
+// 260 bytes, whose lines are written by two, 61 us instead of 36.
 // (Combined rows lie one after the other, and still: rows of 64 bytes 69 us and 67 without, of 32 bytes 98 and 78.)
 // Read: combined rows of 128 MB and more in all, half of what the last cache holds: 128 MB 31 us instead of 33, 2.1 GB 429 instead of 464;
 // with 64 MB 17 us instead of 15.  (Its backward pass: 0 to 3 % either way, left alone.)
@@ -571,7 +575,7 @@ template <template <int, int, int> class F> static int ex_by_type(const ExpertRo
 }
 
 int mne_launch_expert_dispatch(ExpertRowArgs a, int type, hipStream_t st) {
-    const int past = ex_whole_lines(a, type) && ex_bytes(a, type) <= 1ll << 30;
+    const int past = ex_whole_lines(a, type);
     return type == MNE_T_F32 ? ex_by_piece<ExDispatch, MNE_T_F32>(a, past, st) : ex_by_piece<ExDispatch, MNE_T_F16>(a, past, st);   // (rows are copied: any 16-bit type)
 }
 int mne_launch_expert_combine(ExpertRowArgs a, int type, hipStream_t st) {
