@@ -216,7 +216,7 @@ static int ex_per_wave(long long m, int experts) {
 }
 static int ex_chunks(long long m, int experts) {
     const long long chunk = (long long)EX_WAVES * ex_per_wave(m, experts);
-    return (int)((m + chunk - 1) / chunk);
+    return m ? (int)((m + chunk - 1) / chunk) : 1;          // (one without slots writes the offsets)
 }
 static bool ex_sums(long long m, int experts) {
     int span = 1;
