@@ -220,7 +220,8 @@ __device__ __forceinline__ void adamw8_body(const Adamw8Args& a, const AdamwHype
             if (a.zero_grad) aw_store<GT, N, FULL, PAST>(g[k], a.g[s], i, n);
         }
     }
-    // Largest magnitudes of the block.  Of sqrt(v) by the bits, where NaN is above infinity; where all of it is finite, all of m is.
+    // Largest magnitudes of the block.  Of sqrt(v) by the bits, where NaN is above infinity; where all of it is finite and the block's m
+    // was, all of m is (a gradient that is not finite, or too large for m, is too large for sqrt(v)).
     float most = 0.0f;
     unsigned br = 0;
 #pragma unroll
@@ -233,7 +234,7 @@ __device__ __forceinline__ void adamw8_body(const Adamw8Args& a, const AdamwHype
         }
     unsigned bm = __float_as_uint(most);
     br = aw_max(br);
-    if (__ballot(br >= 0x7F800000u)) {                // (the whole wave goes this way)
+    if (__ballot(br >= 0x7F800000u || !(fabsf(scale.x) < __uint_as_float(0x7F800000u)))) {      // (the whole wave goes this way)
         bm = 0;
 #pragma unroll
         for (int k = 0; k < K; ++k)
