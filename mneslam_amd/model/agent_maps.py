@@ -51,9 +51,11 @@ class AgentMaps:
         return routing.expert_combine(raw, plan, weights)
 
     def query_sdf(self, points):
+        """sdf [...] of points [...,3]; zero where no map holds the point (see ``covered``)."""
         return self.query_color_sdf(points)[:, 3].reshape(points.shape[:-1])
 
     def query_color(self, points):
+        """rgb [N,3] in 0..1 of points [...,3]; grey (0.5) where no map holds the point."""
         return torch.sigmoid(self.query_color_sdf(points)[:, :3])
 
     def covered(self, points):

@@ -503,6 +503,19 @@ def check_adamw_nonfinite(device, bits):
             assert torch.isnan(m[256:512]).all() == (value != 1e30) and torch.isnan(p[256:512]).all()
 
 
+def check_adamw8_poisoned(device):
+    """A block whose scale of either moment is NaN (a state from elsewhere) stays so, its neighbours do not notice."""
+    for which in (0, 1):
+        p, g = torch.ones(768, device=device), torch.full((768,), 0.01, device=device)
+        state = _step([p], [g], 8, device)
+        state[0][1][1, which] = float("nan")
+        for step in (2, 3):
+            _step([p], [g], 8, device, step=step, state=state)
+        values = optim.adamw_moments(*state[0][0], state[0][1])
+        assert torch.isnan(values[which][256:512]).all() and torch.isfinite(values[which][:256]).all() and torch.isfinite(values[which][512:]).all()
+        assert torch.isfinite(values[1 - which]).all() and torch.isfinite(p[:256]).all() and torch.isfinite(p[512:]).all()
+
+
 def check_adamw8_small_and_zero(device):
     """Zero blocks stay zero, tiny values neither overflow a scale nor lose the second moment."""
     p, g = torch.ones(1024, device=device), torch.zeros(1024, device=device)
@@ -785,6 +798,8 @@ def check_routing_views(device):
             up[t, j] += 1.0
             diff = ((expert_combine(yd, plan, up) - expert_combine(yd, plan, w.detach())).double() * probe.double()).sum()
             assert abs(float(diff) - float(w.grad[t, j])) <= 64 * EPS32
+    for experts in (2000, 2001, 4096):
+        assert expert_sort(torch.zeros(0, 2, dtype=torch.int64, device=device), experts).offsets.tolist() == [0] * (experts + 1)
     empty = expert_sort(torch.zeros(0, 2, dtype=torch.int64, device=device), 3)
     assert empty.offsets.tolist() == [0, 0, 0, 0] and expert_dispatch(torch.zeros(0, 5, device=device), empty).shape == (0, 5)
     assert expert_combine(torch.zeros(0, 5, device=device), empty).shape == (0, 5)

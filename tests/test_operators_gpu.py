@@ -101,6 +101,10 @@ def test_adamw_nonfinite(bits):
     oc.check_adamw_nonfinite(DEV, bits)
 
 
+def test_adamw_8_poisoned():
+    oc.check_adamw8_poisoned(DEV)
+
+
 def test_adamw_8_small_and_zero():
     oc.check_adamw8_small_and_zero(DEV)
 
