@@ -5,12 +5,14 @@
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <algorithm>
 #include <map>
+#include <unordered_set>
 #include <vector>
 
 #include "mneslam_hip.h"
@@ -213,6 +215,28 @@ void once(const char* what) {
     if (c10::GradMode::is_enabled()) throw std::runtime_error(std::string(what) + ": differentiable once (create_graph=True is not supported)");
 }
 
+// A backward pass that is being recorded must not lead on to the default stream, which cannot be recorded: the recording would be broken
+// there in a way that ends the process.  It leads there if something upstream was built on that stream, also by a leaf alone that an
+// eager graph still holds.
+void recordable(const char* what, const at::Device& dev) {
+    if (!dev.is_cuda() || c10::hip::getCurrentHIPStream(dev.index()).id() == 0) return;
+    const c10::DeviceGuard guard(dev);
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    const std::shared_ptr<torch::autograd::Node> self = torch::autograd::get_current_node();
+    std::vector<torch::autograd::Node*> open = {self.get()};
+    std::unordered_set<torch::autograd::Node*> seen;
+    while (!open.empty()) {
+        torch::autograd::Node* node = open.back();
+        open.pop_back();
+        if (!node || !seen.insert(node).second) continue;
+        const auto stream = node->stream();
+        if (stream && stream->id() == 0)
+            throw std::runtime_error(std::string(what) + ": this backward pass cannot be recorded, it leads to " + node->name() +
+                                     " on the default stream (drop the eager graphs of the same leaves first)");
+        for (const auto& edge : node->next_edges()) open.push_back(edge.function.get());
+    }
+}
+
 Library library_of(AutogradContext* ctx) {
     Library lib;
     const std::string bytes = ctx->saved_data["library"].toStringRef();
@@ -229,6 +253,7 @@ struct DispatchNode : torch::autograd::Function<DispatchNode> {
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         once("expert_dispatch");
         if (!grads[0].defined()) return {Variable(), Variable(), Variable()};
+        recordable("expert_dispatch", grads[0].device());
         return {combine(library_of(ctx), grads[0], ctx->get_saved_variables()[0], at::Tensor()), Variable(), Variable()};
     }
 };
@@ -245,6 +270,7 @@ struct CombineNode : torch::autograd::Function<CombineNode> {
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         once("expert_combine");
         if (!grads[0].defined()) return {Variable(), Variable(), Variable(), Variable(), Variable()};
+        recordable("expert_combine", grads[0].device());
         const Library lib = library_of(ctx);
         const variable_list saved = ctx->get_saved_variables();
         const at::Tensor y = rows(saved[0], "expert_combine"), &position = saved[1], &offsets = saved[2];

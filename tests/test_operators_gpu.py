@@ -280,6 +280,31 @@ def test_routing_recorded():
                 assert torch.equal(a, b)
 
 
+def test_routing_recorded_beside_an_eager_graph():
+    """Recording a backward pass whose leaves an eager graph on the default stream holds is refused; without that graph it is recorded."""
+    from mneslam_amd.routing import expert_combine, expert_dispatch, expert_sort
+    ids = torch.tensor([[0, 1], [2, 0], [1, -1]], device=DEV)
+    x, w = torch.randn(3, 8, device=DEV, requires_grad=True), torch.rand(3, 2, device=DEV, requires_grad=True)
+
+    def work():
+        plan = expert_sort(ids, 3)
+        return expert_combine(expert_dispatch(x * 1.0, plan), plan, w)
+
+    eager = work()
+    with pytest.raises(RuntimeError, match="default stream"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            torch.autograd.grad(work().sum(), (x, w))
+    want = torch.autograd.grad(eager.sum(), (x, w))
+    del eager
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(work().sum(), (x, w))
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 @pytest.mark.parametrize("bits", [8, 32])
 def test_adamw_recorded(bits):
     """A step with a clock in a recorded graph equals eager steps; without one it is refused."""
