@@ -87,7 +87,7 @@ void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& exp_
     const at::Device dev = params[0].device();
     const c10::DeviceGuard guard(dev);
     std::map<std::pair<int, int>, std::vector<int64_t>> tables;          // by the types of parameter and gradient
-    std::vector<std::pair<int64_t, int64_t>> ranges;
+    std::vector<std::pair<int64_t, int64_t>> ranges;                     // what the step writes
     Tensors keep;
     c10::NoGradGuard no_grad;
     for (size_t i = 0; i < n; ++i) {
@@ -120,16 +120,23 @@ void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& exp_
             g = at::empty_like(p, p.options().dtype(g.scalar_type())).copy_(g);
             keep.push_back(g);
         }
-        const int64_t at = (int64_t)p.data_ptr();
-        ranges.emplace_back(at, at + count * (int64_t)p.element_size());
+        const auto writes = [&](const at::Tensor& t) {
+            const int64_t at = (int64_t)t.data_ptr();
+            ranges.emplace_back(at, at + t.numel() * (int64_t)t.element_size());
+        };
+        writes(p);
+        writes(m);
+        writes(v);
+        if (small) writes((*scales)[i]);
+        if (zero_grad) writes(g);
         std::vector<int64_t>& table = tables[{pt, gt}];
-        const int64_t row[7] = {at, (int64_t)g.data_ptr(), (int64_t)m.data_ptr(), (int64_t)v.data_ptr(),
+        const int64_t row[7] = {(int64_t)p.data_ptr(), (int64_t)g.data_ptr(), (int64_t)m.data_ptr(), (int64_t)v.data_ptr(),
                                 small ? (int64_t)(*scales)[i].data_ptr() : 0, count, ordinal};
         table.insert(table.end(), row, row + 7);
     }
     std::sort(ranges.begin(), ranges.end());
     for (size_t i = 1; i < ranges.size(); ++i)
-        if (ranges[i].first < ranges[i - 1].second) throw py::value_error("adamw_step: parameters overlap (the same one twice?)");
+        if (ranges[i].first < ranges[i - 1].second) throw py::value_error("adamw_step: parameters or moments overlap (the same one twice?)");
     for (const auto& t : tables) {
         mne_adamw_cfg_t cfg = {};
         cfg.lr = lr; cfg.beta1 = beta1; cfg.beta2 = beta2; cfg.eps = eps; cfg.weight_decay = weight_decay;
@@ -259,10 +266,11 @@ struct DispatchNode : torch::autograd::Function<DispatchNode> {
 };
 
 struct CombineNode : torch::autograd::Function<CombineNode> {
-    // (a node takes no undefined tensor: without weights, `weights` is any other)
+    // (a node takes no undefined tensor: without weights, `weights` is any other; so is what is saved for `y` where the weights have no
+    // gradient, which is all that its values are needed for)
     static Variable forward(AutogradContext* ctx, const Variable& y, const Variable& position, const Variable& offsets, const Variable& weights,
                             bool weighted) {
-        ctx->save_for_backward({y, position, offsets, weights});
+        ctx->save_for_backward({weighted && weights.requires_grad() ? y : position, position, offsets, weights});
         ctx->saved_data["library"] = std::string((const char*)&g_lib, sizeof(g_lib));
         ctx->saved_data["weighted"] = weighted;
         return combine(g_lib, y, position, weighted ? weights : at::Tensor());
@@ -273,18 +281,19 @@ struct CombineNode : torch::autograd::Function<CombineNode> {
         recordable("expert_combine", grads[0].device());
         const Library lib = library_of(ctx);
         const variable_list saved = ctx->get_saved_variables();
-        const at::Tensor y = rows(saved[0], "expert_combine"), &position = saved[1], &offsets = saved[2];
+        const at::Tensor &position = saved[1], &offsets = saved[2];
         const at::Tensor weights = ctx->saved_data["weighted"].toBool() ? saved[3] : at::Tensor();
         const at::Tensor dout = rows(grads[0], "expert_combine"), w = weights.defined() ? weights.to(at::kFloat).contiguous() : weights;
-        const c10::DeviceGuard guard(y.device());
-        const int64_t n = position.size(0), k = position.size(1), width = y.size(1);
+        const c10::DeviceGuard guard(dout.device());
+        const int64_t n = position.size(0), k = position.size(1), width = dout.size(1);
         const bool want_dw = weights.defined() && ctx->needs_input_grad(3), want_dy = ctx->needs_input_grad(0);
+        const at::Tensor y = want_dw ? rows(saved[0], "expert_combine") : dout;          // (not read without dw)
         at::Tensor dy, dw;
-        if (want_dy) dy = at::empty({n * k, width}, y.options());
+        if (want_dy) dy = at::empty({n * k, width}, dout.options());
         if (want_dw) dw = width ? at::empty({n, k}, w.options()) : at::zeros({n, k}, w.options());
-        check(lib.combine_backward(dout.data_ptr(), dout.stride(0), y.data_ptr(), y.stride(0), type_code(y.scalar_type()), n, (int)k, width,
+        check(lib.combine_backward(dout.data_ptr(), dout.stride(0), y.data_ptr(), y.stride(0), type_code(dout.scalar_type()), n, (int)k, width,
                                    ints(position), live_rows(offsets), floats(w), want_dy ? dy.data_ptr() : nullptr,
-                                   want_dw ? (float*)dw.data_ptr() : nullptr, stream_of(y.device())), "mne_expert_combine_backward");
+                                   want_dw ? (float*)dw.data_ptr() : nullptr, stream_of(dout.device())), "mne_expert_combine_backward");
         return {dy, Variable(), Variable(), want_dw ? dw.to(weights.scalar_type()) : dw, Variable()};
     }
 };

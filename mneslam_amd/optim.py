@@ -136,7 +136,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, scales=None, *, step, lr, b
 
     Parameters are float32, bfloat16 or float16; a gradient has its parameter's type or float32 (any of the three beside a float32
     parameter).  The arithmetic is fp32; a 16-bit parameter is rounded to nearest even.  Every tensor is dense (contiguous or
-    channels_last); moments are laid out like their parameter, a gradient laid out otherwise is copied.  Parameters do not overlap.
+    channels_last); moments are laid out like their parameter, a gradient laid out otherwise is copied.  What the step writes does not
+    overlap: parameters, moments, scales, gradients that it clears.
 
     ``scales`` None: moments are float32.  Otherwise they are held in 8 bits: ``exp_avgs`` int8, ``exp_avg_sqs`` uint8, and
     ``scales`` the list of their float32 [ceil(n / 256), 2] scales, two for each 256 consecutive elements of the tensor's memory
@@ -248,8 +249,12 @@ class FusedAdamW(torch.optim.Optimizer):
         return adamw_moments(st["exp_avg"], st["exp_avg_sq"], st["scales"]) if "scales" in st else (st["exp_avg"], st["exp_avg_sq"])
 
     def load_state_dict(self, state_dict):
-        """Also of torch.optim.AdamW's states.  The base class casts floating-point state to its parameter's type: here moments and
-        scales are float32 or the codes they were saved as, laid out like their parameter."""
+        """Also of torch.optim.AdamW's states (not with amsgrad or maximize).  The base class casts floating-point state to its
+        parameter's type: here moments and scales are float32 or the codes they were saved as, laid out like their parameter."""
+        for group in state_dict["param_groups"]:
+            for rule in ("amsgrad", "maximize"):
+                if group.get(rule):
+                    raise ValueError(f"FusedAdamW has no {rule}: the loaded state would go on by another rule")
         super().load_state_dict(state_dict)
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
         for i, p in zip(saved, (p for g in self.param_groups for p in g["params"])):

@@ -516,6 +516,37 @@ def check_adamw8_poisoned(device):
         assert torch.isfinite(values[1 - which]).all() and torch.isfinite(p[:256]).all() and torch.isfinite(p[512:]).all()
 
 
+def check_adamw_shared_state(device):
+    """What a step writes may not be one tensor's and another's: moments, scales, gradients that it clears."""
+    p = [torch.ones(300, device=device) for _ in range(2)]
+    g = [torch.ones(300, device=device) for _ in range(2)]
+    m, v = ([torch.zeros(300, device=device) for _ in range(2)] for _ in range(2))
+    c = [torch.zeros(300, dtype=torch.int8, device=device) for _ in range(2)]
+    d = [torch.zeros(300, dtype=torch.uint8, device=device) for _ in range(2)]
+    s = [torch.zeros(2, 2, device=device) for _ in range(2)]
+    for lists, scales, zero in (([p, g, [m[0], m[0]], v], None, False), ([p, g, m, [v[0], v[0]]], None, False), ([p, g, m, m[::-1]], None, False),
+                                ([p, g, [c[0], c[0]], d], s, False), ([p, g, c, [d[0], d[0]]], s, False), ([p, g, c, d], [s[0], s[0]], False),
+                                ([p, [g[0], g[0]], m, v], None, True), ([p, g, [p[1], m[1]], v], None, False)):
+        with pytest.raises(ValueError, match="overlap"):
+            optim.adamw_step(*lists, scales, step=1, lr=0.1, zero_grad=zero)
+    assert all((x == 1.0).all() for x in p + g) and not any(x.any() for x in m + v + c + d + s)
+    optim.adamw_step(p, [g[0], g[0]], m, v, step=1, lr=0.1)          # a gradient that is only read may be shared
+    assert torch.equal(p[0], p[1]) and (p[0] < 1.0).all()
+
+
+def check_adamw_loads_no_other_rule(device):
+    """States of torch.optim.AdamW with another rule than this step's are refused, and nothing is loaded."""
+    for kw in (dict(amsgrad=True), dict(maximize=True)):
+        p = torch.nn.Parameter(torch.ones(4, device=device))
+        ref = torch.optim.AdamW([p], lr=0.5, **kw)
+        p.grad = torch.ones_like(p)
+        ref.step()
+        opt = optim.FusedAdamW([p], lr=0.25)
+        with pytest.raises(ValueError, match=next(iter(kw))):
+            opt.load_state_dict(ref.state_dict())
+        assert opt.param_groups[0]["lr"] == 0.25 and not opt.state
+
+
 def check_adamw8_small_and_zero(device):
     """Zero blocks stay zero, tiny values neither overflow a scale nor lose the second moment."""
     p, g = torch.ones(1024, device=device), torch.zeros(1024, device=device)
@@ -762,6 +793,28 @@ def check_routing_refusals(device):
     out = expert_combine(y, plan, v * 1)
     y.add_(1)
     with pytest.raises(RuntimeError):
+        out.sum().backward()
+
+
+def check_combine_keeps_what_it_needs(device):
+    """Rows may be written again where their values are no part of a gradient."""
+    from mneslam_amd.routing import expert_combine, expert_sort
+    plan = expert_sort(torch.tensor([[1, 0], [1, -1]], device=device), 2)
+    for w in (None, torch.tensor([[0.5, 2.0], [4.0, 1.0]], device=device)):
+        a = torch.ones(4, 3, device=device, requires_grad=True)
+        y = a * 1.0
+        out = expert_combine(y, plan, w)
+        y.zero_()
+        out.sum().backward()
+        want = torch.zeros(4, 3)
+        for t, j in ((0, 0), (0, 1), (1, 0)):
+            want[int(plan.position[t, j])] = 1.0 if w is None else float(w[t, j])
+        assert torch.equal(a.grad.cpu(), want)
+    w = torch.ones(2, 2, device=device, requires_grad=True)
+    y = torch.ones(4, 3, device=device)
+    out = expert_combine(y, plan, w)
+    y.zero_()
+    with pytest.raises(RuntimeError, match="inplace"):
         out.sum().backward()
 
 

@@ -96,6 +96,18 @@ def test_adamw_8_poisoned():
     oc.check_adamw8_poisoned(DEV)
 
 
+def test_adamw_shared_state():
+    oc.check_adamw_shared_state(DEV)
+
+
+def test_adamw_loads_no_other_rule():
+    oc.check_adamw_loads_no_other_rule(DEV)
+
+
+def test_combine_keeps_what_it_needs():
+    oc.check_combine_keeps_what_it_needs(DEV)
+
+
 def test_adamw_8_small_and_zero():
     oc.check_adamw8_small_and_zero(DEV)
 
