@@ -1,6 +1,6 @@
 // host_tensors.cpp -- the host side of optim.adamw_step and of routing: torch tensors checked and handed to the C ABI, and the autograd
 // nodes of the row movements.  Calls that take a few microseconds on the GPU are bound by what runs before and between them: a list of
-// several hundred tensors costs 2.5 us a tensor in python (about thirty attribute reads) and 0.1 us here, and a backward pass through two
+// several hundred tensors costs 2.5 us a tensor in python (about thirty attribute reads) and 0.25 us here, and a backward pass through two
 // python nodes 140 us and 30 us.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
