@@ -66,6 +66,9 @@ int type_code(at::ScalarType t) {
     return t == at::kFloat ? MNE_T_F32 : t == at::kBFloat16 ? MNE_T_BF16 : t == at::kHalf ? MNE_T_F16 : -1;
 }
 
+// A tensor whose memory holds its values: one that is negated lazily (the imaginary part of a conjugate) is copied.
+at::Tensor in_memory(const at::Tensor& t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
+
 // equal strides in every dimension that has more than one entry (the shapes are equal)
 bool laid_out_alike(const at::Tensor& a, const at::Tensor& b) {
     for (int64_t d = 0; d < a.dim(); ++d)
@@ -105,6 +108,13 @@ void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& exp_
             throw py::type_error(small ? "adamw_step: 8-bit moments must be int8 and uint8" : "adamw_step: moments must be float32");
         if (g.sizes() != p.sizes() || m.sizes() != p.sizes() || v.sizes() != p.sizes())
             throw py::value_error("adamw_step: gradient and moments need their parameter's shape");
+        for (const at::Tensor* t : {&p, &m, &v, small ? &(*scales)[i] : &p})
+            if (t->is_neg()) throw py::value_error("adamw_step: what is written in place must not be a negated view");
+        if (g.is_neg()) {
+            if (zero_grad) throw py::value_error("adamw_step: zero_grad cannot clear a negated view");
+            g = in_memory(g);
+            keep.push_back(g);
+        }
         const int64_t count = p.numel(), ordinal = ordinals ? (*ordinals)[i] : (int64_t)i;
         if (ordinal < 0 || ordinal > 0xFFFFFFFFll) throw py::value_error("adamw_step: ordinals are numbers of 32 bits");
         if (small) {
@@ -148,8 +158,10 @@ void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& exp_
         if (!p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
 }
 
-std::vector<at::Tensor> adamw_moments(const at::Tensor& m, const at::Tensor& v, const at::Tensor& scales) {
-    one_device("adamw_moments", {&m, &v, &scales});
+std::vector<at::Tensor> adamw_moments(const at::Tensor& given_m, const at::Tensor& given_v, const at::Tensor& given_scales) {
+    one_device("adamw_moments", {&given_m, &given_v, &given_scales});
+    c10::NoGradGuard no_grad;
+    const at::Tensor m = in_memory(given_m), v = in_memory(given_v), scales = in_memory(given_scales);
     if (m.scalar_type() != at::kChar || v.scalar_type() != at::kByte) throw py::type_error("adamw_moments: the codes are int8 and uint8");
     if (m.sizes() != v.sizes() || !m.is_non_overlapping_and_dense() || !laid_out_alike(m, v))
         throw py::value_error("adamw_moments: the codes must be dense and laid out alike");
@@ -157,7 +169,6 @@ std::vector<at::Tensor> adamw_moments(const at::Tensor& m, const at::Tensor& v, 
     if (scales.scalar_type() != at::kFloat || scales.dim() != 2 || scales.size(0) != (n + 255) / 256 || scales.size(1) != 2 || !scales.is_contiguous())
         throw py::value_error("adamw_moments: scales must be contiguous float32 [ceil(n / 256), 2]");
     const c10::DeviceGuard guard(m.device());
-    c10::NoGradGuard no_grad;
     at::Tensor a = at::empty_like(m, m.options().dtype(at::kFloat)), b = at::empty_like(a);
     check(g_lib.adamw_moments((const int8_t*)m.data_ptr(), (const uint8_t*)v.data_ptr(), (const float*)scales.data_ptr(), n,
                               (float*)a.data_ptr(), (float*)b.data_ptr(), stream_of(m.device())), "mne_adamw_moments");
@@ -176,7 +187,7 @@ std::vector<at::Tensor> expert_sort(const at::Tensor& given, int64_t experts) {
     if (m >= (1ll << 31) - 65536) throw py::value_error("expert_sort: too many choices for 32-bit rows");
     const c10::DeviceGuard guard(given.device());
     c10::NoGradGuard no_grad;
-    const at::Tensor ids = given.contiguous();
+    const at::Tensor ids = in_memory(given).contiguous();
     const size_t bytes = g_lib.sort_bytes(m, (int)experts);
     // one allocation: order, position, offsets, workspace
     const at::Tensor all = at::empty({2 * m + experts + 1 + (int64_t)bytes / 4}, ids.options().dtype(at::kInt));
@@ -187,12 +198,14 @@ std::vector<at::Tensor> expert_sort(const at::Tensor& given, int64_t experts) {
 }
 
 // a row's elements next to each other (a copy where they are not)
-at::Tensor rows(const at::Tensor& t, const char* what) {
+at::Tensor rows(const at::Tensor& given, const char* what) {
+    const at::Tensor t = in_memory(given);
     if (t.dim() != 2) throw py::value_error(std::string(what) + ": rows must be [rows, width]");
     if (type_code(t.scalar_type()) < 0)
         throw py::type_error(std::string(what) + ": " + c10::toString(t.scalar_type()) + " is not supported (float32, bfloat16, float16)");
     return t.stride(1) == 1 || t.size(1) <= 1 ? t : t.contiguous();
 }
+at::Tensor weights32(const at::Tensor& t) { return t.defined() ? in_memory(t).to(at::kFloat).contiguous() : t; }
 const int32_t* ints(const at::Tensor& t) { return (const int32_t*)t.data_ptr(); }
 const int32_t* live_rows(const at::Tensor& offsets) { return ints(offsets) + offsets.size(0) - 1; }
 const float* floats(const at::Tensor& t) { return t.defined() ? (const float*)t.data_ptr() : nullptr; }
@@ -208,7 +221,7 @@ at::Tensor dispatch(const Library& lib, const at::Tensor& given, const at::Tenso
 }
 
 at::Tensor combine(const Library& lib, const at::Tensor& given, const at::Tensor& position, const at::Tensor& weights) {
-    const at::Tensor y = rows(given, "expert_combine"), w = weights.defined() ? weights.to(at::kFloat).contiguous() : weights;
+    const at::Tensor y = rows(given, "expert_combine"), w = weights32(weights);
     const c10::DeviceGuard guard(y.device());
     const int64_t n = position.size(0), k = position.size(1), width = y.size(1);
     at::Tensor out = at::empty({n, width}, y.options());
@@ -283,7 +296,7 @@ struct CombineNode : torch::autograd::Function<CombineNode> {
         const variable_list saved = ctx->get_saved_variables();
         const at::Tensor &position = saved[1], &offsets = saved[2];
         const at::Tensor weights = ctx->saved_data["weighted"].toBool() ? saved[3] : at::Tensor();
-        const at::Tensor dout = rows(grads[0], "expert_combine"), w = weights.defined() ? weights.to(at::kFloat).contiguous() : weights;
+        const at::Tensor dout = rows(grads[0], "expert_combine"), w = weights32(weights);
         const c10::DeviceGuard guard(dout.device());
         const int64_t n = position.size(0), k = position.size(1), width = dout.size(1);
         const bool want_dw = weights.defined() && ctx->needs_input_grad(3), want_dy = ctx->needs_input_grad(0);
@@ -302,6 +315,7 @@ void check_plan(const char* what, const at::Tensor& position, const at::Tensor& 
     if (position.scalar_type() != at::kInt || offsets.scalar_type() != at::kInt) throw py::type_error(std::string(what) + ": a plan's tensors are int32");
     if (position.dim() != 2 || position.size(1) < 1 || offsets.dim() != 1 || offsets.size(0) < 2 || !position.is_contiguous() || !offsets.is_contiguous())
         throw py::value_error(std::string(what) + ": not a plan of expert_sort");
+    if (position.is_neg() || offsets.is_neg()) throw py::value_error(std::string(what) + ": a plan's tensors must not be negated views");
 }
 
 at::Tensor expert_dispatch(const at::Tensor& x, const at::Tensor& position, const at::Tensor& offsets) {

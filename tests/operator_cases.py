@@ -856,3 +856,65 @@ def check_routing_views(device):
     empty = expert_sort(torch.zeros(0, 2, dtype=torch.int64, device=device), 3)
     assert empty.offsets.tolist() == [0, 0, 0, 0] and expert_dispatch(torch.zeros(0, 5, device=device), empty).shape == (0, 5)
     assert expert_combine(torch.zeros(0, 5, device=device), empty).shape == (0, 5)
+
+
+# ------------------------------------------------------------------------------------------- tensors whose memory is not their values
+def _lazily_negated(t):
+    """``t`` as a view whose memory holds -t; t of one column (or one element) also as torch's public calls make it."""
+    if t.is_floating_point() and t.dtype == torch.float32 and t.stride(-1) == 1 and t.shape[-1] == 1:
+        view = torch.complex(torch.zeros_like(t), -t).conj().imag
+    else:
+        view = torch._neg_view(-t)
+    assert view.is_neg() and torch.equal(view, t)
+    return view
+
+
+def check_negated_rows(device, dtype, width):
+    """A lazily negated input of routing counts as its values: ids, tokens, rows, weights and the gradients that come in."""
+    from mneslam_amd.routing import ExpertPlan, expert_combine, expert_dispatch, expert_sort
+    gen = torch.Generator().manual_seed(41)
+    n, k, e = 9, 2, 3
+    dt = NAMES[dtype]
+    ids = torch.randint(0, e, (n, k), generator=gen).to(device)
+    x, y, w, gx, gy = (torch.randn(s, generator=gen).to(t).to(device) for s, t in
+                       (((n, width), dt), ((n * k, width), dt), ((n, k), torch.float32), ((n * k, width), dt), ((n, width), dt)))
+    plan = expert_sort(ids, e)
+    again = expert_sort(_lazily_negated(ids), e)
+    assert torch.equal(plan.position, again.position) and torch.equal(plan.order, again.order)
+    results = []
+    for seen in (lambda t: t, _lazily_negated):
+        a, b, c = (seen(t).detach().requires_grad_(True) for t in (x, y, w))
+        xs, out = expert_dispatch(a, plan), expert_combine(b, plan, c)
+        results.append([xs, out, *torch.autograd.grad((xs, out), (a, b, c), (seen(gx), seen(gy)))])
+    for plain, negated in zip(*results):
+        assert torch.equal(plain, negated)
+    wrong = ExpertPlan(plan.order, torch._neg_view(plan.position), plan.offsets)
+    for f in (lambda: expert_dispatch(x, wrong), lambda: expert_combine(y, wrong)):
+        with pytest.raises(ValueError, match="negated"):
+            f()
+
+
+def check_negated_adamw(device, bits):
+    """A lazily negated gradient counts as its values; what is written in place must not be such a view."""
+    for n in (1, 300):
+        gen = torch.Generator().manual_seed(42)
+        g = torch.randn(n, generator=gen).to(device)
+        ps = [torch.ones(n, device=device) for _ in range(2)]
+        states = [_step([p], [h], bits, device)[0] for p, h in zip(ps, (g, _lazily_negated(g)))]
+        assert torch.equal(*ps) and (n == 1 or not torch.equal(ps[0], torch.ones_like(ps[0])))
+        for a, b in zip(*(s[0] for s in states)):
+            assert torch.equal(a, b)
+        p, (lists, scales) = ps[0], states[0]
+        before = p.clone()
+        written = [[p], [lists[0]], [lists[1]]] + ([[scales]] if bits == 8 else [])
+        for k in range(len(written)):
+            args = [[torch._neg_view(t[0])] if i == k else t for i, t in enumerate(written)]
+            with pytest.raises(ValueError, match="negated"):
+                optim.adamw_step(args[0], [g], args[1], args[2], args[3] if bits == 8 else None, step=2, lr=0.1)
+        with pytest.raises(ValueError, match="negated"):
+            optim.adamw_step([p], [_lazily_negated(g)], [lists[0]], [lists[1]], [scales] if bits == 8 else None, step=2, lr=0.1, zero_grad=True)
+        assert torch.equal(p, before)
+        if bits == 8:
+            want = optim.adamw_moments(*lists, scales)
+            got = optim.adamw_moments(_lazily_negated(lists[0]), lists[1], _lazily_negated(scales))
+            assert all(torch.equal(a, b) for a, b in zip(got, want))

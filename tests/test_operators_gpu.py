@@ -351,3 +351,14 @@ def test_adamw_recorded(bits):
         with torch.cuda.graph(torch.cuda.CUDAGraph()):
             opt.step(clock=clock)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("width", [1, 6])
+def test_routing_of_negated_views(dtype, width):
+    oc.check_negated_rows(DEV, dtype, width)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_adamw_of_negated_views(bits):
+    oc.check_negated_adamw(DEV, bits)

@@ -142,3 +142,14 @@ def test_routing_refusals():
 
 def test_routing_views():
     oc.check_routing_views(DEV)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("width", [1, 6])
+def test_routing_of_negated_views(dtype, width):
+    oc.check_negated_rows(DEV, dtype, width)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_adamw_of_negated_views(bits):
+    oc.check_negated_adamw(DEV, bits)
