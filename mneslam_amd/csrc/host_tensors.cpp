@@ -5,9 +5,12 @@
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <algorithm>
@@ -48,11 +51,30 @@ void check(int rc, const char* what) {
     if (rc) throw std::runtime_error(std::string("libmneslam_hip ") + what + " failed (" + std::to_string(rc) + "): " + g_lib.last_error());
 }
 
+// These calls are no operators of torch's dispatcher: a tracer sees the allocation of their results and not what fills it, so the program it
+// makes would return memory that nothing wrote.  (Modes that only watch real operations, a counter for instance, are let through.)
+void not_traced(const char* what) {
+    using c10::impl::TorchDispatchModeKey;
+    using c10::impl::TorchDispatchModeTLS;
+    bool traced = torch::jit::tracer::isTracing() || c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch);
+    if (TorchDispatchModeTLS::any_modes_set())
+        for (const auto key : {TorchDispatchModeKey::PROXY, TorchDispatchModeKey::FAKE, TorchDispatchModeKey::FUNCTIONAL})
+            traced = traced || TorchDispatchModeTLS::get_mode(key).has_value();
+    if (traced) throw std::runtime_error(std::string(what) + ": this call cannot be traced (torch.jit.trace, make_fx, fake tensors)");
+}
+// ... and a tensor whose class brings its own operations is not the memory it holds.
+void no_subclass(const char* what, const at::Tensor& t) {
+    if (t.unsafeGetTensorImpl()->is_python_dispatch())
+        throw py::type_error(std::string(what) + ": tensors of classes with operations of their own are not supported");
+}
+
 // All on one device that the library reaches (a kernel that is given an address of host memory would fault).
 void one_device(const char* what, std::initializer_list<const at::Tensor*> tensors) {
+    not_traced(what);
     const at::Device dev = (*tensors.begin())->device();
     for (const at::Tensor* t : tensors) {
         if (!t->defined()) continue;
+        no_subclass(what, *t);
         if (t->layout() != at::kStrided) throw py::value_error(std::string(what) + ": sparse tensors are not supported");
         if (t->device() != dev) throw py::value_error(std::string(what) + ": tensors on " + dev.str() + " and on " + t->device().str());
     }
@@ -98,6 +120,7 @@ void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& exp_
         at::Tensor g = grads[i];
         for (const at::Tensor* t : {&p, (const at::Tensor*)&g, &m, &v, small ? &(*scales)[i] : &p}) {
             if (!t->defined() || t->layout() != at::kStrided) throw py::value_error("adamw_step: sparse or undefined tensors are not supported");
+            no_subclass("adamw_step", *t);
             if (t->device() != dev) throw py::value_error("adamw_step: tensors on " + dev.str() + " and on " + t->device().str());
         }
         const int pt = type_code(p.scalar_type()), gt = type_code(g.scalar_type());
@@ -272,6 +295,7 @@ struct DispatchNode : torch::autograd::Function<DispatchNode> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         once("expert_dispatch");
+        not_traced("expert_dispatch");
         if (!grads[0].defined()) return {Variable(), Variable(), Variable()};
         recordable("expert_dispatch", grads[0].device());
         return {combine(library_of(ctx), grads[0], ctx->get_saved_variables()[0], at::Tensor()), Variable(), Variable()};
@@ -290,6 +314,7 @@ struct CombineNode : torch::autograd::Function<CombineNode> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         once("expert_combine");
+        not_traced("expert_combine");
         if (!grads[0].defined()) return {Variable(), Variable(), Variable(), Variable(), Variable()};
         recordable("expert_combine", grads[0].device());
         const Library lib = library_of(ctx);

@@ -7,8 +7,9 @@
 
 ``expert_dispatch`` and ``expert_combine`` are differentiable (tokens, rows and weights; once).  Nothing waits for the GPU:
 ``plan.sizes()`` is the one call that does, for experts whose calls need their number of rows on the host.  All of it can be recorded into
-a graph; a backward pass that is recorded while an eager graph of the same leaves lives on the default stream is refused.  The kernels
-are csrc/routing.hip; there is no fallback."""
+a graph; a backward pass that is recorded while an eager graph of the same leaves lives on the default stream is refused.  Under a
+tracer (torch.jit.trace, make_fx, torch.export) the calls are refused; torch.compile runs them between its graphs.  The kernels are
+csrc/routing.hip; there is no fallback."""
 from . import _lib
 
 

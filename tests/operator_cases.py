@@ -918,3 +918,45 @@ def check_negated_adamw(device, bits):
             want = optim.adamw_moments(*lists, scales)
             got = optim.adamw_moments(_lazily_negated(lists[0]), lists[1], _lazily_negated(scales))
             assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def check_not_traced(device):
+    """A tracer cannot see what these calls compute: they are refused under one, and do nothing; modes that only watch are let through."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils.flop_counter import FlopCounterMode
+    from mneslam_amd.routing import expert_combine, expert_dispatch, expert_sort
+    ids = torch.tensor([[0, 1], [1, -1], [2, 0]], device=device)
+    plan = expert_sort(ids, 3)
+    x, y = torch.arange(15.0, device=device).view(3, 5), torch.arange(30.0, device=device).view(6, 5)
+    p, m, v = torch.ones(5, device=device), torch.zeros(5, device=device), torch.zeros(5, device=device)
+    c, d, s = torch.ones(5, device=device, dtype=torch.int8), torch.ones(5, device=device, dtype=torch.uint8), torch.ones(1, 2, device=device)
+    calls = [(lambda t: expert_dispatch(t * 2, plan), x), (lambda t: expert_combine(t * 2, plan), y), (lambda t: expert_sort(t + 0, 3).position, ids),
+             (lambda t: optim.adamw_step([p], [t * 2], [m], [v], step=1, lr=0.1) or p * 1, torch.ones(5, device=device)),
+             (lambda t: optim.adamw_moments(c, d, t * 1)[0], s)]
+    leaf = x.clone().requires_grad_(True)
+    out = expert_dispatch(leaf, plan)
+    calls.append((lambda t: torch.autograd.grad(out, leaf, t * 1, retain_graph=True)[0], torch.ones(6, 5, device=device)))
+    for k, (f, arg) in enumerate(calls):
+        with pytest.raises(RuntimeError, match="traced|Cannot insert a Tensor that requires grad"):      # (the latter: torch's own)
+            torch.jit.trace(f, arg, check_trace=False)
+        for mode, pre in (("real", False), ("real", True), ("fake", False), ("symbolic", False)):
+            with pytest.raises((RuntimeError, TypeError), match="traced|classes"):
+                make_fx(f, tracing_mode=mode, pre_dispatch=pre)(arg)
+        with pytest.raises((RuntimeError, TypeError), match="traced|classes"):
+            with FakeTensorMode(allow_non_fake_inputs=True):
+                f(arg)
+    assert (p == 1).all() and not m.any() and not v.any()
+    with FlopCounterMode(display=False):
+        got = [f(arg) for f, arg in calls[:3]]
+    assert all(torch.equal(a, f(arg)) for a, (f, arg) in zip(got, calls))
+    assert torch.equal(calls[5][0](calls[5][1]), torch.tensor([2.0, 1.0, 2.0], device=device)[:, None].expand(3, 5))
+
+    class Own(torch.Tensor):                                        # a class with operations of its own
+        @classmethod
+        def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+            return NotImplemented
+    own = torch.Tensor._make_subclass(Own, x)
+    for f in (lambda: expert_dispatch(own, plan), lambda: optim.adamw_step([p], [torch.Tensor._make_subclass(Own, m)], [m], [v], step=1, lr=0.1)):
+        with pytest.raises(TypeError, match="classes"):
+            f()

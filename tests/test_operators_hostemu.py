@@ -153,3 +153,7 @@ def test_routing_of_negated_views(dtype, width):
 @pytest.mark.parametrize("bits", [8, 32])
 def test_adamw_of_negated_views(bits):
     oc.check_negated_adamw(DEV, bits)
+
+
+def test_operators_are_not_traced():
+    oc.check_not_traced(DEV)
