@@ -88,8 +88,13 @@ int type_code(at::ScalarType t) {
     return t == at::kFloat ? MNE_T_F32 : t == at::kBFloat16 ? MNE_T_BF16 : t == at::kHalf ? MNE_T_F16 : -1;
 }
 
-// A tensor whose memory holds its values: one that is negated lazily (the imaginary part of a conjugate) is copied.
-at::Tensor in_memory(const at::Tensor& t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
+// A tensor whose memory holds its values: one that is negated lazily (the imaginary part of a conjugate) is copied, and one of zeros that
+// has no memory (forward-mode differentiation makes them) gets some.
+at::Tensor in_memory(const at::Tensor& t) {
+    if (t.defined() && t._is_zerotensor()) return t.clone();
+    return t.defined() && t.is_neg() ? t.resolve_neg() : t;
+}
+bool written_in_memory(const at::Tensor& t) { return !t.is_neg() && !t._is_zerotensor(); }
 
 // equal strides in every dimension that has more than one entry (the shapes are equal)
 bool laid_out_alike(const at::Tensor& a, const at::Tensor& b) {
@@ -132,9 +137,9 @@ void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& exp_
         if (g.sizes() != p.sizes() || m.sizes() != p.sizes() || v.sizes() != p.sizes())
             throw py::value_error("adamw_step: gradient and moments need their parameter's shape");
         for (const at::Tensor* t : {&p, &m, &v, small ? &(*scales)[i] : &p})
-            if (t->is_neg()) throw py::value_error("adamw_step: what is written in place must not be a negated view");
-        if (g.is_neg()) {
-            if (zero_grad) throw py::value_error("adamw_step: zero_grad cannot clear a negated view");
+            if (!written_in_memory(*t)) throw py::value_error("adamw_step: what is written in place must not be a negated view or without memory");
+        if (!written_in_memory(g)) {
+            if (zero_grad) throw py::value_error("adamw_step: zero_grad cannot clear a negated view or zeros without memory");
             g = in_memory(g);
             keep.push_back(g);
         }
@@ -340,7 +345,8 @@ void check_plan(const char* what, const at::Tensor& position, const at::Tensor& 
     if (position.scalar_type() != at::kInt || offsets.scalar_type() != at::kInt) throw py::type_error(std::string(what) + ": a plan's tensors are int32");
     if (position.dim() != 2 || position.size(1) < 1 || offsets.dim() != 1 || offsets.size(0) < 2 || !position.is_contiguous() || !offsets.is_contiguous())
         throw py::value_error(std::string(what) + ": not a plan of expert_sort");
-    if (position.is_neg() || offsets.is_neg()) throw py::value_error(std::string(what) + ": a plan's tensors must not be negated views");
+    if (!written_in_memory(position) || !written_in_memory(offsets))
+        throw py::value_error(std::string(what) + ": a plan's tensors must not be negated views or without memory");
 }
 
 at::Tensor expert_dispatch(const at::Tensor& x, const at::Tensor& position, const at::Tensor& offsets) {

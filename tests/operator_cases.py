@@ -960,3 +960,24 @@ def check_not_traced(device):
     for f in (lambda: expert_dispatch(own, plan), lambda: optim.adamw_step([p], [torch.Tensor._make_subclass(Own, m)], [m], [v], step=1, lr=0.1)):
         with pytest.raises(TypeError, match="classes"):
             f()
+
+
+def check_zeros_without_memory(device):
+    """Zeros that torch keeps without memory (as forward-mode differentiation makes them) are zeros; they cannot be written."""
+    from mneslam_amd.routing import ExpertPlan, expert_combine, expert_dispatch, expert_sort
+    zeros = lambda *shape, **kw: torch._efficientzerotensor(shape, device=device, **kw)         # noqa: E731
+    plan = expert_sort(torch.tensor([[0], [1], [0]], device=device), 2)
+    assert torch.equal(expert_dispatch(zeros(3, 4), plan), torch.zeros(3, 4, device=device))
+    assert torch.equal(expert_combine(torch.ones(3, 2, device=device), plan, zeros(3, 1)), torch.zeros(3, 2, device=device))
+    assert torch.equal(expert_combine(zeros(3, 2), plan), torch.zeros(3, 2, device=device))
+    assert expert_sort(zeros(3, 1, dtype=torch.int64), 2).offsets.tolist() == [0, 3, 3]
+    with pytest.raises(ValueError):
+        expert_dispatch(torch.ones(3, 4, device=device), ExpertPlan(plan.order, zeros(3, 1, dtype=torch.int32), plan.offsets))
+    p, m, v = torch.ones(3, device=device), torch.ones(3, device=device), torch.ones(3, device=device)
+    for lists in (([zeros(3)], [p], [m], [v]), ([p], [m.clone()], [zeros(3)], [v]), ([p], [m.clone()], [m], [zeros(3)])):
+        with pytest.raises(ValueError):
+            optim.adamw_step(*lists, step=1, lr=0.1)
+    q = [t.clone() for t in (p, m, v)]
+    optim.adamw_step([p], [zeros(3)], [m], [v], step=1, lr=0.1)
+    optim.adamw_step(q[:1], [torch.zeros(3, device=device)], q[1:2], q[2:], step=1, lr=0.1)
+    assert all(torch.equal(a, b) for a, b in zip((p, m, v), q))

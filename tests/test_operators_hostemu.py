@@ -157,3 +157,7 @@ def test_adamw_of_negated_views(bits):
 
 def test_operators_are_not_traced():
     oc.check_not_traced(DEV)
+
+
+def test_zeros_without_memory():
+    oc.check_zeros_without_memory(DEV)
