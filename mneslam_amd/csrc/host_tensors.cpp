@@ -225,12 +225,15 @@ std::vector<at::Tensor> expert_sort(const at::Tensor& given, int64_t experts) {
     return {all.narrow(0, 0, m), all.narrow(0, m, m).view({n, k}), all.narrow(0, 2 * m, experts + 1)};
 }
 
-// a row's elements next to each other (a copy where they are not)
-at::Tensor rows(const at::Tensor& given, const char* what) {
-    const at::Tensor t = in_memory(given);
+void check_rows(const at::Tensor& t, const char* what) {
     if (t.dim() != 2) throw py::value_error(std::string(what) + ": rows must be [rows, width]");
     if (type_code(t.scalar_type()) < 0)
         throw py::type_error(std::string(what) + ": " + c10::toString(t.scalar_type()) + " is not supported (float32, bfloat16, float16)");
+}
+// a row's elements next to each other (a copy where they are not)
+at::Tensor rows(const at::Tensor& given, const char* what) {
+    check_rows(given, what);
+    const at::Tensor t = in_memory(given);
     return t.stride(1) == 1 || t.size(1) <= 1 ? t : t.contiguous();
 }
 at::Tensor weights32(const at::Tensor& t) { return t.defined() ? in_memory(t).to(at::kFloat).contiguous() : t; }
@@ -354,7 +357,7 @@ at::Tensor expert_dispatch(const at::Tensor& x, const at::Tensor& position, cons
     check_plan("expert_dispatch", position, offsets);
     if (x.dim() != 2 || x.size(0) != position.size(0))
         throw py::value_error("expert_dispatch: x must be [" + std::to_string(position.size(0)) + " tokens, width]");
-    rows(x, "expert_dispatch");
+    check_rows(x, "expert_dispatch");
     return DispatchNode::apply(x, position, offsets);
 }
 
@@ -368,7 +371,7 @@ at::Tensor expert_combine(const at::Tensor& y, const at::Tensor& position, const
         if (w.sizes() != position.sizes()) throw py::value_error("expert_combine: weights must be [tokens, choices]");
         if (type_code(w.scalar_type()) < 0) throw py::type_error("expert_combine: weights must be float32, bfloat16 or float16");
     }
-    rows(y, "expert_combine");
+    check_rows(y, "expert_combine");
     return CombineNode::apply(y, position, offsets, w.defined() ? w : position, w.defined());
 }
 

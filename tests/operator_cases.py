@@ -981,3 +981,22 @@ def check_zeros_without_memory(device):
     optim.adamw_step([p], [zeros(3)], [m], [v], step=1, lr=0.1)
     optim.adamw_step(q[:1], [torch.zeros(3, device=device)], q[1:2], q[2:], step=1, lr=0.1)
     assert all(torch.equal(a, b) for a, b in zip((p, m, v), q))
+
+
+def check_rows_copied_once(device):
+    """Rows whose elements do not lie next to each other are copied once, the others never."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+    from mneslam_amd.routing import expert_combine, expert_dispatch, expert_sort
+
+    class Copies(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.count = getattr(self, "count", 0) + (func in (torch.ops.aten.clone.default, torch.ops.aten.copy_.default))
+            return func(*args, **(kwargs or {}))
+
+    plan = expert_sort(torch.tensor([[0, 1], [1, 0]], device=device), 2)
+    for f, n in ((lambda t: expert_dispatch(t, plan), 2), (lambda t: expert_combine(t, plan), 4)):
+        t = torch.arange(3.0 * n, device=device).view(n, 3)
+        for given, want in ((t, 0), (t.t().contiguous().t(), 1)):
+            with Copies() as seen:
+                got = f(given)
+            assert torch.equal(got, f(t)) and seen.count == want

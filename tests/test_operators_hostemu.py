@@ -161,3 +161,7 @@ def test_operators_are_not_traced():
 
 def test_zeros_without_memory():
     oc.check_zeros_without_memory(DEV)
+
+
+def test_rows_are_copied_once():
+    oc.check_rows_copied_once(DEV)
