@@ -430,9 +430,12 @@ __global__ __launch_bounds__(EX_THREADS) void expert_combine_backward_kernel(Exp
                         const int c = c0 + u * group, twice = c * Col::N - Col::start(c, a.width);     // elements that the column before has
 #pragma unroll
                         for (int j = 0; j < Col::N; ++j) {
-                            const float x = j >= twice ? d[u].get(j) : 0.0f;
+                            const float x = d[u].get(j);
 #pragma unroll
-                            for (int i = 0; i < K; ++i) dot[i] = fmaf(x, y[i][u].get(j), dot[i]);
+                            for (int i = 0; i < K; ++i) {           // (left out, not multiplied by zero: y may be infinite there)
+                                const float more = fmaf(x, y[i][u].get(j), dot[i]);
+                                dot[i] = j >= twice ? more : dot[i];
+                            }
                         }
                     }
                 }

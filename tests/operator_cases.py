@@ -1000,3 +1000,24 @@ def check_rows_copied_once(device):
             with Copies() as seen:
                 got = f(given)
             assert torch.equal(got, f(t)) and seen.count == want
+
+
+def check_infinite_rows(device, dtype):
+    """A row with one infinite element: the gradient of its weight is infinite wherever the element is, the others are what they are."""
+    from mneslam_amd.routing import expert_combine, expert_sort
+    dt = NAMES[dtype]
+    for width in (1, 3, 4, 5, 8, 9, 13, 21):
+        for k in (1, 2, 3):
+            plan = expert_sort(torch.zeros(width, k, dtype=torch.int32, device=device), 1)          # token t's element t is the infinite one
+            y = torch.ones(width * k, width, device=device, dtype=dt)
+            y[plan.position[:, 0].long(), torch.arange(width, device=device)] = float("inf")
+            w = torch.ones(width, k, device=device, requires_grad=True)
+            (dw,) = torch.autograd.grad(expert_combine(y, plan, w), w, torch.ones(width, width, device=device, dtype=dt))
+            want = torch.full((width, k), float(width))
+            want[:, 0] = float("inf")
+            assert torch.equal(dw.cpu(), want), (width, k)
+            # ... and of the incoming gradient's element
+            g = torch.ones(width, width, device=device, dtype=dt)
+            g.fill_diagonal_(float("inf"))
+            (dw,) = torch.autograd.grad(expert_combine(torch.ones_like(y), plan, w), w, g)
+            assert torch.isposinf(dw).all(), (width, k)

@@ -374,3 +374,8 @@ def test_zeros_without_memory():
 
 def test_rows_are_copied_once():
     oc.check_rows_copied_once(DEV)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_expert_rows_infinite(dtype):
+    oc.check_infinite_rows(DEV, dtype)
