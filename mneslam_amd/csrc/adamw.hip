@@ -206,14 +206,15 @@ __device__ __forceinline__ void adamw8_body(const Adamw8Args& a, const AdamwHype
 #pragma unroll
                 for (int j = 0; j < N; ++j) r[k][j] = mne_sqrt_rn(r[k][j]);
         }
-        const float inv = 1.0f / h.root_bc2;
+        // (a reciprocal is enough here: nothing of the parameter enters the codes.  It takes a number below 2^-126, which eps may be where
+        // there has been no gradient, for zero: the quotient is formed 2^24 too small)
+        const float up = 16777216.0f, inv = up / h.root_bc2, eps = up * h.eps, size = up * h.step_size;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             const long long i = i0 + k * (LANES * N);
 #pragma unroll
             for (int j = 0; j < N; ++j) {
-                // (a reciprocal is enough here: nothing of the parameter enters the codes)
-                p[k][j] = fmaf(-h.step_size, m[k][j] * mne_rcp_fast(fmaf(r[k][j], inv, h.eps)), p[k][j] * h.decay);
+                p[k][j] = fmaf(-size, m[k][j] * mne_rcp_fast(fmaf(r[k][j], inv, eps)), p[k][j] * h.decay);
                 g[k][j] = 0.0f;
             }
             aw_store<PT, N, FULL, PAST>(p[k], a.p[s], i, n);

@@ -1021,3 +1021,23 @@ def check_infinite_rows(device, dtype):
             g.fill_diagonal_(float("inf"))
             (dw,) = torch.autograd.grad(expert_combine(torch.ones_like(y), plan, w), w, g)
             assert torch.isposinf(dw).all(), (width, k)
+
+
+def check_adamw_tiny_eps(device, ptype, bits):
+    """An eps below fp32's normal range: what has no gradient stays where it is, and the others step by lr."""
+    for eps in (1e-37, 1e-38, 1e-40, 1e-44):
+        p, g = torch.ones(600, device=device, dtype=NAMES[ptype]), torch.zeros(600, device=device, dtype=NAMES[ptype])
+        g[300:] = 0.5
+        _step([p], [g], bits, device, eps=eps, lr=0.25)
+        assert (p[:300] == 1).all() and (p[300:] == 0.75).all(), eps
+
+
+def check_adamw8_quotient(device):
+    """The update of a float32 parameter is one rounded quotient also with 8-bit moments: with beta = 0, lr = 1 and g = 1 nothing else of
+    the step rounds, and p = -1 / (1 + eps)."""
+    for j in range(1, 60):
+        eps = float(np.float32(j / 61))
+        p, g = torch.zeros(300, device=device), torch.ones(300, device=device)
+        _step([p], [g], 8, device, betas=(0.0, 0.0), lr=1.0, eps=eps)
+        want = -np.float32(1) / (np.float32(1) + np.float32(eps))
+        assert (p.cpu().numpy() == want).all(), (j, float(p[0]), float(want))

@@ -379,3 +379,9 @@ def test_rows_are_copied_once():
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 def test_expert_rows_infinite(dtype):
     oc.check_infinite_rows(DEV, dtype)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("ptype", ["f32", "bf16", "f16"])
+def test_adamw_tiny_eps(ptype, bits):
+    oc.check_adamw_tiny_eps(DEV, ptype, bits)
