@@ -206,15 +206,22 @@ __device__ __forceinline__ void adamw8_body(const Adamw8Args& a, const AdamwHype
 #pragma unroll
                 for (int j = 0; j < N; ++j) r[k][j] = mne_sqrt_rn(r[k][j]);
         }
-        // (a reciprocal is enough here: nothing of the parameter enters the codes.  It takes a number below 2^-126, which eps may be where
-        // there has been no gradient, for zero: the quotient is formed 2^24 too small)
+        // The quotient: a reciprocal 1 ulp off, and for a 32-bit parameter one correction, which leaves a rounded quotient (a 16-bit one is
+        // rounded at 2^-9 or 2^-12 anyway, and its step is bound by instructions).  The reciprocal takes a number below 2^-126, which eps may
+        // be where there has been no gradient, for zero: the quotient is formed 2^24 too small.
         const float up = 16777216.0f, inv = up / h.root_bc2, eps = up * h.eps, size = up * h.step_size;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             const long long i = i0 + k * (LANES * N);
 #pragma unroll
             for (int j = 0; j < N; ++j) {
-                p[k][j] = fmaf(-size, m[k][j] * mne_rcp_fast(fmaf(r[k][j], inv, eps)), p[k][j] * h.decay);
+                const float d = fmaf(r[k][j], inv, eps), y = mne_rcp_fast(d);
+                float q = m[k][j] * y;
+                if (PT == MNE_T_F32) {
+                    const float off = fmaf(-d, q, m[k][j]);
+                    q = off == off ? fmaf(off, y, q) : q;          // (not where d is infinite: the quotient is 0)
+                }
+                p[k][j] = fmaf(-size, q, p[k][j] * h.decay);
                 g[k][j] = 0.0f;
             }
             aw_store<PT, N, FULL, PAST>(p[k], a.p[s], i, n);

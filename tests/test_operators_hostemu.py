@@ -176,3 +176,7 @@ def test_expert_rows_infinite(dtype):
 @pytest.mark.parametrize("ptype", ["f32", "bf16", "f16"])
 def test_adamw_tiny_eps(ptype, bits):
     oc.check_adamw_tiny_eps(DEV, ptype, bits)
+
+
+def test_adamw_8_quotient():
+    oc.check_adamw8_quotient(DEV)
