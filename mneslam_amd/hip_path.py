@@ -10,7 +10,7 @@ import ctypes as C
 
 import torch
 
-from . import _lib
+from . import _lib, plane_sums
 
 
 # --------------------------------------------------------------------------------------------------
@@ -216,12 +216,8 @@ class RenderFunction(torch.autograd.Function):
                 if p.dtype == torch.float16:
                     # autograd wants the parameter's dtype; the fp32 sums are kept beside it for the optimizer (FusedAdam reads
                     # ``grad32``, accumulated over backward calls like .grad, cleared by zero_grad): a cast to fp16 flushes a
-                    # mean-reduced plane gradient to zero below ~3e-8 (ADVICE r04)
-                    acc = getattr(p, "grad32", None)
-                    if acc is None or acc.shape != g.shape or acc.device != g.device:
-                        p.grad32 = g.clone()
-                    else:
-                        acc.add_(g)
+                    # mean-reduced plane gradient to zero below ~3e-8
+                    plane_sums.add(p, g)
         return (None, None, d_o if ctx.needs_input_grad[2] else None, d_d if ctx.needs_input_grad[3] else None,
                 None, None, None, None,
                 *([g if g.dtype == p.dtype else g.to(p.dtype) for g, p in zip(grads, planes)] if grads is not None else [None] * n_planes),

@@ -11,7 +11,7 @@ import ctypes as C
 
 import torch
 
-from . import _lib
+from . import _lib, plane_sums
 
 
 def _dense_like(p, t):
@@ -45,8 +45,8 @@ class FusedAdam(torch.optim.Optimizer):
         for group in self.param_groups:
             b1, b2 = group["betas"]
             for p in group["params"]:
-                if p.grad is None and getattr(p, "grad32", None) is not None:
-                    p.grad32 = None              # .grad was dropped by someone else's zero_grad: the fp32 sum beside it is stale
+                if p.grad is None:
+                    plane_sums.drop(p)           # .grad was dropped by someone else's zero_grad: the fp32 sum beside it is stale
                 g = p.grad if zero_grad_buffers is None else zero_grad_buffers.get(p)   # explicit map: only those params
                 if g is None:
                     continue
@@ -108,8 +108,7 @@ class FusedAdam(torch.optim.Optimizer):
     def zero_grad(self, set_to_none=True):
         for group in self.param_groups:
             for p in group["params"]:
-                if getattr(p, "grad32", None) is not None:
-                    p.grad32 = None                      # the fp32 gradient sum of a half-precision plane (see ``segments``)
+                plane_sums.drop(p)                       # the fp32 gradient sum of a half-precision plane (see ``segments``)
         return super().zero_grad(set_to_none=set_to_none)
 
 
@@ -170,7 +169,10 @@ def adamw_moments(exp_avg, exp_avg_sq, scales):
 class FusedAdamW(torch.optim.Optimizer):
     """torch.optim.AdamW (amsgrad=False, maximize=False) whose ``step()`` is ``adamw_step``: one launch for up to 80 tensors of a
     group that are at the same step count.  ``state_bits`` 8 (also per group) holds the moments in 8 bits with two scales for each 256
-    elements -- 2.06 bytes an element instead of 8; ``moments(p)`` gives them in fp32.  ``seed`` is that of the codes' dither."""
+    elements -- 2.06 bytes an element instead of 8; ``moments(p)`` gives them in fp32.  ``seed`` is that of the codes' dither.
+
+    The gradient is ``.grad``.  That of a half-precision plane is taken in fp32, before its rounding, wherever it is still what the render
+    node's backward pass left; where it was changed since (clipped, unscaled, added to) it is taken as it is, in its own type."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, seed=0):
         if not 0 <= int(seed) < 1 << 32:
@@ -217,13 +219,11 @@ class FusedAdamW(torch.optim.Optimizer):
             for p in group["params"]:
                 ordinal += 1
                 if p.grad is None:
-                    if getattr(p, "grad32", None) is not None:
-                        p.grad32 = None                 # .grad was dropped by someone else: the fp32 sum beside it is stale
+                    plane_sums.drop(p)                  # .grad was dropped by someone else: the fp32 sum beside it is stale
                     continue
                 if p.grad.is_sparse:
                     raise RuntimeError("FusedAdamW does not support sparse gradients")
-                # a half-precision plane: the render node leaves the fp32 sum beside the rounded gradient
-                g = p.grad32 if getattr(p, "grad32", None) is not None else p.grad
+                g = plane_sums.gradient(p)              # (a half-precision plane: the fp32 sum that .grad is the rounding of)
                 st = self._state(p, group["state_bits"])
                 batches.setdefault((p.device, st["step"] + 1), []).append((p, g, st, ordinal - 1))
             for (_, step), batch in batches.items():
@@ -236,9 +236,9 @@ class FusedAdamW(torch.optim.Optimizer):
                     for s in sts:
                         s["step"] = step
                 if zero_grad:
-                    for p, g in zip(ps, gs):
-                        if g is not p.grad:
-                            p.grad.zero_()
+                    for p in ps:
+                        if getattr(p, "grad32", None) is not None:
+                            plane_sums.zero(p)
         return loss
 
     def moments(self, p):
@@ -271,6 +271,5 @@ class FusedAdamW(torch.optim.Optimizer):
     def zero_grad(self, set_to_none=True):
         for group in self.param_groups:
             for p in group["params"]:
-                if getattr(p, "grad32", None) is not None:
-                    p.grad32 = None                      # the fp32 gradient sum of a half-precision plane
+                plane_sums.drop(p)
         return super().zero_grad(set_to_none=set_to_none)

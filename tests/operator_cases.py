@@ -1041,3 +1041,122 @@ def check_adamw8_quotient(device):
         _step([p], [g], 8, device, betas=(0.0, 0.0), lr=1.0, eps=eps)
         want = -np.float32(1) / (np.float32(1) + np.float32(eps))
         assert (p.cpu().numpy() == want).all(), (j, float(p[0]), float(want))
+
+
+# ------------------------------------------------------------------------------------------ the fp32 sums beside half-precision planes
+class _RenderLike(torch.autograd.Function):
+    """What the render node does for a half-precision plane: the fp32 gradient beside, its rounding to autograd."""
+
+    @staticmethod
+    def forward(ctx, p, g32):
+        ctx.p, ctx.g32 = p, g32
+        return p.float().sum()
+
+    @staticmethod
+    def backward(ctx, g):
+        from mneslam_amd import plane_sums
+        plane_sums.add(ctx.p, ctx.g32 * g)
+        return (ctx.g32 * g).half(), None
+
+
+def check_plane_gradients(device):
+    """FusedAdamW takes a half-precision plane's gradient in fp32 while ``.grad`` is its rounding, and ``.grad`` itself wherever that is
+    another: clipped, added to by another node, dropped and filled again, asked for without being accumulated."""
+    tiny = torch.tensor([1e-9, -3e-9, 0.3, 2.0 ** -12 * 1.0003], device=device)        # two of them round to zero in fp16
+    render = lambda p, s=1.0: _RenderLike.apply(p, tiny * s)                           # noqa: E731
+
+    def moved(grads, **kw):
+        """Where a zero parameter goes with beta = 0 after the gradients that ``grads(p)`` leaves: the moment is the gradient."""
+        p = torch.nn.Parameter(torch.zeros(4, device=device, dtype=torch.float16))
+        opt = optim.FusedAdamW([p], betas=(0.0, 0.0), weight_decay=0.0)
+        grads(p, opt)
+        opt.step(**kw)
+        return opt.moments(p)[0], p, opt
+
+    g, p, opt = moved(lambda p, _: render(p).backward())
+    assert torch.equal(g, tiny)                                                        # not rounded
+    opt.step()
+    assert torch.equal(opt.moments(p)[0], tiny)
+
+    def clipped(p, _):
+        render(p).backward()
+        torch.nn.utils.clip_grad_norm_([p], 1e-3)
+    g, p, _ = moved(clipped)
+    assert torch.equal(g, p.grad.float()) and float(g.norm()) < 1.01e-3
+    assert torch.equal(moved(lambda p, _: (render(p).backward(), p.grad.neg_()))[0], -tiny.half().float())
+    assert torch.equal(moved(lambda p, _: (render(p).backward(), setattr(p, "grad", p.grad * 4)))[0], 4 * tiny.half().float())
+
+    more = torch.tensor([0.0, 1.0, 1.0, 0.0], device=device)                           # another source, in the same pass and in its own
+    want = torch.where(more == 0, tiny, (tiny.half() + more.half()).float())
+    assert torch.equal(moved(lambda p, _: (render(p) + (p * more.half()).sum()).backward())[0], want)
+    assert torch.equal(moved(lambda p, _: (render(p).backward(), (p * more.half()).sum().backward()))[0], want)
+    assert torch.equal(moved(lambda p, _: ((p * more.half()).sum().backward(), render(p).backward()))[0], want)
+
+    def refilled(p, _):
+        render(p).backward()
+        p.grad = None
+        (p * torch.zeros_like(p)).sum().backward()
+    assert not moved(refilled)[0].any()                                                # the old sum is nobody's
+
+    def dropped(p, _):
+        render(p, 7.0).backward()
+        p.grad = None
+        render(p).backward()
+    assert torch.equal(moved(dropped)[0], tiny)                                        # nor is it added to
+
+    def asked(p, _):
+        torch.autograd.grad(render(p, 5.0), p)
+        render(p).backward()
+    assert torch.equal(moved(asked)[0], tiny)
+
+    def asked_after(p, _):
+        render(p).backward()
+        torch.autograd.grad(render(p, 5.0), p)
+    assert torch.equal(moved(asked_after)[0], tiny.half().float())
+
+    # added up over two passes and in one, cleared by the step, by the optimizer and by somebody else
+    twice = torch.where((tiny.half() * 2) == (tiny * 2).half(), tiny * 2, (tiny.half() * 2).float())
+    assert torch.equal(moved(lambda p, _: (render(p).backward(), render(p).backward()))[0], twice)
+    assert torch.equal(moved(lambda p, _: (render(p) + render(p)).backward())[0], twice)
+    for clear in (lambda p, opt: opt.step(zero_grad=True), lambda p, opt: opt.zero_grad(), lambda p, opt: opt.zero_grad(set_to_none=False),
+                  lambda p, opt: setattr(p, "grad", None)):
+        def cleared(p, opt):
+            render(p, 3.0).backward()
+            clear(p, opt)
+            assert p.grad is None or not p.grad.any()
+            render(p).backward()
+        assert torch.equal(moved(cleared)[0], tiny)
+
+    def cleared_beside(p, _):
+        render(p, 3.0).backward()
+        p.grad.zero_()
+        render(p).backward()
+    assert torch.equal(moved(cleared_beside)[0], tiny.half().float())
+
+
+def check_plane_gradients_rendered(device):
+    """The same with the render node itself: FusedAdamW's first moments of the planes are the fp32 sums, or what clipping left of ``.grad``."""
+    import parity_cases as pc
+    from helpers import load_golden
+    from mneslam_amd import configs, slam_glue
+    g = load_golden("fwd_onegrid")
+    for clip in (False, True):
+        cfg = configs.small_test_config(**pc.FWD_CASES["fwd_onegrid"])
+        m = pc.model_from_golden(g, cfg, device).train()
+        for lst in m.all_planes:
+            for k in range(len(lst)):
+                lst[k] = lst[k].half()
+        opt = slam_glue.create_optimizer(m, cfg, optimizer_cls=optim.FusedAdamW)
+        rays_o, rays_d, rgb, d, U = pc.to_dev(pc.fixture_inputs(g), device)
+        losses = m._render(rays_o, rays_d, rgb, d, u=U)[-1]
+        slam_glue.get_loss_from_ret(cfg, {k: losses[i] for i, k in enumerate(pc.LOSS_KEYS)}, is_co_sdf=False).backward()
+        planes = [p for lst in m.all_planes for p in lst]
+        sums = [p.grad32.clone() for p in planes]
+        assert all(torch.equal(s.half(), p.grad) for s, p in zip(sums, planes)) and any(s.any() for s in sums)
+        if clip:
+            torch.nn.utils.clip_grad_value_(planes, 1e-6)
+        opt.step()
+        for s, p in zip(sums, planes):
+            want = _as_param(p.grad.float() if clip else s, p)
+            m1 = opt.moments(p)[0]
+            assert (m1 - 0.1 * want).abs().max() <= 2 * EPS32 * 0.1 * want.abs().max()

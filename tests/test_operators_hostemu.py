@@ -180,3 +180,11 @@ def test_adamw_tiny_eps(ptype, bits):
 
 def test_adamw_8_quotient():
     oc.check_adamw8_quotient(DEV)
+
+
+def test_plane_gradients():
+    oc.check_plane_gradients(DEV)
+
+
+def test_plane_gradients_rendered():
+    oc.check_plane_gradients_rendered(DEV)
