@@ -1160,3 +1160,45 @@ def check_plane_gradients_rendered(device):
             want = _as_param(p.grad.float() if clip else s, p)
             m1 = opt.moments(p)[0]
             assert (m1 - 0.1 * want).abs().max() <= 2 * EPS32 * 0.1 * want.abs().max()
+
+
+class _FlatMap:
+    """A map that answers one value everywhere."""
+
+    def __init__(self, box, value):
+        self.bounding_box, self.value = torch.tensor(box, dtype=torch.float64), value
+
+    def query_color_sdf(self, points):
+        return torch.full((len(points), 4), self.value, device=points.device)
+
+
+def check_agent_maps_have_no_seam(device):
+    """Three boxes and more over one place: the answer is continuous where one map takes another's place among the deepest."""
+    from mneslam_amd.model.agent_maps import AgentMaps
+    wide = [[-4.0, 4.0], [-4.0, 4.0]]
+    three = [_FlatMap([[-5.0, 5.0], *wide], 0.0), _FlatMap([[-3.0, 2.0], *wide], 1.0), _FlatMap([[-2.0, 3.0], *wide], -1.0)]
+    four = three + [_FlatMap([[-4.0, 2.5], [-4.5, 5.0], [-3.0, 3.0]], 3.0)]
+    for maps, tops in ((three, (2, 3)), (four, (2, 3, 4))):
+        for top in tops:
+            union = AgentMaps(maps, top=top)
+            # along lines through the place, away from where top + 1 maps are equally deep at once
+            x = torch.linspace(-4.5, 4.5, 9001, dtype=torch.float64, device=device)
+            for y, z in ((0.3, -0.2), (-1.1, 0.7)):
+                p = torch.stack([x, torch.full_like(x, y), torch.full_like(x, z)], 1)
+                got = union.query_sdf(p).double()
+                # a depth changes by at most the step, 1e-3; the weights' sum is the depth of the deepest map above that of the one left
+                # out, at the least
+                depth = torch.stack([torch.minimum(p - m.bounding_box[:, 0].to(device), m.bounding_box[:, 1].to(device) - p).amin(1) for m in maps], 1)
+                ranked = depth.clamp(min=0).sort(1, descending=True).values
+                margin = ranked[:, 0] - (ranked[:, top] if top < len(maps) else 0.0)
+                clear = torch.minimum(margin[1:], margin[:-1])
+                jump = (got[1:] - got[:-1]).abs()
+                # (a quotient of sums of `top` weights, each changing by 2e-3 at most, of values that are 4 apart at most; fp32; the 1e-6
+                # share of a box that a map keeps at its edge)
+                assert (jump <= 4 * 2 * top * 2e-3 / clear.clamp(min=1e-9) + 1e-5 / clear.clamp(min=1e-9) + 1e-5).all(), (top, float(jump.max()))
+    union = AgentMaps(three)
+    at = lambda v: float(union.query_sdf(torch.tensor([[v, 0.0, 0.0]], device=device)))          # noqa: E731
+    assert abs(at(-1e-3)) < 1e-2 and abs(at(1e-3)) < 1e-2
+    ids, w = union.route(torch.tensor([[1.0, 0.0, 0.0], [4.9, 0.0, 0.0], [2.5, 0.0, 0.0]], device=device))
+    # depths 4, 1, 2 (0.1 and none; 2.5, none and 0.5): the third is left out at depth 1
+    assert ids.tolist() == [[0, 2], [0, -1], [0, 2]] and torch.allclose(w.cpu(), torch.tensor([[0.75, 0.25], [1.0, 0.0], [2.5 / 3, 0.5 / 3]]), atol=1e-5)

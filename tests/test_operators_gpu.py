@@ -397,3 +397,7 @@ def test_plane_gradients():
 
 def test_plane_gradients_rendered():
     oc.check_plane_gradients_rendered(DEV)
+
+
+def test_agent_maps_have_no_seam():
+    oc.check_agent_maps_have_no_seam(DEV)
