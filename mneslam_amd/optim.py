@@ -166,6 +166,22 @@ def adamw_moments(exp_avg, exp_avg_sq, scales):
     return tuple(_lib.host_tensors().adamw_moments(exp_avg, exp_avg_sq, scales))
 
 
+def _check_saved(p, st):
+    """``st``: a saved entry of FusedAdamW or torch.optim.AdamW for a parameter like ``p``."""
+    if any(not torch.is_tensor(st.get(key)) or st[key].shape != p.shape for key in ("exp_avg", "exp_avg_sq")) or "step" not in st:
+        raise ValueError(f"the saved state of a parameter of shape {tuple(p.shape)} is none, or has another shape")
+    types = st["exp_avg"].dtype, st["exp_avg_sq"].dtype
+    if all(t.is_floating_point for t in types):
+        return
+    if types != (torch.int8, torch.uint8):
+        raise ValueError(f"moments are floating-point numbers, or int8 and uint8 codes, not {types}")
+    scales = st.get("scales")
+    if not torch.is_tensor(scales) or not scales.is_floating_point() or scales.shape != (-(-p.numel() // MOMENT_BLOCK), 2):
+        raise ValueError("8-bit moments without scales for their blocks")
+    if any(n > 1 and a != b for key in ("exp_avg", "exp_avg_sq") for n, a, b in zip(p.shape, p.stride(), st[key].stride())):
+        raise ValueError("8-bit moments of a parameter that was laid out otherwise: its blocks are others")
+
+
 class FusedAdamW(torch.optim.Optimizer):
     """torch.optim.AdamW (amsgrad=False, maximize=False) whose ``step()`` is ``adamw_step``: one launch for up to 80 tensors of a
     group that are at the same step count.  ``state_bits`` 8 (also per group) holds the moments in 8 bits with two scales for each 256
@@ -250,23 +266,39 @@ class FusedAdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """Also of torch.optim.AdamW's states (not with amsgrad or maximize).  The base class casts floating-point state to its
-        parameter's type: here moments and scales are float32 or the codes they were saved as, laid out like their parameter."""
-        for group in state_dict["param_groups"]:
-            for rule in ("amsgrad", "maximize"):
-                if group.get(rule):
-                    raise ValueError(f"FusedAdamW has no {rule}: the loaded state would go on by another rule")
-        super().load_state_dict(state_dict)
-        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
-        for i, p in zip(saved, (p for g in self.param_groups for p in g["params"])):
-            for key, value in state_dict["state"].get(i, {}).items():
+        parameter's type: here moments and scales are float32 or the codes they were saved as, laid out like their parameter.  A state that
+        does not fit is refused before anything is loaded."""
+        seen = []
+
+        def check(_, state_dict):                        # (behind the hooks that may change it)
+            for group in state_dict["param_groups"]:
+                for rule in ("amsgrad", "maximize"):
+                    if group.get(rule):
+                        raise ValueError(f"FusedAdamW has no {rule}: the loaded state would go on by another rule")
+            for p, st in self._saved_states(state_dict):
+                _check_saved(p, st)
+            seen.append(state_dict)
+
+        hook = self.register_load_state_dict_pre_hook(check)
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            hook.remove()
+        for p, st in self._saved_states(seen[0]):
+            for key, value in st.items():
                 if key == "step":
                     self.state[p][key] = int(value)
                 elif key in ("exp_avg", "exp_avg_sq", "scales"):
                     like = value if key == "scales" else p
-                    if not value.is_floating_point() and any(n > 1 and a != b for n, a, b in zip(p.shape, p.stride(), value.stride())):
-                        raise ValueError("8-bit moments of a parameter that was laid out otherwise: its blocks are others")
                     dtype = torch.float32 if value.is_floating_point() else value.dtype
                     self.state[p][key] = torch.empty_like(like, dtype=dtype, device=p.device, requires_grad=False).copy_(value)
+
+    def _saved_states(self, state_dict):
+        """(parameter, its entry of ``state_dict``) of those that have one, as far as the groups are alike (the base class checks that)."""
+        for group, saved in zip(self.param_groups, state_dict["param_groups"]):
+            for p, i in zip(group["params"], saved["params"]):
+                if state_dict["state"].get(i):
+                    yield p, state_dict["state"][i]
 
     def zero_grad(self, set_to_none=True):
         for group in self.param_groups:

@@ -1202,3 +1202,51 @@ def check_agent_maps_have_no_seam(device):
     ids, w = union.route(torch.tensor([[1.0, 0.0, 0.0], [4.9, 0.0, 0.0], [2.5, 0.0, 0.0]], device=device))
     # depths 4, 1, 2 (0.1 and none; 2.5, none and 0.5): the third is left out at depth 1
     assert ids.tolist() == [[0, 2], [0, -1], [0, 2]] and torch.allclose(w.cpu(), torch.tensor([[0.75, 0.25], [1.0, 0.0], [2.5 / 3, 0.5 / 3]]), atol=1e-5)
+
+
+# --------------------------------------------------------------------------------------------------- FusedAdamW: loaded states
+def _stepped(p, **kw):
+    opt = optim.FusedAdamW([p], **kw)
+    p.grad = torch.ones_like(p)
+    opt.step()
+    return opt
+
+
+def check_fused_adamw_loads_all_or_nothing(device):
+    """A saved state that does not fit is refused, and the optimizer goes on as if nothing had been asked."""
+    shape = (6, 5, 3, 4)
+    p = torch.nn.Parameter(torch.ones(shape, device=device))
+    good = {bits: _stepped(p, lr=0.5, state_bits=bits).state_dict() for bits in (8, 32)}
+
+    def changed(bits, **kw):
+        saved = {"param_groups": good[bits]["param_groups"], "state": {0: {**good[bits]["state"][0], **kw}}}
+        return {**saved, "state": {0: {k: v for k, v in saved["state"][0].items() if v is not None}}}
+
+    st = good[8]["state"][0]
+    other_order = st["exp_avg"].contiguous(memory_format=torch.channels_last)
+    bad = [changed(8, exp_avg=other_order, exp_avg_sq=other_order.to(torch.uint8)), changed(8, scales=st["scales"][:1]), changed(8, scales=None),
+           changed(8, scales=st["scales"].to(torch.int32)), changed(8, exp_avg_sq=st["exp_avg"]), changed(8, exp_avg=st["exp_avg"].float()),
+           changed(32, exp_avg=torch.ones(4, device=device)), changed(32, exp_avg_sq=torch.ones(1, 5, 3, 4, device=device)), changed(32, exp_avg=None),
+           changed(32, step=None), changed(32, exp_avg=1.0)]
+    for saved in bad:
+        for bits in (8, 32):
+            q = torch.nn.Parameter(torch.ones(shape, device=device))
+            opt = _stepped(q, lr=0.25, state_bits=bits)
+            before = {k: v.clone() if torch.is_tensor(v) else v for k, v in opt.state[q].items()}
+            with pytest.raises(ValueError):
+                opt.load_state_dict(saved)
+            assert opt.param_groups[0]["lr"] == 0.25 and opt.param_groups[0]["state_bits"] == bits
+            for k, v in before.items():
+                assert torch.equal(opt.state[q][k], v) and opt.state[q][k].dtype == v.dtype if torch.is_tensor(v) else opt.state[q][k] == v
+            opt.step()
+    for bits in (8, 32):                                  # what fits is loaded, also through a hook that changes it
+        q = torch.nn.Parameter(torch.ones(shape, device=device))
+        opt = optim.FusedAdamW([q])
+        hook = opt.register_load_state_dict_pre_hook(lambda _, sd: {**sd, "state": {0: {**sd["state"][0], "step": 7}}})
+        opt.load_state_dict(good[bits])
+        hook.remove()
+        assert opt.state[q]["step"] == 7 and torch.equal(opt.state[q]["exp_avg"], good[bits]["state"][0]["exp_avg"])
+        opt.load_state_dict(good[bits])
+        assert opt.state[q]["step"] == 1
+    empty = optim.FusedAdamW([torch.nn.Parameter(torch.zeros(0, 3, device=device))])
+    empty.load_state_dict(empty.state_dict())

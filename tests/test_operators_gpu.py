@@ -401,3 +401,7 @@ def test_plane_gradients_rendered():
 
 def test_agent_maps_have_no_seam():
     oc.check_agent_maps_have_no_seam(DEV)
+
+
+def test_fused_adamw_loads_all_or_nothing():
+    oc.check_fused_adamw_loads_all_or_nothing(DEV)
