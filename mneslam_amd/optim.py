@@ -166,8 +166,24 @@ def adamw_moments(exp_avg, exp_avg_sq, scales):
     return tuple(_lib.host_tensors().adamw_moments(exp_avg, exp_avg_sq, scales))
 
 
+def _check_rule(group):
+    """``group``: a saved group of FusedAdamW, or of an optimizer that goes on by the same rule."""
+    for rule in ("amsgrad", "maximize"):
+        if group.get(rule):
+            raise ValueError(f"FusedAdamW has no {rule}: the loaded state would go on by another rule")
+    if "state_bits" in group:
+        return
+    if any(key not in group for key in ("lr", "betas", "eps", "weight_decay")) or ("decoupled_weight_decay" in group and "amsgrad" not in group):
+        raise ValueError("the saved state is none of AdamW: it would go on by another rule")
+    # torch.optim.Adam says that its decay is folded into the gradient; FusedAdam's groups have the four entries above alone
+    if group["weight_decay"] and not group.get("decoupled_weight_decay", "amsgrad" in group):
+        raise ValueError("the saved state is Adam's, with a decay that is folded into the gradient: it would go on by another rule")
+
+
 def _check_saved(p, st):
     """``st``: a saved entry of FusedAdamW or torch.optim.AdamW for a parameter like ``p``."""
+    if not st.keys() <= {"step", "exp_avg", "exp_avg_sq", "scales"}:
+        raise ValueError(f"the saved state is none of AdamW: it has {sorted(st)}")
     if any(not torch.is_tensor(st.get(key)) or st[key].shape != p.shape for key in ("exp_avg", "exp_avg_sq")) or "step" not in st:
         raise ValueError(f"the saved state of a parameter of shape {tuple(p.shape)} is none, or has another shape")
     types = st["exp_avg"].dtype, st["exp_avg_sq"].dtype
@@ -265,16 +281,14 @@ class FusedAdamW(torch.optim.Optimizer):
         return adamw_moments(st["exp_avg"], st["exp_avg_sq"], st["scales"]) if "scales" in st else (st["exp_avg"], st["exp_avg_sq"])
 
     def load_state_dict(self, state_dict):
-        """Also of torch.optim.AdamW's states (not with amsgrad or maximize).  The base class casts floating-point state to its
+        """Also of torch.optim.AdamW's states (not with amsgrad or maximize), and of Adam's without weight decay.  The base class casts floating-point state to its
         parameter's type: here moments and scales are float32 or the codes they were saved as, laid out like their parameter.  A state that
         does not fit is refused before anything is loaded."""
         seen = []
 
         def check(_, state_dict):                        # (behind the hooks that may change it)
             for group in state_dict["param_groups"]:
-                for rule in ("amsgrad", "maximize"):
-                    if group.get(rule):
-                        raise ValueError(f"FusedAdamW has no {rule}: the loaded state would go on by another rule")
+                _check_rule(group)
             for p, st in self._saved_states(state_dict):
                 _check_saved(p, st)
             seen.append(state_dict)

@@ -1250,3 +1250,34 @@ def check_fused_adamw_loads_all_or_nothing(device):
         assert opt.state[q]["step"] == 1
     empty = optim.FusedAdamW([torch.nn.Parameter(torch.zeros(0, 3, device=device))])
     empty.load_state_dict(empty.state_dict())
+
+
+def check_fused_adamw_loads_no_other_decay(device):
+    """States of optimizers that go on by another rule are refused, those that go on by the same are loaded."""
+    def other(cls, **kw):
+        p = torch.nn.Parameter(torch.ones(4))
+        opt = cls([p], lr=0.5, **kw)
+        p.grad = torch.ones_like(p)
+        if cls is not optim.FusedAdam:
+            opt.step()
+        return opt.state_dict()
+
+    for cls, kw in ((torch.optim.Adam, dict(weight_decay=0.1)), (torch.optim.NAdam, {}), (torch.optim.RAdam, {}), (torch.optim.Adamax, {}), (torch.optim.Adagrad, {}),
+                    (torch.optim.SGD, dict(momentum=0.9)), (optim.FusedAdam, dict(weight_decay=1e-6)), (torch.optim.AdamW, dict(amsgrad=True))):
+        opt = optim.FusedAdamW([torch.nn.Parameter(torch.ones(4, device=device))], lr=0.25)
+        with pytest.raises(ValueError):
+            opt.load_state_dict(other(cls, **kw))
+        assert opt.param_groups[0]["lr"] == 0.25 and not opt.state, cls
+    for cls, kw in ((torch.optim.Adam, {}), (torch.optim.AdamW, dict(weight_decay=0.1)), (torch.optim.AdamW, {}), (optim.FusedAdam, {}), (optim.FusedAdamW, {})):
+        p = torch.nn.Parameter(torch.ones(4, device=device))
+        opt = optim.FusedAdamW([p], lr=0.25)
+        saved = other(cls, **kw) if cls is not optim.FusedAdamW else optim.FusedAdamW([torch.nn.Parameter(torch.ones(4))], lr=0.5).state_dict()
+        opt.load_state_dict(saved)
+        assert opt.param_groups[0]["lr"] == 0.5 and opt.param_groups[0]["weight_decay"] == saved["param_groups"][0]["weight_decay"]
+        p.grad = torch.ones_like(p)
+        opt.step()
+        assert opt.state[p]["step"] == (2 if saved["state"] else 1)
+        opt.param_groups[0]["weight_decay"] = 0.3                  # from here on the decay is this optimizer's
+        again = optim.FusedAdamW([torch.nn.Parameter(torch.ones(4, device=device))])
+        again.load_state_dict(opt.state_dict())
+        assert again.param_groups[0]["weight_decay"] == 0.3

@@ -196,3 +196,7 @@ def test_agent_maps_have_no_seam():
 
 def test_fused_adamw_loads_all_or_nothing():
     oc.check_fused_adamw_loads_all_or_nothing(DEV)
+
+
+def test_fused_adamw_loads_no_other_decay():
+    oc.check_fused_adamw_loads_no_other_decay(DEV)
