@@ -180,14 +180,16 @@ def _check_rule(group):
         raise ValueError("the saved state is Adam's, with a decay that is folded into the gradient: it would go on by another rule")
 
 
-def _check_saved(p, st):
-    """``st``: a saved entry of FusedAdamW or torch.optim.AdamW for a parameter like ``p``."""
+def _check_saved(p, st, bits):
+    """``st``: a saved entry of FusedAdamW or torch.optim.AdamW for a parameter like ``p``, in a group with moments of ``bits`` bits."""
     if not st.keys() <= {"step", "exp_avg", "exp_avg_sq", "scales"}:
         raise ValueError(f"the saved state is none of AdamW: it has {sorted(st)}")
     if any(not torch.is_tensor(st.get(key)) or st[key].shape != p.shape for key in ("exp_avg", "exp_avg_sq")) or "step" not in st:
         raise ValueError(f"the saved state of a parameter of shape {tuple(p.shape)} is none, or has another shape")
     types = st["exp_avg"].dtype, st["exp_avg_sq"].dtype
-    if all(t.is_floating_point for t in types):
+    if all(t.is_floating_point for t in types) != (bits == 32):
+        raise ValueError(f"a group with state_bits={bits} cannot go on from moments that are {types}")
+    if bits == 32:
         return
     if types != (torch.int8, torch.uint8):
         raise ValueError(f"moments are floating-point numbers, or int8 and uint8 codes, not {types}")
@@ -282,23 +284,27 @@ class FusedAdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """Also of torch.optim.AdamW's states (not with amsgrad or maximize), and of Adam's without weight decay.  The base class casts floating-point state to its
-        parameter's type: here moments and scales are float32 or the codes they were saved as, laid out like their parameter.  A state that
-        does not fit is refused before anything is loaded."""
+        parameter's type: here moments and scales are float32 or the codes they were saved as, laid out like their parameter.  ``state_bits``
+        and ``seed`` are the saved ones; where a state has none (torch's), they stay, and moments in 32 bits are refused by a group with
+        8-bit ones.  A state that does not fit is refused before anything is loaded."""
         seen = []
 
         def check(_, state_dict):                        # (behind the hooks that may change it)
-            for group in state_dict["param_groups"]:
+            groups = []
+            for own, group in zip(self.param_groups, state_dict["param_groups"]):
                 _check_rule(group)
-            for p, st in self._saved_states(state_dict):
-                _check_saved(p, st)
-            seen.append(state_dict)
+                groups.append({"state_bits": own["state_bits"], "seed": own["seed"], **group})
+            seen.append({**state_dict, "param_groups": groups + list(state_dict["param_groups"][len(groups):])})
+            for group, p, st in self._saved_states(seen[0]):
+                _check_saved(p, st, group["state_bits"])
+            return seen[0]
 
         hook = self.register_load_state_dict_pre_hook(check)
         try:
             super().load_state_dict(state_dict)
         finally:
             hook.remove()
-        for p, st in self._saved_states(seen[0]):
+        for _, p, st in self._saved_states(seen[0]):
             for key, value in st.items():
                 if key == "step":
                     self.state[p][key] = int(value)
@@ -308,11 +314,11 @@ class FusedAdamW(torch.optim.Optimizer):
                     self.state[p][key] = torch.empty_like(like, dtype=dtype, device=p.device, requires_grad=False).copy_(value)
 
     def _saved_states(self, state_dict):
-        """(parameter, its entry of ``state_dict``) of those that have one, as far as the groups are alike (the base class checks that)."""
+        """(saved group, parameter, its entry of ``state_dict``) of those that have one, as far as the groups are alike (the base class checks that)."""
         for group, saved in zip(self.param_groups, state_dict["param_groups"]):
             for p, i in zip(group["params"], saved["params"]):
                 if state_dict["state"].get(i):
-                    yield p, state_dict["state"][i]
+                    yield saved, p, state_dict["state"][i]
 
     def zero_grad(self, set_to_none=True):
         for group in self.param_groups:

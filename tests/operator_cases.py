@@ -1281,3 +1281,32 @@ def check_fused_adamw_loads_no_other_decay(device):
         again = optim.FusedAdamW([torch.nn.Parameter(torch.ones(4, device=device))])
         again.load_state_dict(opt.state_dict())
         assert again.param_groups[0]["weight_decay"] == 0.3
+
+
+def check_fused_adamw_keeps_its_bits(device):
+    """A state of torch.optim.AdamW says nothing of 8-bit moments: an optimizer made with them stays one, and refuses moments in 32 bits
+    where it cannot go on from them."""
+    p = torch.nn.Parameter(torch.ones(300))
+    ref = torch.optim.AdamW([p], lr=0.5)
+    fresh = ref.state_dict()
+    p.grad = torch.ones_like(p)
+    ref.step()
+    q = torch.nn.Parameter(torch.ones(300, device=device))
+    opt = optim.FusedAdamW([q], lr=0.25, state_bits=8, seed=6)
+    with pytest.raises(ValueError, match="state_bits"):
+        opt.load_state_dict(ref.state_dict())
+    assert opt.param_groups[0]["lr"] == 0.25 and not opt.state
+    opt.load_state_dict(fresh)                                            # no step taken: nothing to go on from
+    assert opt.param_groups[0]["lr"] == 0.5 and opt.param_groups[0]["state_bits"] == 8 and opt.param_groups[0]["seed"] == 6
+    q.grad = torch.ones_like(q)
+    opt.step()
+    assert opt.state[q]["exp_avg"].dtype == torch.int8
+    saved = opt.state_dict()                                              # ... and what says so decides
+    other = optim.FusedAdamW([torch.nn.Parameter(torch.ones(300, device=device))], state_bits=32, seed=1)
+    other.load_state_dict(saved)
+    assert other.param_groups[0]["state_bits"] == 8 and other.param_groups[0]["seed"] == 6
+    mixed = {**saved, "param_groups": [{**saved["param_groups"][0], "state_bits": 32}]}
+    with pytest.raises(ValueError, match="state_bits"):
+        other.load_state_dict(mixed)
+    with pytest.raises(ValueError):                                       # another number of groups: torch's own refusal
+        other.load_state_dict({**saved, "param_groups": saved["param_groups"] * 2})

@@ -409,3 +409,7 @@ def test_fused_adamw_loads_all_or_nothing():
 
 def test_fused_adamw_loads_no_other_decay():
     oc.check_fused_adamw_loads_no_other_decay(DEV)
+
+
+def test_fused_adamw_keeps_its_bits():
+    oc.check_fused_adamw_keeps_its_bits(DEV)
