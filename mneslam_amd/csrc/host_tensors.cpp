@@ -3,6 +3,7 @@
 // several hundred tensors costs 2.5 us a tensor in python (about thirty attribute reads) and 0.25 us here, and a backward pass through two
 // python nodes 140 us and 30 us.
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
@@ -103,23 +104,35 @@ bool laid_out_alike(const at::Tensor& a, const at::Tensor& b) {
     return true;
 }
 
-void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& exp_avgs, const Tensors& exp_avg_sqs,
-               const c10::optional<Tensors>& scales, const c10::optional<std::vector<int64_t>>& ordinals, double lr, double beta1,
-               double beta2, double eps, double weight_decay, int64_t step, int64_t seed, bool zero_grad, uintptr_t clock) {
+// A step that has been checked, ready to be launched.
+struct AdamwStep {
+    Tensors params, keep, clear;                         // clear: gradients that are zeroed behind it
+    at::Device dev = at::kCPU;
+    std::map<std::pair<int, int>, std::vector<int64_t>> tables;          // by the types of parameter and gradient
+    mne_adamw_cfg_t cfg = {};
+    uintptr_t clock = 0;
+};
+typedef std::vector<std::pair<int64_t, int64_t>> Ranges;
+
+// zero_grad: 1, by the step itself; 2, also of gradients laid out otherwise, behind it
+AdamwStep adamw_prepare(Ranges& ranges, const Tensors& params, const Tensors& grads, const Tensors& exp_avgs, const Tensors& exp_avg_sqs,
+                        const c10::optional<Tensors>& scales, const c10::optional<std::vector<int64_t>>& ordinals, double lr, double beta1,
+                        double beta2, double eps, double weight_decay, int64_t step, int64_t seed, int64_t zero_grad, uintptr_t clock) {
+    AdamwStep s;
     const size_t n = params.size();
     const bool small = scales.has_value();
     if (grads.size() != n || exp_avgs.size() != n || exp_avg_sqs.size() != n || (small && scales->size() != n) ||
         (ordinals && ordinals->size() != n))
         throw py::value_error("adamw_step: lists of different lengths");
-    if (!n) return;
+    if (!n) return s;
     if (!params[0].defined()) throw py::value_error("adamw_step: undefined tensors");
     one_device("adamw_step", {&params[0]});
     const at::Device dev = params[0].device();
     const c10::DeviceGuard guard(dev);
-    std::map<std::pair<int, int>, std::vector<int64_t>> tables;          // by the types of parameter and gradient
-    std::vector<std::pair<int64_t, int64_t>> ranges;                     // what the step writes
-    Tensors keep;
     c10::NoGradGuard no_grad;
+    s.params = params; s.dev = dev; s.clock = clock;
+    s.cfg.lr = lr; s.cfg.beta1 = beta1; s.cfg.beta2 = beta2; s.cfg.eps = eps; s.cfg.weight_decay = weight_decay;
+    s.cfg.step = (int32_t)step; s.cfg.state_bits = small ? 8 : 32; s.cfg.zero_grad = zero_grad != 0; s.cfg.seed = (uint32_t)seed;
     for (size_t i = 0; i < n; ++i) {
         const at::Tensor &p = params[i], &m = exp_avgs[i], &v = exp_avg_sqs[i];
         at::Tensor g = grads[i];
@@ -141,22 +154,26 @@ void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& exp_
         if (!written_in_memory(g)) {
             if (zero_grad) throw py::value_error("adamw_step: zero_grad cannot clear a negated view or zeros without memory");
             g = in_memory(g);
-            keep.push_back(g);
+            s.keep.push_back(g);
         }
         const int64_t count = p.numel(), ordinal = ordinals ? (*ordinals)[i] : (int64_t)i;
         if (ordinal < 0 || ordinal > 0xFFFFFFFFll) throw py::value_error("adamw_step: ordinals are numbers of 32 bits");
         if (small) {
-            const at::Tensor& s = (*scales)[i];
-            if (s.scalar_type() != at::kFloat || s.dim() != 2 || s.size(0) != (count + 255) / 256 || s.size(1) != 2 || !s.is_contiguous())
-                throw py::value_error("adamw_step: scales must be contiguous float32 [ceil(n / 256), 2]");
+            const at::Tensor& t = (*scales)[i];
+            if (t.scalar_type() != at::kFloat || t.dim() != 2 || t.size(0) != (count + 255) / 256 || t.size(1) != 2 || !t.is_contiguous() ||
+                (count && (uintptr_t)t.data_ptr() % 8))
+                throw py::value_error("adamw_step: scales must be contiguous float32 [ceil(n / 256), 2] at a multiple of 8 bytes");
         }
         if (!count) continue;
         if (!p.is_non_overlapping_and_dense()) throw py::value_error("adamw_step: parameters must be dense");
         if (!laid_out_alike(m, p) || !laid_out_alike(v, p)) throw py::value_error("adamw_step: moments must be laid out like their parameter");
         if (!laid_out_alike(g, p)) {
-            if (zero_grad) throw py::value_error("adamw_step: zero_grad needs gradients laid out like their parameters");
+            if (zero_grad == 1) throw py::value_error("adamw_step: zero_grad needs gradients laid out like their parameters");
+            if (zero_grad && at::has_internal_overlap(g) != at::MemOverlap::No)
+                throw py::value_error("adamw_step: zero_grad cannot clear a gradient whose elements share memory");
+            if (zero_grad) s.clear.push_back(g);
             g = at::empty_like(p, p.options().dtype(g.scalar_type())).copy_(g);
-            keep.push_back(g);
+            s.keep.push_back(g);
         }
         const auto writes = [&](const at::Tensor& t) {
             const int64_t at = (int64_t)t.data_ptr();
@@ -167,23 +184,54 @@ void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& exp_
         writes(v);
         if (small) writes((*scales)[i]);
         if (zero_grad) writes(g);
-        std::vector<int64_t>& table = tables[{pt, gt}];
+        std::vector<int64_t>& table = s.tables[{pt, gt}];
         const int64_t row[7] = {(int64_t)p.data_ptr(), (int64_t)g.data_ptr(), (int64_t)m.data_ptr(), (int64_t)v.data_ptr(),
                                 small ? (int64_t)(*scales)[i].data_ptr() : 0, count, ordinal};
         table.insert(table.end(), row, row + 7);
     }
+    if (clock) check(g_lib.adamw_step(nullptr, 0, &s.cfg, (const mne_clock_t*)clock, nullptr), "mne_adamw_step");        // (of no tensors: the clock alone)
+    return s;
+}
+
+void adamw_apart(Ranges& ranges) {
     std::sort(ranges.begin(), ranges.end());
     for (size_t i = 1; i < ranges.size(); ++i)
         if (ranges[i].first < ranges[i - 1].second) throw py::value_error("adamw_step: parameters or moments overlap (the same one twice?)");
-    for (const auto& t : tables) {
-        mne_adamw_cfg_t cfg = {};
-        cfg.lr = lr; cfg.beta1 = beta1; cfg.beta2 = beta2; cfg.eps = eps; cfg.weight_decay = weight_decay;
-        cfg.step = (int32_t)step; cfg.state_bits = small ? 8 : 32; cfg.p_type = t.first.first; cfg.g_type = t.first.second;
-        cfg.zero_grad = zero_grad; cfg.seed = (uint32_t)seed;
-        check(g_lib.adamw_step(t.second.data(), (int64_t)t.second.size() / 7, &cfg, (const mne_clock_t*)clock, stream_of(dev)), "mne_adamw_step");
+}
+
+void adamw_launch(AdamwStep& s) {
+    const c10::DeviceGuard guard(s.dev);
+    c10::NoGradGuard no_grad;
+    for (const auto& t : s.tables) {
+        s.cfg.p_type = t.first.first;
+        s.cfg.g_type = t.first.second;
+        check(g_lib.adamw_step(t.second.data(), (int64_t)t.second.size() / 7, &s.cfg, (const mne_clock_t*)s.clock, stream_of(s.dev)), "mne_adamw_step");
     }
-    for (const at::Tensor& p : params)              // what autograd has saved of a parameter is out of date, as after p.add_()
+    for (const at::Tensor& g : s.clear) g.zero_();
+    for (const at::Tensor& p : s.params)            // what autograd has saved of a parameter is out of date, as after p.add_()
         if (!p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
+}
+
+void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& exp_avgs, const Tensors& exp_avg_sqs,
+                const c10::optional<Tensors>& scales, const c10::optional<std::vector<int64_t>>& ordinals, double lr, double beta1,
+                double beta2, double eps, double weight_decay, int64_t step, int64_t seed, int64_t zero_grad, uintptr_t clock) {
+    Ranges ranges;
+    AdamwStep s = adamw_prepare(ranges, params, grads, exp_avgs, exp_avg_sqs, scales, ordinals, lr, beta1, beta2, eps, weight_decay, step, seed,
+                                zero_grad, clock);
+    adamw_apart(ranges);
+    adamw_launch(s);
+}
+
+// Several of them (an optimizer's groups): all are checked before the first is launched.
+typedef std::tuple<Tensors, Tensors, Tensors, Tensors, c10::optional<Tensors>, c10::optional<std::vector<int64_t>>, double, double, double, double, double,
+                   int64_t, int64_t, int64_t, uintptr_t> AdamwCall;
+void adamw_steps(const std::vector<AdamwCall>& calls) {
+    Ranges ranges;
+    std::vector<AdamwStep> steps;
+    for (const AdamwCall& call : calls)
+        steps.push_back(std::apply([&](const auto&... args) { return adamw_prepare(ranges, args...); }, call));
+    adamw_apart(ranges);
+    for (AdamwStep& s : steps) adamw_launch(s);
 }
 
 std::vector<at::Tensor> adamw_moments(const at::Tensor& given_m, const at::Tensor& given_v, const at::Tensor& given_scales) {
@@ -380,6 +428,7 @@ at::Tensor expert_combine(const at::Tensor& y, const at::Tensor& position, const
 PYBIND11_MODULE(_host_tensors, m) {
     m.def("bind", &bind);
     m.def("adamw_step", &adamw_step);
+    m.def("adamw_steps", &adamw_steps);
     m.def("adamw_moments", &adamw_moments);
     m.def("expert_sort", &expert_sort);
     m.def("expert_dispatch", &expert_dispatch);

@@ -146,18 +146,22 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, scales=None, *, step, lr, b
 
     ``step`` counts from 1 and is the list's; ``clock`` (mneslam_amd._lib.Clock, graph recording) adds the device's step offset.
     Without one a step is not recorded into a graph: every replay would be the same step."""
+    params = list(params)
+    args = _step_args(params, grads, exp_avgs, exp_avg_sqs, scales, ordinals, lr, betas, eps, weight_decay, step, seed, int(bool(zero_grad)), clock)
+    if params:
+        _lib.host_tensors().adamw_step(*args)
+
+
+def _step_args(params, grads, exp_avgs, exp_avg_sqs, scales, ordinals, lr, betas, eps, weight_decay, step, seed, zero_grad, clock):
     lr, eps, weight_decay = float(lr), float(eps), float(weight_decay)
     _check_hyper(lr, betas, eps, weight_decay)
     if not 1 <= step < 1 << 31 or not 0 <= seed < 1 << 32:
         raise ValueError(f"adamw_step: step counts from 1 and seed is a number of 32 bits, got {step} and {seed}")
-    params = list(params)
-    if not params:
-        return
-    if clock is None and params[0].is_cuda and torch.cuda.is_current_stream_capturing():
+    if clock is None and params and params[0].is_cuda and torch.cuda.is_current_stream_capturing():
         raise RuntimeError("adamw_step: recording a step needs a clock (the step count would be the same at every replay)")
-    _lib.host_tensors().adamw_step(params, list(grads), list(exp_avgs), list(exp_avg_sqs), None if scales is None else list(scales),
-                                   None if ordinals is None else list(ordinals), lr, betas[0], betas[1], eps, weight_decay, step, seed,
-                                   zero_grad, 0 if clock is None else C.addressof(clock))
+    return (params, list(grads), list(exp_avgs), list(exp_avg_sqs), None if scales is None else list(scales),
+            None if ordinals is None else list(ordinals), lr, float(betas[0]), float(betas[1]), eps, weight_decay, step, seed, zero_grad,
+            0 if clock is None else C.addressof(clock))
 
 
 def adamw_moments(exp_avg, exp_avg_sq, scales):
@@ -241,13 +245,14 @@ class FusedAdamW(torch.optim.Optimizer):
 
     @torch.no_grad()
     def step(self, closure=None, zero_grad=False, clock=None):
-        """``zero_grad``: the gradients are zero behind the step (one pass less over them).  ``clock`` (graph recording): the kernels
-        add the device step offset to the parameters' CURRENT step + 1, and the step counts here are left alone."""
+        """All of it or, where something is refused, nothing.  ``zero_grad``: the gradients are zero behind the step (one pass less over
+        them).  ``clock`` (graph recording): the kernels add the device step offset to the parameters' CURRENT step + 1, and the step counts
+        here are left alone."""
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        ordinal = 0
+        ordinal, calls, counts, sums = 0, [], [], []
         for group in self.param_groups:
             batches = {}                                # tensors of one device at one step count
             for p in group["params"]:
@@ -258,21 +263,26 @@ class FusedAdamW(torch.optim.Optimizer):
                 if p.grad.is_sparse:
                     raise RuntimeError("FusedAdamW does not support sparse gradients")
                 g = plane_sums.gradient(p)              # (a half-precision plane: the fp32 sum that .grad is the rounding of)
+                if getattr(p, "grad32", None) is not None:
+                    sums.append(p)
                 st = self._state(p, group["state_bits"])
                 batches.setdefault((p.device, st["step"] + 1), []).append((p, g, st, ordinal - 1))
             for (_, step), batch in batches.items():
                 ps, gs, sts, ords = zip(*batch)
-                adamw_step(ps, gs, [s["exp_avg"] for s in sts], [s["exp_avg_sq"] for s in sts],
-                           [s["scales"] for s in sts] if group["state_bits"] == 8 else None, step=step, lr=group["lr"],
-                           betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"], seed=group["seed"],
-                           ordinals=ords, zero_grad=zero_grad, clock=clock)
-                if clock is None:
-                    for s in sts:
-                        s["step"] = step
-                if zero_grad:
-                    for p in ps:
-                        if getattr(p, "grad32", None) is not None:
-                            plane_sums.zero(p)
+                calls.append(_step_args(list(ps), gs, [s["exp_avg"] for s in sts], [s["exp_avg_sq"] for s in sts],
+                                        [s["scales"] for s in sts] if group["state_bits"] == 8 else None, ords, group["lr"], group["betas"],
+                                        group["eps"], group["weight_decay"], step, group["seed"], 2 if zero_grad else 0, clock))
+                counts.append((step, sts))
+        if not calls:
+            return loss
+        _lib.host_tensors().adamw_steps(calls)          # (all of them are checked before the first is launched)
+        if clock is None:
+            for step, sts in counts:
+                for s in sts:
+                    s["step"] = step
+        if zero_grad:
+            for p in sums:
+                plane_sums.zero(p)
         return loss
 
     def moments(self, p):

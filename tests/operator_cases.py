@@ -1310,3 +1310,54 @@ def check_fused_adamw_keeps_its_bits(device):
         other.load_state_dict(mixed)
     with pytest.raises(ValueError):                                       # another number of groups: torch's own refusal
         other.load_state_dict({**saved, "param_groups": saved["param_groups"] * 2})
+
+
+def check_fused_adamw_steps_all_or_nothing(device):
+    """A step that is refused for one group has changed none; a gradient laid out otherwise is cleared like the others."""
+    from mneslam_amd import _lib
+    make = lambda *shape: torch.nn.Parameter(torch.ones(shape, device=device))                 # noqa: E731
+
+    def refused(error, last, grad, bits=32, **kw):
+        first, second = make(300), make(20)
+        opt = optim.FusedAdamW([{"params": [first]}, {"params": [second], "lr": 0.5, "betas": (0.9, 0.99)}, {"params": [last]}], state_bits=bits)
+        for p in (first, second):
+            p.grad = torch.ones_like(p)
+        opt.step()
+        last.grad = grad
+        before = [t.detach().clone() for p in (first, second) for t in (p, p.grad, *opt.moments(p))]
+        with pytest.raises(error):
+            opt.step(**kw)
+        assert all(torch.equal(a, b) for a, b in zip(before, [t for p in (first, second) for t in (p, p.grad, *opt.moments(p))]))
+        assert opt.state[first]["step"] == opt.state[second]["step"] == 1
+        last.grad = None
+        opt.step()
+        assert opt.state[first]["step"] == 2 and not torch.equal(first, before[0])
+
+    for bits in (8, 32):
+        refused(RuntimeError, make(5), torch.ones(5, device=device).to_sparse(), bits)
+        double = torch.nn.Parameter(torch.ones(5, device=device, dtype=torch.float64))
+        refused(TypeError, double, torch.ones(5, device=device, dtype=torch.float64), bits)
+        refused(ValueError, make(4, 5), torch.ones(1, 1, device=device).expand(4, 5), bits, zero_grad=True)
+        refused(ValueError, torch.nn.Parameter(torch.ones(1, device=device).expand(5)), torch.ones(5, device=device), bits)
+    offset, table = torch.zeros(1, dtype=torch.int32, device=device), torch.ones(9, 2, dtype=torch.float64, device=device)
+    clock = _lib.Clock()
+    clock.step_offset, clock.bias_table, clock.n_table, clock.beta1, clock.beta2 = offset.data_ptr(), table.data_ptr(), 9, 0.9, 0.999
+    refused(RuntimeError, make(5), torch.ones(5, device=device), clock=clock)                   # (the second group has other betas)
+
+    for bits in (8, 32):
+        gen = torch.Generator().manual_seed(51)
+        p, q = make(6, 7), make(6, 7)
+        g = torch.randn(6, 7, generator=gen).to(device)
+        opt = optim.FusedAdamW([p, q], state_bits=bits)
+        p.grad, q.grad = g.clone(), g.t().contiguous().t()
+        seen = q.grad
+        opt.step(zero_grad=True)
+        assert not p.grad.any() and q.grad is seen and not seen.any()
+        want = optim.FusedAdamW([r := make(6, 7), s := make(6, 7)], state_bits=bits)
+        r.grad, s.grad = g.clone(), g.clone()
+        want.step()
+        assert torch.equal(p, r) and torch.equal(q, s)
+    p = torch.ones(300, device=device)
+    scales = torch.zeros(5, device=device)[1:].view(2, 2)                                     # not at a multiple of 8 bytes
+    with pytest.raises(ValueError, match="scales"):
+        optim.adamw_step([p], [p.clone()], [p.to(torch.int8)], [p.to(torch.uint8)], [scales], step=1, lr=0.1)

@@ -413,3 +413,7 @@ def test_fused_adamw_loads_no_other_decay():
 
 def test_fused_adamw_keeps_its_bits():
     oc.check_fused_adamw_keeps_its_bits(DEV)
+
+
+def test_fused_adamw_steps_all_or_nothing():
+    oc.check_fused_adamw_steps_all_or_nothing(DEV)
