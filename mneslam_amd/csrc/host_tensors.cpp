@@ -112,7 +112,14 @@ struct AdamwStep {
     mne_adamw_cfg_t cfg = {};
     uintptr_t clock = 0;
 };
-typedef std::vector<std::pair<int64_t, int64_t>> Ranges;
+// Memory that the steps write and read: from where to where, and whose.
+struct Range {
+    int64_t from, to, owner;
+};
+struct Ranges {
+    std::vector<Range> written, read;
+    int64_t owners = 0;
+};
 
 // zero_grad: 1, by the step itself; 2, also of gradients laid out otherwise, behind it
 AdamwStep adamw_prepare(Ranges& ranges, const Tensors& params, const Tensors& grads, const Tensors& exp_avgs, const Tensors& exp_avg_sqs,
@@ -175,15 +182,14 @@ AdamwStep adamw_prepare(Ranges& ranges, const Tensors& params, const Tensors& gr
             g = at::empty_like(p, p.options().dtype(g.scalar_type())).copy_(g);
             s.keep.push_back(g);
         }
-        const auto writes = [&](const at::Tensor& t) {
+        const int64_t owner = ranges.owners++;
+        const auto note = [owner](std::vector<Range>& to, const at::Tensor& t) {
             const int64_t at = (int64_t)t.data_ptr();
-            ranges.emplace_back(at, at + t.numel() * (int64_t)t.element_size());
+            to.push_back({at, at + t.numel() * (int64_t)t.element_size(), owner});
         };
-        writes(p);
-        writes(m);
-        writes(v);
-        if (small) writes((*scales)[i]);
-        if (zero_grad) writes(g);
+        for (const at::Tensor* t : {&p, &m, &v}) note(ranges.written, *t);
+        if (small) note(ranges.written, (*scales)[i]);
+        note(zero_grad ? ranges.written : ranges.read, g);
         std::vector<int64_t>& table = s.tables[{pt, gt}];
         const int64_t row[7] = {(int64_t)p.data_ptr(), (int64_t)g.data_ptr(), (int64_t)m.data_ptr(), (int64_t)v.data_ptr(),
                                 small ? (int64_t)(*scales)[i].data_ptr() : 0, count, ordinal};
@@ -193,10 +199,18 @@ AdamwStep adamw_prepare(Ranges& ranges, const Tensors& params, const Tensors& gr
     return s;
 }
 
+// What is written is nobody else's, and what is read (a gradient) is at most its own tensor's, element for element.
 void adamw_apart(Ranges& ranges) {
-    std::sort(ranges.begin(), ranges.end());
-    for (size_t i = 1; i < ranges.size(); ++i)
-        if (ranges[i].first < ranges[i - 1].second) throw py::value_error("adamw_step: parameters or moments overlap (the same one twice?)");
+    std::vector<Range>& w = ranges.written;
+    std::sort(w.begin(), w.end(), [](const Range& a, const Range& b) { return a.from < b.from; });
+    for (size_t i = 1; i < w.size(); ++i)
+        if (w[i].from < w[i - 1].to) throw py::value_error("adamw_step: parameters or moments overlap (the same one twice?)");
+    for (const Range& r : ranges.read) {
+        auto at = std::upper_bound(w.begin(), w.end(), r.from, [](int64_t from, const Range& x) { return from < x.to; });
+        for (; at != w.end() && at->from < r.to; ++at)
+            if (at->owner != r.owner || at->from != r.from || at->to != r.to)
+                throw py::value_error("adamw_step: a gradient overlaps what the step writes (parameters, moments)");
+    }
 }
 
 void adamw_launch(AdamwStep& s) {

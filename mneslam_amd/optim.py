@@ -136,7 +136,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, scales=None, *, step, lr, b
     Parameters are float32, bfloat16 or float16; a gradient has its parameter's type or float32 (any of the three beside a float32
     parameter).  The arithmetic is fp32; a 16-bit parameter is rounded to nearest even.  Every tensor is dense (contiguous or
     channels_last); moments are laid out like their parameter, a gradient laid out otherwise (or negated lazily) is copied.  What the step
-    writes does not overlap and is no negated view: parameters, moments, scales, gradients that it clears.
+    writes does not overlap and is no negated view: parameters, moments, scales, gradients that it clears.  A gradient that it only reads
+    may be another's too, but not a part of what is written.
 
     ``scales`` None: moments are float32.  Otherwise they are held in 8 bits: ``exp_avgs`` int8, ``exp_avg_sqs`` uint8, and
     ``scales`` the list of their float32 [ceil(n / 256), 2] scales, two for each 256 consecutive elements of the tensor's memory

@@ -1361,3 +1361,25 @@ def check_fused_adamw_steps_all_or_nothing(device):
     scales = torch.zeros(5, device=device)[1:].view(2, 2)                                     # not at a multiple of 8 bytes
     with pytest.raises(ValueError, match="scales"):
         optim.adamw_step([p], [p.clone()], [p.to(torch.int8)], [p.to(torch.uint8)], [scales], step=1, lr=0.1)
+
+
+def check_adamw_gradient_in_written_memory(device):
+    """A gradient that lies over what the step writes would be read half before and half after: refused, unless it is a tensor's own
+    memory element for element."""
+    flat = torch.arange(1000.0, device=device)
+    p, q = flat[:300], flat[300:600]
+    for bits in (8, 32):
+        states = [_state_for(t, bits, device) for t in (p, q)]
+        before = flat.clone()
+        m = states[0][0][0]
+        for grads in ([flat[1:301], q.clone()], [flat[600:900], flat[450:750]], [q, q.clone()], [q, p], [flat[299:599], q.clone()]) + \
+                (([m.new_ones(300), m],) if bits == 32 else ()):
+            with pytest.raises(ValueError, match="overlap"):
+                _step([p, q], grads, bits, device, state=states)
+        assert torch.equal(flat, before) and not m.any()
+        _step([p, q], [flat[600:900], flat[650:950]], bits, device, state=states)            # beside it, and shared
+        assert torch.equal(flat[600:], before[600:]) and not torch.equal(p, before[:300])
+    p, g = torch.ones(300, device=device), torch.ones(300, device=device)
+    _step([p], [p], 32, device)
+    _step([g], [g.clone()], 32, device)
+    assert torch.equal(p, g)

@@ -208,3 +208,7 @@ def test_fused_adamw_keeps_its_bits():
 
 def test_fused_adamw_steps_all_or_nothing():
     oc.check_fused_adamw_steps_all_or_nothing(DEV)
+
+
+def test_adamw_gradient_in_written_memory():
+    oc.check_adamw_gradient_in_written_memory(DEV)
