@@ -106,7 +106,8 @@ bool laid_out_alike(const at::Tensor& a, const at::Tensor& b) {
 
 // A step that has been checked, ready to be launched.
 struct AdamwStep {
-    Tensors params, keep, clear;                         // clear: gradients that are zeroed behind it
+    Tensors keep, clear;                                 // clear: gradients that are zeroed behind it
+    std::vector<c10::TensorImpl*> written;               // (the caller holds them)
     at::Device dev = at::kCPU;
     std::map<std::pair<int, int>, std::vector<int64_t>> tables;          // by the types of parameter and gradient
     mne_adamw_cfg_t cfg = {};
@@ -137,7 +138,7 @@ AdamwStep adamw_prepare(Ranges& ranges, const Tensors& params, const Tensors& gr
     const at::Device dev = params[0].device();
     const c10::DeviceGuard guard(dev);
     c10::NoGradGuard no_grad;
-    s.params = params; s.dev = dev; s.clock = clock;
+    s.dev = dev; s.clock = clock;
     s.cfg.lr = lr; s.cfg.beta1 = beta1; s.cfg.beta2 = beta2; s.cfg.eps = eps; s.cfg.weight_decay = weight_decay;
     s.cfg.step = (int32_t)step; s.cfg.state_bits = small ? 8 : 32; s.cfg.zero_grad = zero_grad != 0; s.cfg.seed = (uint32_t)seed;
     for (size_t i = 0; i < n; ++i) {
@@ -190,6 +191,9 @@ AdamwStep adamw_prepare(Ranges& ranges, const Tensors& params, const Tensors& gr
         for (const at::Tensor* t : {&p, &m, &v}) note(ranges.written, *t);
         if (small) note(ranges.written, (*scales)[i]);
         note(zero_grad ? ranges.written : ranges.read, g);
+        for (const at::Tensor* t : {&p, &m, &v}) s.written.push_back(t->unsafeGetTensorImpl());
+        if (small) s.written.push_back((*scales)[i].unsafeGetTensorImpl());
+        if (zero_grad && g.is_same(grads[i])) s.written.push_back(g.unsafeGetTensorImpl());
         std::vector<int64_t>& table = s.tables[{pt, gt}];
         const int64_t row[7] = {(int64_t)p.data_ptr(), (int64_t)g.data_ptr(), (int64_t)m.data_ptr(), (int64_t)v.data_ptr(),
                                 small ? (int64_t)(*scales)[i].data_ptr() : 0, count, ordinal};
@@ -222,8 +226,8 @@ void adamw_launch(AdamwStep& s) {
         check(g_lib.adamw_step(t.second.data(), (int64_t)t.second.size() / 7, &s.cfg, (const mne_clock_t*)s.clock, stream_of(s.dev)), "mne_adamw_step");
     }
     for (const at::Tensor& g : s.clear) g.zero_();
-    for (const at::Tensor& p : s.params)            // what autograd has saved of a parameter is out of date, as after p.add_()
-        if (!p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
+    for (c10::TensorImpl* t : s.written)            // what autograd has saved of them is out of date, as after p.add_()
+        if (!t->is_inference()) t->bump_version();
 }
 
 void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& exp_avgs, const Tensors& exp_avg_sqs,

@@ -1383,3 +1383,24 @@ def check_adamw_gradient_in_written_memory(device):
     _step([p], [p], 32, device)
     _step([g], [g.clone()], 32, device)
     assert torch.equal(p, g)
+
+
+def check_adamw_outdates_what_it_writes(device):
+    """What autograd has saved of anything that a step writes is out of date: parameters, moments, scales, gradients that it clears."""
+    for bits in (8, 32):
+        p, g = torch.ones(300, device=device), torch.ones(300, device=device)
+        (m, v), s = state = _state_for(p, bits, device)
+        written = [t for t in (p, m, v, s) if t is not None]
+        old = [t._version for t in written + [g]]
+        _step([p], [g], bits, device, state=[state])
+        assert all(t._version > n for t, n in zip(written, old)) and g._version == old[-1]
+        w = torch.ones(300, device=device, requires_grad=True)
+        products = [(w * t) for t in [g] + [t for t in written if t.is_floating_point() and t.numel() == 300]]
+        _step([p], [g], bits, device, step=2, state=[state], zero_grad=True)
+        for out in products:
+            with pytest.raises(RuntimeError, match="inplace"):
+                out.sum().backward()
+        with torch.inference_mode():
+            q, h = torch.ones(5, device=device), torch.ones(5, device=device)
+            _step([q], [h], bits, device, zero_grad=True)
+            assert (q < 1).all() and not h.any()

@@ -212,3 +212,7 @@ def test_fused_adamw_steps_all_or_nothing():
 
 def test_adamw_gradient_in_written_memory():
     oc.check_adamw_gradient_in_written_memory(DEV)
+
+
+def test_adamw_outdates_what_it_writes():
+    oc.check_adamw_outdates_what_it_writes(DEV)
