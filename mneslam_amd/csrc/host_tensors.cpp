@@ -283,12 +283,13 @@ std::vector<at::Tensor> expert_sort(const at::Tensor& given, int64_t experts) {
     c10::NoGradGuard no_grad;
     const at::Tensor ids = in_memory(given).contiguous();
     const size_t bytes = g_lib.sort_bytes(m, (int)experts);
-    // one allocation: order, position, offsets, workspace
-    const at::Tensor all = at::empty({2 * m + experts + 1 + (int64_t)bytes / 4}, ids.options().dtype(at::kInt));
-    int32_t* base = (int32_t*)all.data_ptr();
-    check(g_lib.sort(ids.data_ptr(), ids.scalar_type() == at::kLong, m, (int)experts, base, base + m, base + 2 * m, base + 2 * m + experts + 1,
-                     bytes, stream_of(ids.device())), "mne_expert_sort");
-    return {all.narrow(0, 0, m), all.narrow(0, m, m).view({n, k}), all.narrow(0, 2 * m, experts + 1)};
+    // (tensors of their own: the workspace is free behind the call, and who writes into one of the plan's changes no other)
+    const at::TensorOptions opts = ids.options().dtype(at::kInt);
+    const at::Tensor order = at::empty({m}, opts), position = at::empty({n, k}, opts), offsets = at::empty({experts + 1}, opts);
+    const at::Tensor workspace = bytes ? at::empty({(int64_t)bytes / 4}, opts) : at::Tensor();
+    check(g_lib.sort(ids.data_ptr(), ids.scalar_type() == at::kLong, m, (int)experts, (int32_t*)order.data_ptr(), (int32_t*)position.data_ptr(),
+                     (int32_t*)offsets.data_ptr(), bytes ? workspace.data_ptr() : nullptr, bytes, stream_of(ids.device())), "mne_expert_sort");
+    return {order, position, offsets};
 }
 
 void check_rows(const at::Tensor& t, const char* what) {

@@ -1404,3 +1404,18 @@ def check_adamw_outdates_what_it_writes(device):
             q, h = torch.ones(5, device=device), torch.ones(5, device=device)
             _step([q], [h], bits, device, zero_grad=True)
             assert (q < 1).all() and not h.any()
+
+
+def check_plan_tensors_are_apart(device):
+    """A plan's tensors are memory of their own: writing into one touches no other, in value or in autograd's eyes, and no workspace stays."""
+    from mneslam_amd.routing import expert_combine, expert_dispatch, expert_sort
+    for n, k, e in ((4, 2, 3), (3000, 2, 3), (5000, 1, 2500), (0, 2, 3)):
+        ids = torch.zeros(n, k, dtype=torch.int32, device=device)
+        plan = expert_sort(ids, e)
+        for t in (plan.order, plan.position, plan.offsets):
+            assert t.untyped_storage().nbytes() == 4 * t.numel() and t.is_contiguous()
+        x = torch.ones(n, 2, device=device, requires_grad=True)
+        out = expert_combine(expert_dispatch(x, plan), plan)
+        plan.order.fill_(-1)
+        out.sum().backward()
+        assert (x.grad == k).all() and plan.offsets.tolist() == [0] + [n * k] * e and plan.position.reshape(-1).tolist() == list(range(n * k))

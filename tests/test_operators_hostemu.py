@@ -216,3 +216,7 @@ def test_adamw_gradient_in_written_memory():
 
 def test_adamw_outdates_what_it_writes():
     oc.check_adamw_outdates_what_it_writes(DEV)
+
+
+def test_plan_tensors_are_apart():
+    oc.check_plan_tensors_are_apart(DEV)
