@@ -507,6 +507,8 @@ static unsigned ex_grid(long long units, int group) {
 // Written: rows of whole 128-byte lines only -- 32768 rows of 2 KB combined 16 us instead of 30, dealt out 17 instead of 22; with rows of
 // 260 bytes, whose lines are written by two, 61 us instead of 36.
 // (Combined rows lie one after the other, and still: rows of 64 bytes 69 us and 67 without, of 32 bytes 98 and 78.)
+// Dealt-out rows only below 1 GB in all: rows of 4 KB, four to a token, 0.5 GB 108 us instead of 121, but 1 GB 254 instead of 249, 2.1 GB
+// 510 instead of 502, 4.3 GB 1025 instead of 1016 (one or two to a token: within 1 % from 0.5 GB on).
 // Read: combined rows of 128 MB and more in all, half of what the last cache holds: 128 MB 31 us instead of 33, 2.1 GB 429 instead of 464;
 // with 64 MB 17 us instead of 15.  (Its backward pass: 0 to 3 % either way, left alone.)
 static bool ex_whole_lines(const ExpertRowArgs& a, int type) { return ex_row_bytes(a, type) % 128 == 0 && (uintptr_t)a.out % 128 == 0; }
@@ -578,7 +580,7 @@ template <template <int, int, int> class F> static int ex_by_type(const ExpertRo
 }
 
 int mne_launch_expert_dispatch(ExpertRowArgs a, int type, hipStream_t st) {
-    const int past = ex_whole_lines(a, type);
+    const int past = ex_whole_lines(a, type) && ex_bytes(a, type) < 1ll << 30;
     return type == MNE_T_F32 ? ex_by_piece<ExDispatch, MNE_T_F32>(a, past, st) : ex_by_piece<ExDispatch, MNE_T_F16>(a, past, st);   // (rows are copied: any 16-bit type)
 }
 int mne_launch_expert_combine(ExpertRowArgs a, int type, hipStream_t st) {
