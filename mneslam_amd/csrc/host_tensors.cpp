@@ -107,15 +107,15 @@ bool laid_out_alike(const at::Tensor& a, const at::Tensor& b) {
 // A step that has been checked, ready to be launched.
 struct AdamwStep {
     Tensors keep, clear;                                 // clear: gradients that are zeroed behind it
-    std::vector<c10::TensorImpl*> written;               // (the caller holds them)
     at::Device dev = at::kCPU;
     std::map<std::pair<int, int>, std::vector<int64_t>> tables;          // by the types of parameter and gradient
     mne_adamw_cfg_t cfg = {};
     uintptr_t clock = 0;
 };
-// Memory that the steps write and read: from where to where, and whose.
+// Memory that the steps write and read: from where to where, of which row, and the tensor (which the caller holds).
 struct Range {
     int64_t from, to, owner;
+    c10::TensorImpl* tensor;
 };
 struct Ranges {
     std::vector<Range> written, read;
@@ -136,17 +136,20 @@ AdamwStep adamw_prepare(Ranges& ranges, const Tensors& params, const Tensors& gr
     if (!params[0].defined()) throw py::value_error("adamw_step: undefined tensors");
     one_device("adamw_step", {&params[0]});
     const at::Device dev = params[0].device();
-    const c10::DeviceGuard guard(dev);
     c10::NoGradGuard no_grad;
     s.dev = dev; s.clock = clock;
+    ranges.written.reserve(ranges.written.size() + 5 * n);
+    ranges.read.reserve(ranges.read.size() + n);
     s.cfg.lr = lr; s.cfg.beta1 = beta1; s.cfg.beta2 = beta2; s.cfg.eps = eps; s.cfg.weight_decay = weight_decay;
     s.cfg.step = (int32_t)step; s.cfg.state_bits = small ? 8 : 32; s.cfg.zero_grad = zero_grad != 0; s.cfg.seed = (uint32_t)seed;
     for (size_t i = 0; i < n; ++i) {
         const at::Tensor &p = params[i], &m = exp_avgs[i], &v = exp_avg_sqs[i];
         at::Tensor g = grads[i];
+        bool plain = true;                               // (all but a few are)
         for (const at::Tensor* t : {&p, (const at::Tensor*)&g, &m, &v, small ? &(*scales)[i] : &p}) {
             if (!t->defined() || t->layout() != at::kStrided) throw py::value_error("adamw_step: sparse or undefined tensors are not supported");
             no_subclass("adamw_step", *t);
+            plain = plain && written_in_memory(*t);
             if (t->device() != dev) throw py::value_error("adamw_step: tensors on " + dev.str() + " and on " + t->device().str());
         }
         const int pt = type_code(p.scalar_type()), gt = type_code(g.scalar_type());
@@ -157,9 +160,9 @@ AdamwStep adamw_prepare(Ranges& ranges, const Tensors& params, const Tensors& gr
             throw py::type_error(small ? "adamw_step: 8-bit moments must be int8 and uint8" : "adamw_step: moments must be float32");
         if (g.sizes() != p.sizes() || m.sizes() != p.sizes() || v.sizes() != p.sizes())
             throw py::value_error("adamw_step: gradient and moments need their parameter's shape");
-        for (const at::Tensor* t : {&p, &m, &v, small ? &(*scales)[i] : &p})
-            if (!written_in_memory(*t)) throw py::value_error("adamw_step: what is written in place must not be a negated view or without memory");
-        if (!written_in_memory(g)) {
+        if (!plain) {
+            for (const at::Tensor* t : {&p, &m, &v, small ? &(*scales)[i] : &p})
+                if (!written_in_memory(*t)) throw py::value_error("adamw_step: what is written in place must not be a negated view or without memory");
             if (zero_grad) throw py::value_error("adamw_step: zero_grad cannot clear a negated view or zeros without memory");
             g = in_memory(g);
             s.keep.push_back(g);
@@ -177,26 +180,21 @@ AdamwStep adamw_prepare(Ranges& ranges, const Tensors& params, const Tensors& gr
         if (!laid_out_alike(m, p) || !laid_out_alike(v, p)) throw py::value_error("adamw_step: moments must be laid out like their parameter");
         if (!laid_out_alike(g, p)) {
             if (zero_grad == 1) throw py::value_error("adamw_step: zero_grad needs gradients laid out like their parameters");
-            if (zero_grad && at::has_internal_overlap(g) != at::MemOverlap::No)
+            if (zero_grad && at::has_internal_overlap(g) == at::MemOverlap::Yes)
                 throw py::value_error("adamw_step: zero_grad cannot clear a gradient whose elements share memory");
             if (zero_grad) s.clear.push_back(g);
             g = at::empty_like(p, p.options().dtype(g.scalar_type())).copy_(g);
             s.keep.push_back(g);
         }
-        const int64_t owner = ranges.owners++;
-        const auto note = [owner](std::vector<Range>& to, const at::Tensor& t) {
-            const int64_t at = (int64_t)t.data_ptr();
-            to.push_back({at, at + t.numel() * (int64_t)t.element_size(), owner});
-        };
-        for (const at::Tensor* t : {&p, &m, &v}) note(ranges.written, *t);
-        if (small) note(ranges.written, (*scales)[i]);
-        note(zero_grad ? ranges.written : ranges.read, g);
-        for (const at::Tensor* t : {&p, &m, &v}) s.written.push_back(t->unsafeGetTensorImpl());
-        if (small) s.written.push_back((*scales)[i].unsafeGetTensorImpl());
-        if (zero_grad && g.is_same(grads[i])) s.written.push_back(g.unsafeGetTensorImpl());
         std::vector<int64_t>& table = s.tables[{pt, gt}];
         const int64_t row[7] = {(int64_t)p.data_ptr(), (int64_t)g.data_ptr(), (int64_t)m.data_ptr(), (int64_t)v.data_ptr(),
                                 small ? (int64_t)(*scales)[i].data_ptr() : 0, count, ordinal};
+        const int64_t owner = ranges.owners++, wide = (int64_t)p.element_size(), state = small ? 1 : 4;
+        ranges.written.push_back({row[0], row[0] + count * wide, owner, p.unsafeGetTensorImpl()});
+        ranges.written.push_back({row[2], row[2] + count * state, owner, m.unsafeGetTensorImpl()});
+        ranges.written.push_back({row[3], row[3] + count * state, owner, v.unsafeGetTensorImpl()});
+        if (small) ranges.written.push_back({row[4], row[4] + (count + 255) / 256 * 8, owner, (*scales)[i].unsafeGetTensorImpl()});
+        (zero_grad ? ranges.written : ranges.read).push_back({row[1], row[1] + count * (int64_t)g.element_size(), owner, g.unsafeGetTensorImpl()});
         table.insert(table.end(), row, row + 7);
     }
     if (clock) check(g_lib.adamw_step(nullptr, 0, &s.cfg, (const mne_clock_t*)clock, nullptr), "mne_adamw_step");        // (of no tensors: the clock alone)
@@ -217,6 +215,12 @@ void adamw_apart(Ranges& ranges) {
     }
 }
 
+// What autograd has saved of it is out of date, as after p.add_().
+void adamw_changed(const Ranges& ranges) {
+    for (const Range& r : ranges.written)
+        if (!r.tensor->is_inference()) r.tensor->bump_version();
+}
+
 void adamw_launch(AdamwStep& s) {
     const c10::DeviceGuard guard(s.dev);
     c10::NoGradGuard no_grad;
@@ -226,8 +230,6 @@ void adamw_launch(AdamwStep& s) {
         check(g_lib.adamw_step(t.second.data(), (int64_t)t.second.size() / 7, &s.cfg, (const mne_clock_t*)s.clock, stream_of(s.dev)), "mne_adamw_step");
     }
     for (const at::Tensor& g : s.clear) g.zero_();
-    for (c10::TensorImpl* t : s.written)            // what autograd has saved of them is out of date, as after p.add_()
-        if (!t->is_inference()) t->bump_version();
 }
 
 void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& exp_avgs, const Tensors& exp_avg_sqs,
@@ -238,6 +240,7 @@ void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& exp_
                                 zero_grad, clock);
     adamw_apart(ranges);
     adamw_launch(s);
+    adamw_changed(ranges);
 }
 
 // Several of them (an optimizer's groups): all are checked before the first is launched.
@@ -250,6 +253,7 @@ void adamw_steps(const std::vector<AdamwCall>& calls) {
         steps.push_back(std::apply([&](const auto&... args) { return adamw_prepare(ranges, args...); }, call));
     adamw_apart(ranges);
     for (AdamwStep& s : steps) adamw_launch(s);
+    adamw_changed(ranges);
 }
 
 std::vector<at::Tensor> adamw_moments(const at::Tensor& given_m, const at::Tensor& given_v, const at::Tensor& given_scales) {

@@ -119,7 +119,7 @@ MOMENT_BLOCK = 256             # consecutive elements of an 8-bit moment that sh
 def _check_hyper(lr, betas, eps, weight_decay):
     if not 0.0 <= lr < float("inf"):
         raise ValueError(f"Invalid learning rate: {lr}")
-    if not (len(betas) == 2 and all(0.0 <= b < 1.0 for b in betas)):
+    if not (len(betas) == 2 and 0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
         raise ValueError(f"Invalid betas: {betas}")
     if not 0.0 <= eps < float("inf"):
         raise ValueError(f"Invalid epsilon value: {eps}")
