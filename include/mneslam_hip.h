@@ -523,7 +523,7 @@ int mne_adam_step(const mne_adam_seg_t* segs, int n_seg, int zero_grad, const mn
  *   m = sign(c) c^2 scales[b][0],  sqrt(v) = c^2 scales[b][1]   (mne_adamw_moments gives both as numbers).
  *   A code is rounded up or down with a dither of 16 bits, a function of (cfg->seed, ordinal, step, element) alone: the same
  *   call gives the same codes.  `ordinal` is the caller's number for the tensor (0 .. 2^32 - 1), the same at every step.
- *   A block that meets a gradient that is not finite holds NaN from then on.
+ *   A block that meets a gradient that is not finite, or one of 1.85e19 and more, whose square is not, holds NaN from then on.
  * clock: as in mne_adam_step (the step, and with it the dither, comes from device memory). */
 int mne_adamw_step(const int64_t* table, int64_t n_tensors, const mne_adamw_cfg_t* cfg, const mne_clock_t* clock, void* stream);
 /* exp_avg [n] and exp_avg_sq [n] in fp32 of n elements' codes and scales (as above; one run that starts with a block). */

@@ -143,7 +143,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, scales=None, *, step, lr, b
     ``scales`` the list of their float32 [ceil(n / 256), 2] scales, two for each 256 consecutive elements of the tensor's memory
     (all zero: all moments zero; ``adamw_moments`` gives the moments in fp32).  Their codes are rounded up or down with a dither that
     depends on ``seed``, the tensor's entry of ``ordinals`` (its place in the list by default; keep it the same at every step),
-    ``step`` and the element alone.  A block that meets a gradient that is not finite holds NaN from then on.
+    ``step`` and the element alone.  A block that meets a gradient that is not finite, or one of 1.85e19 and more, whose square is not
+    in fp32, holds NaN from then on: all its 256 elements (32-bit moments keep that to the one).
 
     ``step`` counts from 1 and is the list's; ``clock`` (mneslam_amd._lib.Clock, graph recording) adds the device's step offset.
     Without one a step is not recorded into a graph: every replay would be the same step."""
