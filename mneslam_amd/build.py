@@ -55,7 +55,8 @@ def _stale(target, deps):
 
 
 def _deps():
-    return [os.path.join(CSRC, h) for h in HEADERS] + [os.path.join(INCLUDE, "mneslam_hip.h")]
+    # (this file has the compiler's flags)
+    return [os.path.join(CSRC, h) for h in HEADERS] + [os.path.join(INCLUDE, "mneslam_hip.h"), os.path.abspath(__file__), isa_check.__file__]
 
 
 def isa_report_path(lib):
@@ -86,8 +87,8 @@ def _compile_one(src, obj, extra, verbose):
 
 def check_isa(obj_dir, lib, strict=True):
     """Run the ISA checks (isa_check.py) over the device assembly of every translation unit of a build; writes
-    isa_report.json next to the library; raises if a kernel carries the spill-in-front-of-exec-restore defect."""
-    report = {"kernels": [], "hazards": []}
+    isa_report.json next to the library; raises if a kernel carries the spill-in-front-of-exec-restore defect or packed fp32 instructions."""
+    report = {"kernels": [], "hazards": [], "packed_fp32": []}
     for s in SOURCES:
         path = os.path.join(obj_dir, s[:-4] + ".gfx950.s")
         if not os.path.exists(path):
@@ -97,8 +98,13 @@ def check_isa(obj_dir, lib, strict=True):
             report["kernels"].append(dict(r, source=s))
         for kernel, (line, block, spill, restore, _) in isa_check.definite_hazards(text):
             report["hazards"].append({"source": s, "kernel": kernel, "line": line, "block": block, "spill": spill, "before": restore})
+        for kernel, line, text in isa_check.packed_fp32(text):
+            report["packed_fp32"].append({"source": s, "kernel": kernel, "line": line, "instruction": text})
     with open(isa_report_path(lib), "w") as f:
         json.dump(report, f, indent=1)
+    if report["packed_fp32"]:
+        raise RuntimeError("packed fp32 instructions in the generated ISA (-packed-fp32-ops was to turn them off): " +
+                           "; ".join(f"{p['kernel']} ({p['source']}:{p['line']}: {p['instruction']})" for p in report["packed_fp32"]))
     if report["hazards"] and strict and os.environ.get("MNE_ALLOW_SPILL_HAZARD", "0") != "1":
         msg = "; ".join(f"{h['kernel']} ({h['source']}:{h['line']}: {h['spill']} <before> {h['before']})" for h in report["hazards"])
         raise RuntimeError("compiler defect in the generated ISA (VGPR spill store in front of an exec restore, DESIGN.md section 9): " + msg)

@@ -13,6 +13,9 @@
 
 2. ``resources`` -- registers / scratch / occupancy of every kernel, from the compiler's own "Kernel info" comments
    (the spill table under profiles/).
+
+3. ``packed_fp32`` -- v_pk_add_f32, v_pk_mul_f32 and v_pk_fma_f32, some of whose forms have given wrong results now and then: the build
+   turns them off (``-packed-fp32-ops``), and a compiler that makes them all the same is found out here.
 """
 import re
 
@@ -23,6 +26,7 @@ EXEC_MOV = re.compile(r"^\s*s_mov_b64 exec, (s\[\d+:\d+\])")
 S_AND_DEF = re.compile(r"^\s*s_and(?:n2)?_b64 (s\[\d+:\d+\]),")
 SPILL_STORE = re.compile(r"^\s*(scratch_store|buffer_store)\S*\s.*Folded Spill")
 LABEL = re.compile(r"^(\.LBB\d+_\d+|[_A-Za-z][\w$.]*):")
+PACKED_FP32 = re.compile(r"^\s*v_pk_(add|mul|fma)_f32\b")
 TERMINATOR = re.compile(r"^\s*(s_cbranch|s_branch|s_endpgm|s_setpc)")
 
 
@@ -65,6 +69,18 @@ def scan_asm(text):
 def definite_hazards(text):
     findings, _ = scan_asm(text)
     return [(k, f) for k, lst in findings.items() for f in lst if f[4] == "definite"]
+
+
+def packed_fp32(text):
+    """-> [(kernel, line_no, instruction)]"""
+    found, kernel = [], None
+    for n, line in enumerate(text.split("\n"), 1):
+        m = LABEL.match(line)
+        if m and not m.group(1).startswith(".LBB"):
+            kernel = m.group(1)
+        elif PACKED_FP32.match(line):
+            found.append((kernel, n, line.strip()))
+    return found
 
 
 _INFO = {"sgpr": r"; TotalNumSgprs: (\d+)", "vgpr": r"; NumVgprs: (\d+)", "agpr": r"; NumAgprs: (\d+)", "scratch": r"; ScratchSize: (\d+)",

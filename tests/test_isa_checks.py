@@ -82,3 +82,40 @@ def test_shipped_build_is_clean(variant):
     for k in rep["kernels"]:
         cap = allowed.get(k["kernel"], 0) if variant is None else 64       # (the layout-fuzz builds reshuffle registers: a looser bound)
         assert k["scratch"] <= cap, f"{k['kernel']}: {k['scratch']} B of scratch per lane (allowed {cap})"
+
+
+PACKED = """
+_Z6kernelv:
+	v_pk_mul_f16 v0, v1, v2
+.LBB0_1:
+	v_pk_fma_f32 v[0:1], v[2:3], v[4:5], v[6:7] op_sel_hi:[1,0,1]
+	v_cvt_pk_bf16_f32 v0, v1, v2
+	v_pk_add_f32 v[0:1], v[2:3], v[4:5]
+	s_endpgm
+_Z5otherv:
+	v_fma_f32 v0, v1, v2, v3
+	v_pk_mul_f32 v[0:1], v[2:3], v[4:5]
+"""
+
+
+def test_scanner_finds_packed_fp32():
+    assert [(k, i.split()[0]) for k, _, i in isa_check.packed_fp32(PACKED)] == [("_Z6kernelv", "v_pk_fma_f32"), ("_Z6kernelv", "v_pk_add_f32"),
+                                                                               ("_Z5otherv", "v_pk_mul_f32")]
+    assert isa_check.packed_fp32(BAD) == []
+
+
+def test_build_refuses_packed_fp32(tmp_path, monkeypatch):
+    monkeypatch.setattr(build, "SOURCES", ["one.hip"])
+    (tmp_path / "one.gfx950.s").write_text(PACKED)
+    with pytest.raises(RuntimeError, match="packed fp32"):
+        build.check_isa(str(tmp_path), str(tmp_path / "lib.so"))
+    (tmp_path / "one.gfx950.s").write_text(GOOD)
+    assert build.check_isa(str(tmp_path), str(tmp_path / "lib.so"))["packed_fp32"] == []
+
+
+@pytest.mark.parametrize("variant", [None] + sorted(build.FUZZ_VARIANTS))
+def test_shipped_build_has_no_packed_fp32(variant):
+    path = build.isa_report_path(build.LIB if variant is None else build.variant_path(variant))
+    if not os.path.exists(path):
+        pytest.skip(f"{path}: library not built here (python -m mneslam_amd.build --fuzz)")
+    assert json.load(open(path))["packed_fp32"] == []
