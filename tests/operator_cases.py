@@ -1419,3 +1419,25 @@ def check_plan_tensors_are_apart(device):
         plan.order.fill_(-1)
         out.sum().backward()
         assert (x.grad == k).all() and plan.offsets.tolist() == [0] + [n * k] * e and plan.position.reshape(-1).tolist() == list(range(n * k))
+
+
+def check_adamw8_follows_32(device):
+    """A hundred steps with 8-bit moments go where 32-bit ones go.  The gradient is constant, so a step is lr, and every |m| and sqrt(v) of a
+    block lies between half its largest and that:
+    a code step of m is (2 c + 1) / c^2 of it, c >= 89: at most 2.3 %; a dither's deviation is at most half of that, and the running mean
+    with beta 0.9 holds 0.9 / sqrt(1 - 0.81) = 2.1 times one step's: 2.4 %.  Of sqrt(v): c >= 180, 0.56 %, and with beta 0.99 at most 7.1
+    times: 4.0 %.  One step is off by 4.7 % of lr (one deviation), the sum of a hundred by no more than that of a hundred lr: five
+    deviations are 24 %.  On average over n elements only the squares stay: (4.0 %)^2 from dividing by sqrt(v), and 0.0056^2 / 0.01 / 2
+    from v's mean, 0.32 % together; and 5 * 4.7 % / sqrt(n)."""
+    n, steps, lr = 256 * 64, 100, 2.0 ** -8
+    gen = torch.Generator().manual_seed(61)
+    g = ((0.5 + 0.5 * torch.rand(n, generator=gen)) * torch.where(torch.rand(n, generator=gen) < 0.5, -1.0, 1.0)).to(device)
+    ends = []
+    for bits in (8, 32):
+        p, state = torch.zeros(n, device=device), None
+        for step in range(1, steps + 1):
+            state = _step([p], [g], bits, device, step=step, state=state, lr=lr)
+        ends.append((p * -torch.sign(g)).double() / (steps * lr))
+    assert (ends[1] - 1).abs().max() < 1e-5
+    assert (ends[0] - 1).abs().max() < 0.24
+    assert abs(float(ends[0].mean()) - 1) < 0.0032 + 5 * 0.047 / n ** 0.5

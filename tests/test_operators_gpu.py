@@ -429,3 +429,7 @@ def test_adamw_outdates_what_it_writes():
 
 def test_plan_tensors_are_apart():
     oc.check_plan_tensors_are_apart(DEV)
+
+
+def test_adamw_8_follows_32():
+    oc.check_adamw8_follows_32(DEV)
