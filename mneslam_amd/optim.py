@@ -195,6 +195,8 @@ def _check_saved(p, st, bits):
     types = st["exp_avg"].dtype, st["exp_avg_sq"].dtype
     if all(t.is_floating_point for t in types) != (bits == 32):
         raise ValueError(f"a group with state_bits={bits} cannot go on from moments that are {types}")
+    if bits == 32 and "scales" in st:
+        raise ValueError("moments in 32 bits have no scales")
     if bits == 32:
         return
     if types != (torch.int8, torch.uint8):

@@ -1441,3 +1441,14 @@ def check_adamw8_follows_32(device):
     assert (ends[1] - 1).abs().max() < 1e-5
     assert (ends[0] - 1).abs().max() < 0.24
     assert abs(float(ends[0].mean()) - 1) < 0.0032 + 5 * 0.047 / n ** 0.5
+
+
+def check_fused_adamw_loads_no_scales_with_32_bits(device):
+    """Scales beside 32-bit moments would be taken for codes' by ``moments``: refused."""
+    p = torch.nn.Parameter(torch.ones(300, device=device))
+    saved = _stepped(p).state_dict()
+    saved = {**saved, "state": {0: {**saved["state"][0], "scales": torch.ones(2, 2)}}}
+    opt = _stepped(torch.nn.Parameter(torch.ones(300, device=device)))
+    with pytest.raises(ValueError, match="scales"):
+        opt.load_state_dict(saved)
+    assert "scales" not in opt.state[opt.param_groups[0]["params"][0]]

@@ -433,3 +433,7 @@ def test_plan_tensors_are_apart():
 
 def test_adamw_8_follows_32():
     oc.check_adamw8_follows_32(DEV)
+
+
+def test_fused_adamw_loads_no_scales_with_32_bits():
+    oc.check_fused_adamw_loads_no_scales_with_32_bits(DEV)
