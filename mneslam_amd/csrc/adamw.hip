@@ -21,8 +21,8 @@
 // the launch or on the machine.
 //
 // With 32-bit moments the step is bound by memory: 38.4 M fp32 values 180 us (28 bytes each, 6.0 TB/s), 67 M bf16 values in 256 tensors 250 us
-// (22 bytes, 5.9 TB/s).  With 8-bit ones it is where the parameters are fp32 (38.4 M: 95 us, 16 bytes, 6.5 TB/s); with bf16 parameters (10
-// bytes) it is bound by its 83 vector instructions an element, four of them roots and reciprocals: 67 M values 176 us (3.8 TB/s).
+// (22 bytes, 5.9 TB/s).  With 8-bit ones it is where the parameters are fp32 (38.4 M: 96 us, 16 bytes, 6.4 TB/s); with bf16 parameters (10
+// bytes) it is bound by its 83 vector instructions an element, four of them roots and reciprocals: 67 M values 169 us (4.0 TB/s).
 #include "mne_device.h"
 #include "mne_elem.h"
 #include "mne_launch.h"
